@@ -224,8 +224,7 @@ def _plain_plan(s):
     end = torch.cumsum(new, 0)
     start = torch.cat([end.new_zeros(1), end])
     first = (length + page - 1) // page
-    wanted = (length + new + page - 1) // page - first
-    need = torch.minimum(wanted, (wide - first).clamp(min=0))
+    need = torch.minimum((length + new + page - 1) // page, first.clamp(min=wide)) - first
     offset = torch.cumsum(need, 0) - need
     free = s["marks"][1] - s["marks"][0]
     granted = torch.minimum((free - offset).clamp(min=0), need)
@@ -237,10 +236,10 @@ def _plain_plan(s):
     position = length[episode] + row - start[episode]
     at = table[episode, (position // page).clamp(max=wide - 1)].long()
     slot = torch.where((at >= 0) & (position // page < wide), at * page + position % page, -1)
-    held = torch.minimum(length + new, (first + granted) * page)
-    marks = torch.stack([s["marks"][0] + granted.sum(), s["marks"][1], (wanted - granted).sum()])
+    held = torch.maximum(torch.minimum(length + new, (first + granted) * page), length)
+    marks = torch.stack([s["marks"][0] + granted.sum(), s["marks"][1], (length + new - held).sum()])
     return {"start": start.int(), "slot": slot, "episode": episode.int(), "position": position.int(), "table": table,
-            "length": torch.maximum(held, length).int(), "marks": marks}
+            "length": held.int(), "marks": marks}
 
 
 def _axis(sizes, interleaved):
