@@ -1,5 +1,5 @@
 """ctypes binding of ``libmkx.so`` (declarations in ``include/mkx.h``, ``include/mkx_prepare.h``,
-``include/mkx_mods.h`` and ``include/mkx_batch.h``).
+``include/mkx_mods.h``, ``include/mkx_batch.h`` and ``include/mkx_cache.h``).
 
 The library is built in-tree by ``reki_megakernel_b200.build``. There is no fallback: if the
 library is missing or does not load, importing this module raises.
@@ -68,6 +68,36 @@ class ModsDims(C.Structure):
     _fields_ = [("H", C.c_int), ("L", C.c_int), ("tdim", C.c_int), ("sdim", C.c_int)]
 
 
+class Rotary(C.Structure):
+    _fields_ = [("base", C.c_double), ("axes", C.c_int), ("sections", C.c_int * 4), ("interleaved", C.c_int)]
+
+
+class PlanInputs(C.Structure):
+    _fields_ = [(n, P) for n in ("length", "new_rows", "table", "ring", "marks", "start", "slot", "episode", "position",
+                                 "length_out", "marks_out", "ticket")] + [
+        (n, C.c_int) for n in ("B", "table_width", "ring_pages", "page_rows", "rows")]
+
+
+class ReleaseInputs(C.Structure):
+    _fields_ = [(n, P) for n in ("ended", "length", "table", "ring", "marks", "ticket")] + [
+        (n, C.c_int) for n in ("B", "table_width", "ring_pages", "page_rows")]
+
+
+class StoreInputs(C.Structure):
+    _fields_ = [(n, P) for n in ("q", "k", "v", "q_out", "k_pages", "v_pages", "slot", "positions")] + [
+        (n, C.c_longlong) for n in ("pos_stride", "q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "qo_row",
+                                    "qo_head", "kp_page", "kp_row", "kp_head", "vp_page", "vp_row", "vp_head")] + [
+        (n, C.c_int) for n in ("rows", "heads", "kv_heads", "head_dim", "dtype", "pages", "page_rows")] + [("rot", Rotary)]
+
+
+class AttendInputs(C.Structure):
+    _fields_ = [(n, P) for n in ("q", "k_pages", "v_pages", "out", "table", "length", "start", "workspace", "error")] + [
+        (n, C.c_longlong) for n in ("q_row", "q_head", "o_row", "o_head", "kp_page", "kp_row", "kp_head", "vp_page",
+                                    "vp_row", "vp_head")] + [
+        (n, C.c_int) for n in ("rows", "B", "heads", "kv_heads", "head_dim", "dtype", "pages", "page_rows",
+                               "table_width", "max_rows", "causal", "window", "sinks")] + [("scale", C.c_float)]
+
+
 SIGNATURES = {
     "mkx_create": (C.c_int, [C.POINTER(Dims), C.POINTER(Weights), C.c_int, C.POINTER(P)]),
     "mkx_run": (C.c_int, [P, C.POINTER(StepInputs), P]),
@@ -101,6 +131,13 @@ SIGNATURES = {
     "mkx_mods_input": (C.c_int, [P, P, P]),
     "mkx_mods_last_error": (C.c_int, [P, C.POINTER(C.c_int)]),
     "mkx_mods_destroy": (None, [P]),
+    "mkx_cache_plan": (C.c_int, [C.POINTER(PlanInputs), C.c_int, P]),
+    "mkx_cache_release": (C.c_int, [C.POINTER(ReleaseInputs), C.c_int, P]),
+    "mkx_rope_tables": (C.c_int, [C.POINTER(Rotary), P, C.c_longlong, C.c_int, C.c_int, P, P, C.c_int, P]),
+    "mkx_cache_store": (C.c_int, [C.POINTER(StoreInputs), C.c_int, P]),
+    "mkx_cache_attend": (C.c_int, [C.POINTER(AttendInputs), C.c_size_t, C.c_int, P]),
+    "mkx_attend_workspace": (C.c_size_t, [C.POINTER(AttendInputs), C.c_int]),
+    "mkx_cache_last_cuda_error": (C.c_char_p, []),
 }
 
 _LIB = None
@@ -156,6 +193,9 @@ def check(status: int, where: str) -> None:
     if status != MKX_OK:
         detail = ""
         if status == MKX_ERR_CUDA:
-            fn = load().mkx_batch_last_cuda_error if where.startswith("mkx_batch") else load().mkx_last_cuda_error
+            lib = load()
+            cache = where.startswith(("mkx_cache", "mkx_attend", "mkx_rope"))
+            fn = (lib.mkx_batch_last_cuda_error if where.startswith("mkx_batch") else
+                  lib.mkx_cache_last_cuda_error if cache else lib.mkx_last_cuda_error)
             detail = (fn() or b"").decode(errors="replace")
         raise MkxError(where, status, detail)

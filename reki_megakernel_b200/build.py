@@ -21,9 +21,12 @@ LIB = PKG / "libmkx.so"
 # %globaltimer at numbered points inside each stage); loaded only after _lib.use_traced_build().
 TRACE_LIB = PKG / "libmkx_trace.so"
 SOURCES = [PKG / "csrc" / "mk_expert.cu", PKG / "csrc" / "mk_prepare.cu", PKG / "csrc" / "mk_mods.cu",
-           PKG / "csrc" / "mk_batch.cu", PKG / "csrc" / "mk_copies.cu"]
-HEADERS = [PKG / "csrc" / "mkx_device.cuh", PKG / "csrc" / "mkx_tma.cuh", ROOT / "include" / "mkx.h",
-           ROOT / "include" / "mkx_prepare.h", ROOT / "include" / "mkx_mods.h", ROOT / "include" / "mkx_batch.h"]
+           PKG / "csrc" / "mk_batch.cu", PKG / "csrc" / "mk_copies.cu", PKG / "csrc" / "mk_cache.cu",
+           PKG / "csrc" / "mk_attend.cu"]
+HEADERS = [PKG / "csrc" / "mkx_device.cuh", PKG / "csrc" / "mkx_tma.cuh", PKG / "csrc" / "mkx_half.cuh",
+           PKG / "csrc" / "mkx_attend.cuh", PKG / "csrc" / "mkx_cache_host.h", ROOT / "include" / "mkx.h",
+           ROOT / "include" / "mkx_prepare.h", ROOT / "include" / "mkx_mods.h", ROOT / "include" / "mkx_batch.h",
+           ROOT / "include" / "mkx_cache.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -1,0 +1,410 @@
+"""Paged K/V cache of many episodes: placing new rows, storing them, and attention over them
+(``include/mkx_cache.h``).
+
+The expert reads K/V that are dense per episode ([SP, NH, HD] per layer, src/mk_expert.py:486-495);
+episodes of different lengths then all take the longest one's memory. Here the rows of all episodes
+share one pool of pages. One step of serving is
+
+1. ``plan_rows``: pages for the new rows of each episode, block tables and slot maps, from the
+   episodes' lengths, on the GPU (nothing is read back);
+2. ``write_rows``: rotary positions (one to four axes: index, or time / height / width of image rows)
+   on q and k, K and V rows to their slots, in one pass;
+3. ``attend``: the new rows over all rows of their episode -- single rows to long chunks, causal or
+   not, with a sliding window and first rows that stay visible.
+
+``EpisodeCache`` keeps the pools, tables and counters of such a cache. ``rope_tables`` makes the
+cos / sin tables of the same positions for ``RegisterPrepare.run`` and ``ExpertMegakernel.run``. All
+calls are asynchronous on the current stream of the tensors' device and can be captured in a CUDA
+graph. There is no CPU fallback: the CUDA library must load.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+import threading
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+
+DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+PAGE_ROWS = (16, 32, 64, 128, 256)
+HEAD_DIMS = (64, 128)          # of attend
+MAX_EPISODES = 4096
+MAX_ROWS = 1 << 30             # rows of one episode that a table can hold
+
+
+class RowPlan(NamedTuple):
+    """Where the new rows of a step go. start [B + 1] int32: first row of each episode; slot [rows] int64 (-1: none),
+    episode and position [rows] int32; length [B] int32 and marks [3] int64: the state after the step."""
+    start: torch.Tensor
+    slot: torch.Tensor
+    episode: torch.Tensor
+    position: torch.Tensor
+    length: torch.Tensor
+    marks: torch.Tensor
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _vector(t, name: str, n: int, dtype, device) -> None:
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} must be a contiguous {dtype} [{n}] tensor on {device}")
+
+
+def _cuda(t: torch.Tensor, name: str) -> torch.device:
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be on a CUDA device")
+    return t.device
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _strides(t: torch.Tensor, name: str):
+    """Strides of the leading dims, in elements; dims must be contiguous, the others multiples of 8 elements (16 bytes)
+    and the start 16-byte aligned. A dim of size one has no stride of its own."""
+    st, shape = t.stride(), t.shape
+    if shape[-1] > 1 and st[-1] != 1:
+        raise ValueError(f"{name}: the last dim must be contiguous")
+    out = [s if n > 1 else shape[-1] for s, n in zip(st[:-1], shape[:-1])]
+    if t.data_ptr() % 16 or any(s % 8 or s < 0 for s in out):
+        raise ValueError(f"{name}: rows, heads and pages must start on 16-byte boundaries")
+    return out
+
+
+# ---- placing ----------------------------------------------------------------------------------------
+
+def check_plan_args(length, new, table, free, marks, page_rows: int, rows: int) -> None:
+    """What ``plan_rows`` checks before it hands raw pointers to the library. Raises ValueError."""
+    dev, B = length.device, length.numel()
+    _need(1 <= B <= MAX_EPISODES, f"1 to {MAX_EPISODES} episodes")
+    _need(page_rows in PAGE_ROWS, f"page_rows must be one of {PAGE_ROWS}")
+    _need(0 <= rows < 1 << 31, "rows must be in 0 .. 2^31 - 1")
+    _vector(length, "length", B, torch.int32, dev)
+    _vector(new, "new", B, torch.int32, dev)
+    _vector(free, "free", free.numel(), torch.int32, dev)
+    _vector(marks, "marks", 3, torch.int64, dev)
+    _need(free.numel() >= 1, "free must hold at least one page")
+    _need(table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == B and table.shape[1] >= 1
+          and table.is_contiguous() and table.device == dev, f"table must be a contiguous int32 [{B}, pages] tensor on {dev}")
+    _need(table.shape[1] * page_rows <= MAX_ROWS, f"a table row may hold up to {MAX_ROWS} rows")
+
+
+def plan_rows(length: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free: torch.Tensor, marks: torch.Tensor, *,
+              page_rows: int, rows: int, out: RowPlan | None = None, ticket: torch.Tensor | None = None) -> RowPlan:
+    """Places ``new[b]`` rows behind the ``length[b]`` rows that episode b holds: pages off the ring ``free``, their
+    table entries (``table`` [B, pages] int32, written in place), and the new rows' start, slot, episode and position.
+
+    ``marks`` [3] int64: pages ever taken, pages ever returned (their difference is free, the next at
+    ``free[taken % len(free)]``), and, in the returned marks, the new rows that got no slot. ``rows``: how many rows
+    the step has room for; rows behind the last new one get slot -1. The returned length and marks are the state after
+    the step; ``out`` may name the arguments themselves (``out.length is length``) to advance them in place, then
+    ``ticket`` ([1] int32, zero) has to be a word that only plans of this state use."""
+    dev = _cuda(length, "length")
+    check_plan_args(length, new, table, free, marks, page_rows, rows)
+    B = length.shape[0]
+    if out is None:
+        e = torch.empty
+        out = RowPlan(e(B + 1, dtype=torch.int32, device=dev), e(rows, dtype=torch.int64, device=dev),
+                      e(rows, dtype=torch.int32, device=dev), e(rows, dtype=torch.int32, device=dev),
+                      e(B, dtype=torch.int32, device=dev), e(3, dtype=torch.int64, device=dev))
+    else:
+        for name, n, dt in (("start", B + 1, torch.int32), ("slot", rows, torch.int64), ("episode", rows, torch.int32),
+                            ("position", rows, torch.int32), ("length", B, torch.int32), ("marks", 3, torch.int64)):
+            _vector(getattr(out, name), f"out.{name}", n, dt, dev)
+    if ticket is None:
+        in_place = out.length.data_ptr() == length.data_ptr() or out.marks.data_ptr() == marks.data_ptr()
+        _need(not in_place, "advancing length or marks in place needs a ticket")
+    else:
+        _vector(ticket, "ticket", 1, torch.int32, dev)
+    a = _lib.PlanInputs(length.data_ptr(), new.data_ptr(), table.data_ptr(), free.data_ptr(), marks.data_ptr(),
+                        out.start.data_ptr(), out.slot.data_ptr(), out.episode.data_ptr(), out.position.data_ptr(),
+                        out.length.data_ptr(), out.marks.data_ptr(), ticket.data_ptr() if ticket is not None else None, B,
+                        table.shape[1],
+                        free.shape[0], page_rows, rows)
+    _lib.check(_lib.load().mkx_cache_plan(C.byref(a), dev.index, _stream(dev)), "mkx_cache_plan")
+    return out
+
+
+# ---- rotary positions and storing -------------------------------------------------------------------
+
+def _rotary(head_dim: int, sections, base: float, interleaved: bool) -> _lib.Rotary:
+    sections = tuple(sections) if sections is not None else (head_dim // 2,)
+    half = sum(sections)
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or half < 8 or half % 8 or 2 * half > head_dim:
+        raise ValueError(f"sections must be 1 to 4 counts whose sum is a multiple of 8 up to {head_dim // 2}")
+    if not (base > 0 and math.isfinite(base)):
+        raise ValueError("base must be positive")
+    return _lib.Rotary(base, len(sections), (C.c_int * 4)(*sections), int(interleaved))
+
+
+def _positions(positions: torch.Tensor, axes: int, rows: int, device) -> torch.Tensor:
+    if positions.dim() == 1:
+        positions = positions[None]
+    if (positions.dtype != torch.int32 or tuple(positions.shape) != (axes, rows) or positions.device != device
+            or (rows > 1 and positions.stride(1) != 1)):
+        raise ValueError(f"positions must be int32 [{axes}, {rows}] on {device}, each axis contiguous")
+    return positions
+
+
+def rope_tables(positions: torch.Tensor, head_dim: int, *, sections=None, base: float = 10000.0,
+                interleaved: bool = False):
+    """cos, sin [rows, head_dim] fp32 of ``positions`` [axes, rows] (or [rows]) int32, as ``RegisterPrepare.run`` and
+    ``ExpertMegakernel.run`` take them. Frequency i of ``sum(sections)`` (default: one axis, head_dim / 2) belongs to
+    dims i and i + sum(sections); see ``write_rows``."""
+    dev = _cuda(positions, "positions")
+    _need(16 <= head_dim <= 256 and head_dim % 16 == 0, "head_dim must be a multiple of 16 up to 256")
+    rot = _rotary(head_dim, sections, base, interleaved)
+    rows = positions.shape[-1]
+    positions = _positions(positions, rot.axes, rows, dev)
+    cos = torch.empty((rows, head_dim), dtype=torch.float32, device=dev)
+    sin = torch.empty_like(cos)
+    _lib.check(_lib.load().mkx_rope_tables(C.byref(rot), positions.data_ptr(), positions.stride(0), rows, head_dim,
+                                           cos.data_ptr(), sin.data_ptr(), dev.index, _stream(dev)), "mkx_rope_tables")
+    return cos, sin
+
+
+def check_write_args(k, v, slot, k_pages, v_pages, q, positions, out) -> None:
+    """What ``write_rows`` checks of shapes, types and devices. Raises ValueError."""
+    _need(k.dim() == 3 and k.shape == v.shape and k.shape[1] >= 1, "k and v must be [rows, kv_heads, head_dim] alike")
+    rows, heads, hd = k.shape
+    _need(k.dtype in DTYPES and 16 <= hd <= 256 and hd % 16 == 0,
+          "k must be bf16 or fp16 with a head_dim that is a multiple of 16 up to 256")
+    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and tuple(k_pages.shape[2:]) == (heads, hd)
+          and k_pages.shape[0] >= 1 and k_pages.shape[1] in PAGE_ROWS,
+          f"k_pages and v_pages must be [pages, page_rows, {heads}, {hd}] with page_rows in {PAGE_ROWS}")
+    for name, t in (("v", v), ("k_pages", k_pages), ("v_pages", v_pages)):
+        _need(t.dtype == k.dtype and t.device == k.device, f"{name} must be {k.dtype} on {k.device}")
+    _vector(slot, "slot", rows, torch.int64, k.device)
+    if q is None:
+        _need(out is None, "out belongs to q")
+        return
+    _need(positions is not None, "q is only rotated: it needs positions")
+    _need(q.dim() == 3 and q.shape[0] == rows and q.shape[1] >= 1 and q.shape[2] == hd and q.dtype == k.dtype
+          and q.device == k.device, f"q must be {k.dtype} [{rows}, heads, {hd}] on {k.device}")
+    if out is not None:
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, "out must be like q")
+
+
+def write_rows(k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, *,
+               q: torch.Tensor | None = None, positions: torch.Tensor | None = None, sections=None,
+               base: float = 10000.0, interleaved: bool = False, out: torch.Tensor | None = None):
+    """Stores rows ``k``, ``v`` [rows, kv_heads, head_dim] at ``slot`` [rows] int64 of the pages [pages, page_rows,
+    kv_heads, head_dim] (a slot outside of them is skipped; two rows must not share one). With ``positions``
+    [axes, rows] (or [rows]) int32, k is rotated on the way, and so is ``q`` [rows, heads, head_dim] into the returned
+    tensor (``out`` when given; ``out`` may be q).
+
+    Dims i and i + h, h = sum(sections), turn by positions[axis(i)] * base^(-i / h); dims from 2 h on pass through.
+    ``sections``: frequencies per axis (default: one axis with head_dim / 2); axis(i) goes through them one axis after
+    the other, or, ``interleaved``, over the axes in turn while each has some left. Tensors may be slices: dims
+    contiguous, rows, heads and pages on 16-byte boundaries."""
+    dev = _cuda(k, "k")
+    check_write_args(k, v, slot, k_pages, v_pages, q, positions, out)
+    rows, kv_heads, hd = k.shape
+    a = _lib.StoreInputs()
+    if positions is not None:
+        a.rot = rot = _rotary(hd, sections, base, interleaved)
+        positions = _positions(positions, rot.axes, rows, dev)
+        a.positions, a.pos_stride = positions.data_ptr(), positions.stride(0)
+    if q is not None:
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        a.q, a.q_out, a.heads = q.data_ptr(), out.data_ptr(), q.shape[1]
+        a.q_row, a.q_head = _strides(q, "q")
+        a.qo_row, a.qo_head = _strides(out, "out")
+    a.k, a.v, a.slot = k.data_ptr(), v.data_ptr(), slot.data_ptr()
+    a.k_pages, a.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
+    a.k_row, a.k_head = _strides(k, "k")
+    a.v_row, a.v_head = _strides(v, "v")
+    a.kp_page, a.kp_row, a.kp_head = _strides(k_pages, "k_pages")
+    a.vp_page, a.vp_row, a.vp_head = _strides(v_pages, "v_pages")
+    a.rows, a.kv_heads, a.head_dim, a.dtype = rows, kv_heads, hd, DTYPES[k.dtype]
+    a.pages, a.page_rows = k_pages.shape[0], k_pages.shape[1]
+    _lib.check(_lib.load().mkx_cache_store(C.byref(a), dev.index, _stream(dev)), "mkx_cache_store")
+    return out
+
+
+# ---- attention ----------------------------------------------------------------------------------------
+
+_TICKET_BYTES = 4096 * 4
+_lock = threading.Lock()
+_spaces: dict = {}   # (device index, stream) -> workspace of eager calls, which that stream keeps in order
+_errors: dict = {}   # device index -> error word, shared by all calls (it is only ever set)
+
+
+def _error_word(device) -> torch.Tensor:
+    with _lock:
+        t = _errors.get(device.index)
+        if t is None:
+            # not from a graph's pool, and zero before any stream can use it
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("call attend once before its first capture")
+            t = _errors[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+            torch.cuda.synchronize(device)
+    return t
+
+
+def _workspace(device, stream: int, size: int) -> torch.Tensor:
+    """``size`` bytes whose first words are zero between calls. Eager calls of one stream share one (the stream keeps
+    them in order); a captured call gets its own out of the graph's pool, zeroed by the graph, so that two graphs may
+    be replayed at once."""
+    if torch.cuda.is_current_stream_capturing():
+        t = torch.empty(size, dtype=torch.uint8, device=device)
+        t[:_TICKET_BYTES].zero_()
+        return t
+    with _lock:
+        t = _spaces.get((device.index, stream))
+        if t is None or t.numel() < size:
+            t = torch.empty(size, dtype=torch.uint8, device=device)
+            t[:_TICKET_BYTES].zero_()
+            _spaces[device.index, stream] = t
+    return t
+
+
+def check_attend_args(q, k_pages, v_pages, table, length, start, max_rows, causal, window, sinks, scale, out) -> None:
+    """What ``attend`` checks of shapes, types, devices and values. Raises ValueError."""
+    _need(q.dim() == 3 and q.dtype in DTYPES and q.shape[2] in HEAD_DIMS,
+          f"q must be bf16 or fp16 [rows, heads, head_dim], head_dim in {HEAD_DIMS}")
+    rows, heads, hd = q.shape
+    dev = q.device
+    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.shape[3] == hd and k_pages.shape[0] >= 1
+          and k_pages.shape[1] in PAGE_ROWS and k_pages.shape[2] >= 1,
+          f"k_pages and v_pages must be [pages, page_rows, kv_heads, {hd}] with page_rows in {PAGE_ROWS}")
+    _need(heads >= 1 and heads % k_pages.shape[2] == 0, "heads must be a multiple of kv_heads")
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        _need(t.dtype == q.dtype and t.device == dev, f"{name} must be {q.dtype} on {dev}")
+    B = length.numel()
+    _need(1 <= B <= MAX_EPISODES, f"1 to {MAX_EPISODES} episodes")
+    _vector(length, "length", B, torch.int32, dev)
+    _vector(start, "start", B + 1, torch.int32, dev)
+    _need(table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == B and table.shape[1] >= 1
+          and table.is_contiguous() and table.device == dev, f"table must be a contiguous int32 [{B}, pages] tensor on {dev}")
+    _need(table.shape[1] * k_pages.shape[1] <= MAX_ROWS, f"a table row may hold up to {MAX_ROWS} rows")
+    _need(max_rows is None or max_rows >= 0, "max_rows must not be negative")
+    _need(window >= 0 and sinks >= 0, "window and sinks must not be negative")
+    _need(causal or window == 0, "a window needs causal=True")
+    _need(window > 0 or sinks == 0, "sinks are the rows that stay visible beside a window")
+    _need(scale is None or math.isfinite(scale), "scale must be finite")
+    if out is not None:
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == dev, "out must be like q")
+
+
+def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, length: torch.Tensor,
+           start: torch.Tensor, *, max_rows: int | None = None, causal: bool = True, window: int = 0, sinks: int = 0,
+           scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the new rows ``q`` [rows, heads, head_dim] over the pages [pages, page_rows, kv_heads, head_dim];
+    heads / kv_heads query heads share a K/V head. Rows ``start[b] .. start[b + 1] - 1`` are the last ones of the
+    ``length[b]`` rows of episode b (stored before: see ``write_rows``), whose row j lies in page
+    ``table[b, j // page_rows]``.
+
+    A row at position p sees the rows j < length[b] of its episode with j <= p (all of them if not ``causal``) and,
+    with a ``window`` > 0, with j > p - window or j < ``sinks``. out = softmax(scale q k^T) v (scale: 1 / sqrt(head_dim)),
+    zero for a row that sees nothing; rows behind start[B] are left as they were. What pages hold beyond an
+    episode's length does not matter; the K and V rows below it are finite. ``max_rows``: no episode has more new rows
+    (default: q's rows); a tight value picks the kernel that fits. A wait that ran out on the device surfaces in
+    ``check_device_error()``."""
+    dev = _cuda(q, "q")
+    check_attend_args(q, k_pages, v_pages, table, length, start, max_rows, causal, window, sinks, scale, out)
+    rows, heads, hd = q.shape
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if rows == 0:
+        return out
+    lib, stream = _lib.load(), _stream(dev)
+    big = (1 << 31) - 1
+    a = _lib.AttendInputs(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), table.data_ptr(), length.data_ptr(),
+        start.data_ptr(), 0, _error_word(dev).data_ptr(), *_strides(q, "q"), *_strides(out, "out"),
+        *_strides(k_pages, "k_pages"), *_strides(v_pages, "v_pages"), rows, length.shape[0], heads, k_pages.shape[2], hd,
+        DTYPES[q.dtype], k_pages.shape[0], k_pages.shape[1], table.shape[1], rows if max_rows is None else min(max_rows, rows),
+        int(causal), min(window, big), min(sinks, big), 1.0 / math.sqrt(hd) if scale is None else scale)
+    size = lib.mkx_attend_workspace(C.byref(a), dev.index)
+    with torch.cuda.device(dev):
+        space = _workspace(dev, stream, max(size, _TICKET_BYTES))
+    a.workspace = space.data_ptr()
+    _lib.check(lib.mkx_cache_attend(C.byref(a), space.numel(), dev.index, stream), "mkx_cache_attend")
+    return out
+
+
+def check_device_error(device=None) -> None:
+    """Raises if a bounded wait of an ``attend`` on ``device`` ran out since the last check (synchronises)."""
+    index = torch.device("cuda", torch.cuda.current_device()).index if device is None else torch.device(device).index or 0
+    word = _errors.get(index)
+    if word is not None:
+        code = int(word.item())
+        if code:
+            word.zero_()
+            raise _lib.MkxError("attend", _lib.MKX_ERR_DEVICE, f"error word {code:#x}")
+
+
+# ---- the cache ------------------------------------------------------------------------------------------
+
+class EpisodeCache:
+    """Pools, tables and counters of a paged cache: ``EpisodeCache(layers=..., pages=..., episodes=...)``.
+
+    k, v [layers, pages, page_rows, kv_heads, head_dim]; table [episodes, pages_per_episode] int32; length [episodes]
+    int32; free [pages] int32 (a ring) and marks [3] int64. One step:
+
+        plan = cache.plan(new, rows)                 # new [episodes] int32 rows per episode, sum <= rows
+        q = cache.write(layer, k, v, plan, q=q, positions=..., sections=...)
+        out = cache.attend(layer, q, plan, max_rows=..., window=..., sinks=...)
+
+    ``plan`` advances the state in place (in stream order), so a captured step can be replayed. ``release`` returns
+    the pages of episodes that ended."""
+
+    def __init__(self, *, layers: int, pages: int, episodes: int, page_rows: int = 32, kv_heads: int = 12,
+                 head_dim: int = 64, pages_per_episode: int | None = None, dtype=torch.bfloat16, device="cuda"):
+        dev = torch.device(device)
+        _need(dev.type == "cuda", "EpisodeCache needs a CUDA device")
+        if dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        _need(layers >= 1 and pages >= 1 and kv_heads >= 1, "layers, pages and kv_heads must be positive")
+        _need(1 <= episodes <= MAX_EPISODES, f"1 to {MAX_EPISODES} episodes")
+        _need(page_rows in PAGE_ROWS, f"page_rows must be one of {PAGE_ROWS}")
+        _need(head_dim in HEAD_DIMS and dtype in DTYPES, f"head_dim in {HEAD_DIMS}, bf16 or fp16")
+        wide = pages if pages_per_episode is None else pages_per_episode
+        _need(wide >= 1 and wide * page_rows <= MAX_ROWS, f"an episode may hold up to {MAX_ROWS} rows")
+        _lib.load()
+        _error_word(dev)
+        self.device, self.page_rows, self.episodes = dev, page_rows, episodes
+        self.k = torch.zeros((layers, pages, page_rows, kv_heads, head_dim), dtype=dtype, device=dev)
+        self.v = torch.zeros_like(self.k)
+        self.table = torch.full((episodes, wide), -1, dtype=torch.int32, device=dev)
+        self.length = torch.zeros(episodes, dtype=torch.int32, device=dev)
+        self.free = torch.arange(pages, dtype=torch.int32, device=dev)
+        self.marks = torch.tensor([0, pages, 0], dtype=torch.int64, device=dev)
+        self._ticket = torch.zeros(1, dtype=torch.int32, device=dev)
+
+    def plan(self, new: torch.Tensor, rows: int) -> RowPlan:
+        """Places ``new`` [episodes] int32 rows (device); ``rows`` is the room of the step's row tensors. The plan's
+        length and marks are the cache's own. Rows without a slot are counted in ``marks[2]``."""
+        dev, e = self.device, torch.empty
+        out = RowPlan(e(self.episodes + 1, dtype=torch.int32, device=dev), e(rows, dtype=torch.int64, device=dev),
+                      e(rows, dtype=torch.int32, device=dev), e(rows, dtype=torch.int32, device=dev), self.length, self.marks)
+        return plan_rows(self.length, new, self.table, self.free, self.marks, page_rows=self.page_rows, rows=rows, out=out,
+                         ticket=self._ticket)
+
+    def release(self, ended: torch.Tensor) -> None:
+        """Returns all pages of the episodes with ``ended`` [episodes] (bool) to the free ring, length 0."""
+        _vector(ended, "ended", self.episodes, torch.bool, self.device)
+        a = _lib.ReleaseInputs(ended.data_ptr(), self.length.data_ptr(), self.table.data_ptr(), self.free.data_ptr(),
+                               self.marks.data_ptr(), self._ticket.data_ptr(), self.episodes, self.table.shape[1],
+                               self.free.shape[0], self.page_rows)
+        _lib.check(_lib.load().mkx_cache_release(C.byref(a), self.device.index, _stream(self.device)), "mkx_cache_release")
+
+    def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, plan: RowPlan, **kw):
+        """``write_rows`` into the pages of ``layer``."""
+        return write_rows(k, v, plan.slot, self.k[layer], self.v[layer], **kw)
+
+    def attend(self, layer: int, q: torch.Tensor, plan: RowPlan, **kw) -> torch.Tensor:
+        """``attend`` over the pages of ``layer``."""
+        return attend(q, self.k[layer], self.v[layer], self.table, self.length, plan.start, **kw)
+
+    def check_device_error(self) -> None:
+        check_device_error(self.device)

@@ -14,6 +14,7 @@ from types import SimpleNamespace
 import torch
 
 from . import _lib
+from .episode_cache import rope_tables
 from .synthetic import PrepareWeights, rope_cos_sin
 
 
@@ -65,14 +66,21 @@ class RegisterPrepare:
         return t
 
     def run(self, src: torch.Tensor, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
-            SP: int | None = None, out=None):
+            SP: int | None = None, out=None, *, positions: torch.Tensor | None = None, sections=None,
+            interleaved: bool = False):
+        """K and V of the source rows; their RoPE tables are ``cos`` / ``sin``, or those of ``positions`` [axes, S] int32
+        (time, height, width of image rows: ``episode_cache.rope_tables``), or of the row indexes."""
         d = self.dims
         if src.dim() != 2 or src.shape[1] != d.src_dim or src.dtype != torch.bfloat16 or src.device != self.device:
             raise ValueError(f"src must be [S, {d.src_dim}] bf16 on {self.device}")
         src = src.contiguous()
         S = src.shape[0]
         SP = SP or S
-        if cos is None or sin is None:
+        if positions is not None:
+            if cos is not None or sin is not None:
+                raise ValueError("give positions or tables, not both")
+            cos, sin = rope_tables(positions, d.HD, sections=sections, interleaved=interleaved)
+        elif cos is None or sin is None:
             cos, sin = self.tables(S)
         check_run_args(d, self.device, S, SP, cos, sin, out)
         if out is None:
