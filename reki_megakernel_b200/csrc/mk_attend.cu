@@ -21,6 +21,7 @@ namespace mkxa {
 namespace {
 
 constexpr int MT = 16;
+using mkxc::MAX_DEVICES;
 constexpr int MAX_KEYS = 1 << 30;  // rows of an episode: keys and positions are 32-bit
 constexpr int ROW_WARPS = 4;
 constexpr int ROW_THREADS = 32 * (ROW_WARPS + 1);
@@ -383,10 +384,15 @@ bool plan_of(const mkx_attend_inputs& a, int sms, Plan& pl) {
 }
 
 template <int DT, int HD>
-bool launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const AttendParams& p, long long grid, cudaStream_t stream) {
-  if (!mkxc::cuda_ok(cudaFuncSetAttribute(rows_kernel<DT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          RowShape<HD>::SMEM)))
-    return false;
+bool launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const AttendParams& p, long long grid, int device,
+                 cudaStream_t stream) {
+  static bool sized[MAX_DEVICES] = {};  // the attribute of this kernel is set once per device
+  if (!sized[device]) {
+    if (!mkxc::cuda_ok(cudaFuncSetAttribute(rows_kernel<DT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            RowShape<HD>::SMEM)))
+      return false;
+    sized[device] = true;
+  }
   rows_kernel<DT, HD><<<(unsigned)grid, ROW_THREADS, RowShape<HD>::SMEM, stream>>>(tk, tv, p);
   return mkxc::cuda_ok(cudaGetLastError());
 }
@@ -467,9 +473,9 @@ extern "C" mkx_status mkx_cache_attend(const mkx_attend_inputs* in, size_t works
   p.min_blocks = 2;
   p.max_parts = pl.max_parts;
   p.timeout_ns = 2000000000ull;
-  const bool ok = a.head_dim == 64 ? (a.dtype == MKX_BF16 ? launch_rows<MKX_BF16, 64>(tk, tv, p, pl.grid, stream)
-                                                          : launch_rows<MKX_FP16, 64>(tk, tv, p, pl.grid, stream))
-                                   : (a.dtype == MKX_BF16 ? launch_rows<MKX_BF16, 128>(tk, tv, p, pl.grid, stream)
-                                                          : launch_rows<MKX_FP16, 128>(tk, tv, p, pl.grid, stream));
+  const bool ok = a.head_dim == 64 ? (a.dtype == MKX_BF16 ? launch_rows<MKX_BF16, 64>(tk, tv, p, pl.grid, device, stream)
+                                                          : launch_rows<MKX_FP16, 64>(tk, tv, p, pl.grid, device, stream))
+                                   : (a.dtype == MKX_BF16 ? launch_rows<MKX_BF16, 128>(tk, tv, p, pl.grid, device, stream)
+                                                          : launch_rows<MKX_FP16, 128>(tk, tv, p, pl.grid, device, stream));
   return ok ? MKX_OK : MKX_ERR_CUDA;
 }

@@ -413,8 +413,8 @@ int page_shift(int page_rows) {
 }
 
 int sm_count(int device) {
-  static int known[64] = {};
-  if (device < 0 || device >= 64) return 0;
+  static int known[MAX_DEVICES] = {};
+  if (device < 0 || device >= MAX_DEVICES) return 0;
   if (known[device] == 0) {
     int n = 0;
     if (!cuda_ok(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device))) return 0;

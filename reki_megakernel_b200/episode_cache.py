@@ -46,14 +46,21 @@ class RowPlan(NamedTuple):
     marks: torch.Tensor
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
+# A call on a few rows is over on the GPU in a few microseconds: the checks below build their messages only when they
+# refuse, and read each property of a tensor once.
 
 def _vector(t, name: str, n: int, dtype, device) -> None:
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != device:
+    if t.dtype != dtype or t.shape != (n,) or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} [{n}] tensor on {device}")
+
+
+def _check_table(table, B: int, page_rows: int, device) -> None:
+    shape = table.shape
+    if (len(shape) != 2 or shape[0] != B or shape[1] < 1 or table.dtype != torch.int32 or table.device != device
+            or not table.is_contiguous()):
+        raise ValueError(f"table must be a contiguous int32 [{B}, pages] tensor on {device}")
+    if shape[1] * page_rows > MAX_ROWS:
+        raise ValueError(f"a table row may hold up to {MAX_ROWS} rows")
 
 
 def _cuda(t: torch.Tensor, name: str) -> torch.device:
@@ -63,7 +70,7 @@ def _cuda(t: torch.Tensor, name: str) -> torch.device:
 
 
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)  # torch.cuda.current_stream builds an object: 2 us
 
 
 def _strides(t: torch.Tensor, name: str):
@@ -83,17 +90,17 @@ def _strides(t: torch.Tensor, name: str):
 def check_plan_args(length, new, table, free, marks, page_rows: int, rows: int) -> None:
     """What ``plan_rows`` checks before it hands raw pointers to the library. Raises ValueError."""
     dev, B = length.device, length.numel()
-    _need(1 <= B <= MAX_EPISODES, f"1 to {MAX_EPISODES} episodes")
-    _need(page_rows in PAGE_ROWS, f"page_rows must be one of {PAGE_ROWS}")
-    _need(0 <= rows < 1 << 31, "rows must be in 0 .. 2^31 - 1")
+    if not 1 <= B <= MAX_EPISODES:
+        raise ValueError(f"1 to {MAX_EPISODES} episodes")
+    if page_rows not in PAGE_ROWS:
+        raise ValueError(f"page_rows must be one of {PAGE_ROWS}")
+    if not 0 <= rows < 1 << 31:
+        raise ValueError("rows must be in 0 .. 2^31 - 1")
     _vector(length, "length", B, torch.int32, dev)
     _vector(new, "new", B, torch.int32, dev)
-    _vector(free, "free", free.numel(), torch.int32, dev)
+    _vector(free, "free", max(1, free.numel()), torch.int32, dev)
     _vector(marks, "marks", 3, torch.int64, dev)
-    _need(free.numel() >= 1, "free must hold at least one page")
-    _need(table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == B and table.shape[1] >= 1
-          and table.is_contiguous() and table.device == dev, f"table must be a contiguous int32 [{B}, pages] tensor on {dev}")
-    _need(table.shape[1] * page_rows <= MAX_ROWS, f"a table row may hold up to {MAX_ROWS} rows")
+    _check_table(table, B, page_rows, dev)
 
 
 def plan_rows(length: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free: torch.Tensor, marks: torch.Tensor, *,
@@ -110,17 +117,20 @@ def plan_rows(length: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free
     check_plan_args(length, new, table, free, marks, page_rows, rows)
     B = length.shape[0]
     if out is None:
-        e = torch.empty
-        out = RowPlan(e(B + 1, dtype=torch.int32, device=dev), e(rows, dtype=torch.int64, device=dev),
-                      e(rows, dtype=torch.int32, device=dev), e(rows, dtype=torch.int32, device=dev),
-                      e(B, dtype=torch.int32, device=dev), e(3, dtype=torch.int64, device=dev))
+        # one allocation: slot, marks, position, episode, each on a 16-byte boundary, then length and start
+        pad = -rows % 4
+        slot, _, m, _, position, _, episode, _, after, start = torch.empty(
+            4 * (rows + pad) + 8 + 2 * B + 1, dtype=torch.int32, device=dev).split_with_sizes(
+                [2 * rows, 2 * pad, 6, 2, rows, pad, rows, pad, B, B + 1])
+        out = RowPlan(start, slot.view(torch.int64), episode, position, after, m.view(torch.int64))
     else:
         for name, n, dt in (("start", B + 1, torch.int32), ("slot", rows, torch.int64), ("episode", rows, torch.int32),
                             ("position", rows, torch.int32), ("length", B, torch.int32), ("marks", 3, torch.int64)):
             _vector(getattr(out, name), f"out.{name}", n, dt, dev)
     if ticket is None:
         in_place = out.length.data_ptr() == length.data_ptr() or out.marks.data_ptr() == marks.data_ptr()
-        _need(not in_place, "advancing length or marks in place needs a ticket")
+        if in_place:
+            raise ValueError("advancing length or marks in place needs a ticket")
     else:
         _vector(ticket, "ticket", 1, torch.int32, dev)
     a = _lib.PlanInputs(length.data_ptr(), new.data_ptr(), table.data_ptr(), free.data_ptr(), marks.data_ptr(),
@@ -159,7 +169,8 @@ def rope_tables(positions: torch.Tensor, head_dim: int, *, sections=None, base: 
     ``ExpertMegakernel.run`` take them. Frequency i of ``sum(sections)`` (default: one axis, head_dim / 2) belongs to
     dims i and i + sum(sections); see ``write_rows``."""
     dev = _cuda(positions, "positions")
-    _need(16 <= head_dim <= 256 and head_dim % 16 == 0, "head_dim must be a multiple of 16 up to 256")
+    if not 16 <= head_dim <= 256 or head_dim % 16:
+        raise ValueError("head_dim must be a multiple of 16 up to 256")
     rot = _rotary(head_dim, sections, base, interleaved)
     rows = positions.shape[-1]
     positions = _positions(positions, rot.axes, rows, dev)
@@ -172,24 +183,33 @@ def rope_tables(positions: torch.Tensor, head_dim: int, *, sections=None, base: 
 
 def check_write_args(k, v, slot, k_pages, v_pages, q, positions, out) -> None:
     """What ``write_rows`` checks of shapes, types and devices. Raises ValueError."""
-    _need(k.dim() == 3 and k.shape == v.shape and k.shape[1] >= 1, "k and v must be [rows, kv_heads, head_dim] alike")
-    rows, heads, hd = k.shape
-    _need(k.dtype in DTYPES and 16 <= hd <= 256 and hd % 16 == 0,
-          "k must be bf16 or fp16 with a head_dim that is a multiple of 16 up to 256")
-    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and tuple(k_pages.shape[2:]) == (heads, hd)
-          and k_pages.shape[0] >= 1 and k_pages.shape[1] in PAGE_ROWS,
-          f"k_pages and v_pages must be [pages, page_rows, {heads}, {hd}] with page_rows in {PAGE_ROWS}")
-    for name, t in (("v", v), ("k_pages", k_pages), ("v_pages", v_pages)):
-        _need(t.dtype == k.dtype and t.device == k.device, f"{name} must be {k.dtype} on {k.device}")
-    _vector(slot, "slot", rows, torch.int64, k.device)
+    shape, dtype, dev = k.shape, k.dtype, k.device
+    if len(shape) != 3 or v.shape != shape or shape[1] < 1:
+        raise ValueError("k and v must be [rows, kv_heads, head_dim] alike")
+    rows, heads, hd = shape
+    if dtype not in DTYPES or not 16 <= hd <= 256 or hd % 16:
+        raise ValueError("k must be bf16 or fp16 with a head_dim that is a multiple of 16 up to 256")
+    pool = k_pages.shape
+    if (len(pool) != 4 or v_pages.shape != pool or pool[2] != heads or pool[3] != hd or pool[0] < 1
+            or pool[1] not in PAGE_ROWS):
+        raise ValueError(f"k_pages and v_pages must be [pages, page_rows, {heads}, {hd}] with page_rows in {PAGE_ROWS}")
+    if v.dtype != dtype or v.device != dev:
+        raise ValueError(f"v must be {dtype} on {dev}")
+    for t in (k_pages, v_pages):
+        if t.dtype != dtype or t.device != dev:
+            raise ValueError(f"k_pages and v_pages must be {dtype} on {dev}")
+    _vector(slot, "slot", rows, torch.int64, dev)
     if q is None:
-        _need(out is None, "out belongs to q")
+        if out is not None:
+            raise ValueError("out belongs to q")
         return
-    _need(positions is not None, "q is only rotated: it needs positions")
-    _need(q.dim() == 3 and q.shape[0] == rows and q.shape[1] >= 1 and q.shape[2] == hd and q.dtype == k.dtype
-          and q.device == k.device, f"q must be {k.dtype} [{rows}, heads, {hd}] on {k.device}")
-    if out is not None:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, "out must be like q")
+    if positions is None:
+        raise ValueError("q is only rotated: it needs positions")
+    qs = q.shape
+    if len(qs) != 3 or qs[0] != rows or qs[1] < 1 or qs[2] != hd or q.dtype != dtype or q.device != dev:
+        raise ValueError(f"q must be {dtype} [{rows}, heads, {hd}] on {dev}")
+    if out is not None and (out.shape != qs or out.dtype != dtype or out.device != dev):
+        raise ValueError("out must be like q")
 
 
 def write_rows(k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, *,
@@ -214,7 +234,7 @@ def write_rows(k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, k_pages: to
         a.positions, a.pos_stride = positions.data_ptr(), positions.stride(0)
     if q is not None:
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            out = torch.empty_like(q)
         a.q, a.q_out, a.heads = q.data_ptr(), out.data_ptr(), q.shape[1]
         a.q_row, a.q_head = _strides(q, "q")
         a.qo_row, a.qo_head = _strides(out, "out")
@@ -243,18 +263,25 @@ def _error_word(device) -> torch.Tensor:
         t = _errors.get(device.index)
         if t is None:
             # not from a graph's pool, and zero before any stream can use it
-            if torch.cuda.is_current_stream_capturing():
+            if _capturing(device):
                 raise RuntimeError("call attend once before its first capture")
             t = _errors[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
             torch.cuda.synchronize(device)
     return t
 
 
+def _capturing(device) -> bool:
+    if torch._C._cuda_getDevice() == device.index:
+        return torch._C._cuda_isCurrentStreamCapturing()
+    with torch.cuda.device(device):
+        return torch._C._cuda_isCurrentStreamCapturing()
+
+
 def _workspace(device, stream: int, size: int) -> torch.Tensor:
     """``size`` bytes whose first words are zero between calls. Eager calls of one stream share one (the stream keeps
     them in order); a captured call gets its own out of the graph's pool, zeroed by the graph, so that two graphs may
     be replayed at once."""
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing(device):
         t = torch.empty(size, dtype=torch.uint8, device=device)
         t[:_TICKET_BYTES].zero_()
         return t
@@ -269,30 +296,36 @@ def _workspace(device, stream: int, size: int) -> torch.Tensor:
 
 def check_attend_args(q, k_pages, v_pages, table, length, start, max_rows, causal, window, sinks, scale, out) -> None:
     """What ``attend`` checks of shapes, types, devices and values. Raises ValueError."""
-    _need(q.dim() == 3 and q.dtype in DTYPES and q.shape[2] in HEAD_DIMS,
-          f"q must be bf16 or fp16 [rows, heads, head_dim], head_dim in {HEAD_DIMS}")
-    rows, heads, hd = q.shape
-    dev = q.device
-    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.shape[3] == hd and k_pages.shape[0] >= 1
-          and k_pages.shape[1] in PAGE_ROWS and k_pages.shape[2] >= 1,
-          f"k_pages and v_pages must be [pages, page_rows, kv_heads, {hd}] with page_rows in {PAGE_ROWS}")
-    _need(heads >= 1 and heads % k_pages.shape[2] == 0, "heads must be a multiple of kv_heads")
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        _need(t.dtype == q.dtype and t.device == dev, f"{name} must be {q.dtype} on {dev}")
+    shape, dtype, dev = q.shape, q.dtype, q.device
+    if len(shape) != 3 or dtype not in DTYPES or shape[2] not in HEAD_DIMS:
+        raise ValueError(f"q must be bf16 or fp16 [rows, heads, head_dim], head_dim in {HEAD_DIMS}")
+    pool = k_pages.shape
+    if (len(pool) != 4 or v_pages.shape != pool or pool[3] != shape[2] or pool[0] < 1 or pool[1] not in PAGE_ROWS
+            or pool[2] < 1):
+        raise ValueError(f"k_pages and v_pages must be [pages, page_rows, kv_heads, {shape[2]}] with page_rows in {PAGE_ROWS}")
+    if shape[1] < 1 or shape[1] % pool[2]:
+        raise ValueError("heads must be a multiple of kv_heads")
+    for t in (k_pages, v_pages):
+        if t.dtype != dtype or t.device != dev:
+            raise ValueError(f"k_pages and v_pages must be {dtype} on {dev}")
     B = length.numel()
-    _need(1 <= B <= MAX_EPISODES, f"1 to {MAX_EPISODES} episodes")
+    if not 1 <= B <= MAX_EPISODES:
+        raise ValueError(f"1 to {MAX_EPISODES} episodes")
     _vector(length, "length", B, torch.int32, dev)
     _vector(start, "start", B + 1, torch.int32, dev)
-    _need(table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == B and table.shape[1] >= 1
-          and table.is_contiguous() and table.device == dev, f"table must be a contiguous int32 [{B}, pages] tensor on {dev}")
-    _need(table.shape[1] * k_pages.shape[1] <= MAX_ROWS, f"a table row may hold up to {MAX_ROWS} rows")
-    _need(max_rows is None or max_rows >= 0, "max_rows must not be negative")
-    _need(window >= 0 and sinks >= 0, "window and sinks must not be negative")
-    _need(causal or window == 0, "a window needs causal=True")
-    _need(window > 0 or sinks == 0, "sinks are the rows that stay visible beside a window")
-    _need(scale is None or math.isfinite(scale), "scale must be finite")
-    if out is not None:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == dev, "out must be like q")
+    _check_table(table, B, pool[1], dev)
+    if max_rows is not None and max_rows < 0:
+        raise ValueError("max_rows must not be negative")
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks must not be negative")
+    if window > 0 and not causal:
+        raise ValueError("a window needs causal=True")
+    if sinks > 0 and window == 0:
+        raise ValueError("sinks are the rows that stay visible beside a window")
+    if scale is not None and not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    if out is not None and (out.shape != shape or out.dtype != dtype or out.device != dev):
+        raise ValueError("out must be like q")
 
 
 def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, length: torch.Tensor,
@@ -313,7 +346,7 @@ def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table:
     check_attend_args(q, k_pages, v_pages, table, length, start, max_rows, causal, window, sinks, scale, out)
     rows, heads, hd = q.shape
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q)
     if rows == 0:
         return out
     lib, stream = _lib.load(), _stream(dev)
@@ -324,9 +357,7 @@ def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table:
         *_strides(k_pages, "k_pages"), *_strides(v_pages, "v_pages"), rows, length.shape[0], heads, k_pages.shape[2], hd,
         DTYPES[q.dtype], k_pages.shape[0], k_pages.shape[1], table.shape[1], rows if max_rows is None else min(max_rows, rows),
         int(causal), min(window, big), min(sinks, big), 1.0 / math.sqrt(hd) if scale is None else scale)
-    size = lib.mkx_attend_workspace(C.byref(a), dev.index)
-    with torch.cuda.device(dev):
-        space = _workspace(dev, stream, max(size, _TICKET_BYTES))
+    space = _workspace(dev, stream, max(lib.mkx_attend_workspace(C.byref(a), dev.index), _TICKET_BYTES))
     a.workspace = space.data_ptr()
     _lib.check(lib.mkx_cache_attend(C.byref(a), space.numel(), dev.index, stream), "mkx_cache_attend")
     return out
@@ -361,15 +392,21 @@ class EpisodeCache:
     def __init__(self, *, layers: int, pages: int, episodes: int, page_rows: int = 32, kv_heads: int = 12,
                  head_dim: int = 64, pages_per_episode: int | None = None, dtype=torch.bfloat16, device="cuda"):
         dev = torch.device(device)
-        _need(dev.type == "cuda", "EpisodeCache needs a CUDA device")
+        if dev.type != "cuda":
+            raise ValueError("EpisodeCache needs a CUDA device")
         if dev.index is None:
             dev = torch.device("cuda", torch.cuda.current_device())
-        _need(layers >= 1 and pages >= 1 and kv_heads >= 1, "layers, pages and kv_heads must be positive")
-        _need(1 <= episodes <= MAX_EPISODES, f"1 to {MAX_EPISODES} episodes")
-        _need(page_rows in PAGE_ROWS, f"page_rows must be one of {PAGE_ROWS}")
-        _need(head_dim in HEAD_DIMS and dtype in DTYPES, f"head_dim in {HEAD_DIMS}, bf16 or fp16")
+        if layers < 1 or pages < 1 or kv_heads < 1:
+            raise ValueError("layers, pages and kv_heads must be positive")
+        if not 1 <= episodes <= MAX_EPISODES:
+            raise ValueError(f"1 to {MAX_EPISODES} episodes")
+        if page_rows not in PAGE_ROWS:
+            raise ValueError(f"page_rows must be one of {PAGE_ROWS}")
+        if head_dim not in HEAD_DIMS or dtype not in DTYPES:
+            raise ValueError(f"head_dim in {HEAD_DIMS}, bf16 or fp16")
         wide = pages if pages_per_episode is None else pages_per_episode
-        _need(wide >= 1 and wide * page_rows <= MAX_ROWS, f"an episode may hold up to {MAX_ROWS} rows")
+        if wide < 1 or wide * page_rows > MAX_ROWS:
+            raise ValueError(f"an episode may hold up to {MAX_ROWS} rows")
         _lib.load()
         _error_word(dev)
         self.device, self.page_rows, self.episodes = dev, page_rows, episodes
