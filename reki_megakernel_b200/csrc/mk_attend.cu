@@ -142,8 +142,8 @@ __global__ void __launch_bounds__(ROW_THREADS)
                                             (long long)(sh.kvh * p.group + r - t * p.group) * p.q_head);
 #pragma unroll
     for (int kk = 0; kk < HD / 16; ++kk) {
-      qf[kk][x] = live ? __ldg(reinterpret_cast<const uint32_t*>(q + 32 * kk + 4 * c)) : 0u;
-      qf[kk][x + 2] = live ? __ldg(reinterpret_cast<const uint32_t*>(q + 32 * kk + 16 + 4 * c)) : 0u;
+      qf[kk][x] = live ? signed_q(p, __ldg(reinterpret_cast<const uint32_t*>(q + 32 * kk + 4 * c))) : 0u;
+      qf[kk][x + 2] = live ? signed_q(p, __ldg(reinterpret_cast<const uint32_t*>(q + 32 * kk + 16 + 4 * c))) : 0u;
     }
   }
   float o[HD / 8][4];
@@ -341,6 +341,387 @@ __global__ void __launch_bounds__(ROW_THREADS)
   }
 }
 
+// ---- chunks ----------------------------------------------------------------------------------------
+// chunk_kernel: tiles of 256 rows as two tiles A, B of 128, one CTA per SM. Both products run on
+// tcgen05 (128-key blocks): S = Q K^T from shared memory into TMEM, O += P V with P read from TMEM (it
+// overwrites the scores it came from) and V as TMA left it (dims contiguous). Four warps per tile hold
+// one row per thread: no shuffles, the row's maximum and sum stay in registers. While one tile's warps
+// take exponentials, the tensor cores work for the other. O is rescaled only when a maximum has grown by
+// more than 2^8 since the last time, which is rare after the first blocks: P stays below 2^8, far inside
+// both types. Bound by the exponentials at head_dim 64 (16 a clock per SM: 2048 clocks for two 128 x 128
+// tiles, whose products take 1024), by both alike at 128.
+constexpr int CT = 256;
+constexpr int CK = 128;
+constexpr int CHUNK_THREADS = 384;  // warps 0-3 tile A, 4-7 tile B, 8 TMA, 9 MMA, 10 and 11 only make 8 and 9 a warpgroup
+// Registers per thread: 384 x 168 at launch; the warps of the tiles, a row of scores each, take 224, the others 56
+// (256 x 224 + 128 x 56 = 384 x 168).
+constexpr int TILE_REGS = 224, OTHER_REGS = 56;
+constexpr int MAX_SLOTS = 8;
+constexpr float LAZY = 8.f;  // log2 of the growth that is let pass
+
+template <int HD>
+struct ChunkShape {
+  static constexpr int TILE = CK * HD * 2;              // one K or V block
+  static constexpr int HALF = CK * 128;                 // its 64-dim half
+  static constexpr int SLOTS = HD == 128 ? 5 : 8;
+  static constexpr int QHALF = CT * 128;
+  static constexpr int SMEM = SLOTS * TILE + CT * HD * 2 + 1024 + 256;
+};
+
+// A 64-dim half of V is 128 keys x 128 bytes, 128-byte swizzle, dims contiguous ("MN-major" B operand):
+// 8-key groups are 1024 bytes apart (stride offset), the 64-dim halves HALF bytes (leading offset).
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t addr, uint32_t half_bytes) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(half_bytes >> 4) << 16) | ((uint64_t)64 << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// D[tmem] (+)= A[tmem] * B[smem]: A is 128 lanes x 16 16-bit values in 8 columns.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int DT, int HD>
+__global__ void __launch_bounds__(CHUNK_THREADS, 1)
+    chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                 const __grid_constant__ AttendParams p) {
+  using S = ChunkShape<HD>;
+  constexpr int SLOTS = S::SLOTS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  char* ring = asmem + ((1024u - (smem_u32(asmem) & 1023u)) & 1023u);
+  char* qs = ring + SLOTS * S::TILE;  // [HD / 64][256 rows][128 bytes], 128-byte swizzle
+  uint64_t* full = reinterpret_cast<uint64_t*>(qs + CT * HD * 2);
+  uint64_t* empty = full + MAX_SLOTS;
+  uint64_t* raw = empty + MAX_SLOTS;
+  uint64_t* sfull = raw + 1;   // [2] scores of a tile are in TMEM
+  uint64_t* pfull = sfull + 2;  // [2] its probabilities are
+  uint64_t* ofull = pfull + 2;  // [2] its sums include them
+  uint64_t* done = ofull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(raw, 1);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&sfull[x], 1);
+      mbar_init(&pfull[x], 4);
+      mbar_init(&ofull[x], 1);
+    }
+    mbar_init(done, 1);
+    fence_mbar_init();
+  }
+  Share sh;
+  if (!find_share<CT, CK, CHUNK_THREADS>(p, blockIdx.x, sh)) return;
+  sh.tile = (int)(((long long)sh.fresh * p.group + CT - 1) / CT) - 1 - sh.tile;  // the longest ones first
+  const int total = sh.fresh * p.group, r0 = sh.tile * CT, r1 = min(r0 + CT, total) - 1;
+  const Keys ks = keys_of<CK>(p, sh, r0, r1);
+  const int i0 = (int)((long long)ks.blocks * sh.split / sh.splits);
+  const int i1 = (int)((long long)ks.blocks * (sh.split + 1) / sh.splits);
+  // the keys that tile A and tile B see by themselves: blocks outside are not computed
+  const Keys ka = keys_of<CK>(p, sh, r0, min(r0 + 127, r1));
+  const bool has_b = r0 + 128 <= r1;
+  const Keys kb = has_b ? keys_of<CK>(p, sh, r0 + 128, r1) : ka;
+  auto uses = [&](int x, int i) {
+    const Keys& k = x ? kb : ka;
+    if (x && !has_b) return false;
+    const int key0 = block_key<CK>(ks, i);
+    return key0 < k.hi && (key0 + CK > k.lo || key0 < p.sinks);
+  };
+
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+  if (warp == 8) {
+    // producer: slots hold K, V, K, V, ... of blocks i0, i0 + 1, ...; lane j fetches the j-th page
+    const int rows_box = min(1 << p.shift, CK), boxes = CK / rows_box;
+    auto page_at = [&](int i) {
+      return lane < boxes ? page_of(p, ks, sh.b, (block_key<CK>(ks, i) >> p.shift) + lane) : -1;
+    };
+    int id = i0 < i1 ? page_at(i0) : -1;
+    bool ok = true;
+    int issued = 0;
+    for (int i = i0; i < i1 && ok; ++i) {
+      const int next = i + 1 < i1 ? page_at(i + 1) : -1;
+      const int key0 = block_key<CK>(ks, i), row = boxes > 1 ? 0 : key0 & ((1 << p.shift) - 1);
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const int n = 2 * (i - i0) + kv, s = n % SLOTS;
+        if (n >= SLOTS && !wait_bounded(&empty[s], ((n / SLOTS) & 1) ^ 1, p.timeout_ns)) {
+          atomicCAS(p.error, 0, 0x211);
+          ok = false;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        // rows of V behind the last key may hold anything, and 0 * NaN is not 0: they are zeroed here
+        const bool ragged = kv == 1 && key0 + CK > ks.hi;
+        uint64_t* bar = ragged ? raw : &full[s];
+        if (lane == 0) mbar_expect_tx(bar, (uint32_t)S::TILE);
+        __syncwarp();
+        char* at = ring + s * S::TILE;
+        if (lane < boxes)
+#pragma unroll
+          for (int h = 0; h < HD / 64; ++h)
+            tma_load_4d(at + h * S::HALF + lane * rows_box * 128, kv ? &tv : &tk, 64 * h, row, sh.kvh, id, bar);
+        issued = n + 1;
+        if (ragged) {  // only the last block
+          ok = __all_sync(0xffffffffu, wait_bounded(raw, 0, p.timeout_ns));
+          if (!ok) {
+            if (lane == 0) atomicCAS(p.error, 0, 0x212);
+            break;
+          }
+          for (int e = lane + (ks.hi - key0) * (HD / 8); e < CK * (HD / 8); e += 32) {
+            const int r = e / (HD / 8), ch = e % (HD / 8);
+            *reinterpret_cast<uint4*>(at + (ch >> 3) * S::HALF + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[s]);
+        }
+      }
+      id = next;
+    }
+    if (!ok && lane == 0)  // let what is in flight land before the block ends
+      for (int n = max(0, issued - SLOTS); n < issued; ++n)
+        wait_bounded(&full[n % SLOTS], (n / SLOTS) & 1, p.timeout_ns);
+  } else if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    asm volatile("bar.sync 2, 288;" ::: "memory");  // Q is in shared memory
+    tmem_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    if (lane == 0) {
+      constexpr uint32_t fmt = DT == MKX_BF16 ? 1u : 0u;
+      const uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(128 >> 4) << 24);
+      const uint32_t id_qk = base | ((uint32_t)(CK >> 3) << 17);
+      const uint32_t id_pv = base | ((uint32_t)(HD >> 3) << 17) | (1u << 16);  // V: dims contiguous
+      int uses_of[2] = {0, 0};
+      bool pending[2] = {false, false}, ok = true;
+      for (int i = i0; i <= i1 && ok; ++i) {
+        const int nk = 2 * (i - i0), nv = nk - 1;  // places of K(i) and V(i - 1)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t st = tmem + 128 * x, ot = tmem + 256 + 128 * x;
+          if (pending[x] && ok) {
+            ok = wait_bounded(&pfull[x], (uses_of[x] - 1) & 1, p.timeout_ns) &&
+                 wait_bounded(&full[nv % SLOTS], (nv / SLOTS) & 1, p.timeout_ns);
+            if (!ok) break;
+            tmem_fence_after();
+            const uint32_t v = smem_u32(ring + (nv % SLOTS) * S::TILE);
+#pragma unroll
+            for (int kk = 0; kk < CK / 16; ++kk)
+              umma_ts(ot, st + 8 * kk, sw128_mn_desc(v + 2048 * kk, S::HALF), id_pv, (uses_of[x] > 1 || kk > 0) ? 1u : 0u);
+            umma_commit(&ofull[x]);
+            pending[x] = false;
+          }
+          if (x == 1 && i > i0) umma_commit(&empty[nv % SLOTS]);
+          if (i < i1 && uses(x, i)) {
+            ok = wait_bounded(&full[nk % SLOTS], (nk / SLOTS) & 1, p.timeout_ns);
+            if (!ok) break;
+            tmem_fence_after();
+            const uint32_t k = smem_u32(ring + (nk % SLOTS) * S::TILE), q = smem_u32(qs) + x * 128 * 128;
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk)
+              umma_bf16(st, sw128_desc(q + (kk >> 2) * S::QHALF + 32 * (kk & 3)),
+                        sw128_desc(k + (kk >> 2) * S::HALF + 32 * (kk & 3)), id_qk, kk > 0 ? 1u : 0u);
+            umma_commit(&sfull[x]);
+            pending[x] = true;
+            ++uses_of[x];
+          }
+        }
+        if (i < i1) umma_commit(&empty[nk % SLOTS]);
+      }
+      if (!ok) atomicCAS(p.error, 0, 0x213);
+      umma_commit(done);
+    }
+    __syncwarp();
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TILE_REGS));
+    // Q into shared memory, coalesced: 16-byte chunks of a row by neighbouring threads
+    for (int e = threadIdx.x; e < CT * (HD / 8); e += 256) {
+      const int row = e / (HD / 8), ch = e % (HD / 8), r = r0 + row;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r <= r1) {
+        const int t = r / p.group;
+        v = __ldg(reinterpret_cast<const uint4*>((const char*)p.q +
+                                                 2 * ((long long)(sh.first_row + t) * p.q_row +
+                                                      (long long)(sh.kvh * p.group + r - t * p.group) * p.q_head + 8 * ch)));
+        v = make_uint4(signed_q(p, v.x), signed_q(p, v.y), signed_q(p, v.z), signed_q(p, v.w));
+      }
+      *reinterpret_cast<uint4*>(qs + (ch >> 3) * S::QHALF + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = v;
+    }
+    fence_proxy_async();
+    asm volatile("bar.sync 2, 288;" ::: "memory");
+    tmem_fence_after();
+    const int x = warp >> 2, row = threadIdx.x;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t st = *tmem_slot + lanes + 128 * x, ot = *tmem_slot + lanes + 256 + 128 * x;
+    const Keys& kx = x ? kb : ka;
+    const int position = sh.past + (r0 + row) / p.group;
+    float m = -INFINITY, l = 0.f;
+    int n = 0;
+    bool ok = true;
+    for (int i = i0; i < i1; ++i) {
+      if (!uses(x, i)) continue;
+      ok = __all_sync(0xffffffffu, wait_bounded(&sfull[x], n & 1, p.timeout_ns));
+      if (!ok) break;
+      tmem_fence_after();
+      const int key0 = block_key<CK>(ks, i);
+      uint32_t s[4][32];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tmem_ld32(st + 32 * j, s[j]);
+      if (!whole_block<CK>(p, kx, key0)) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j)
+          if (!sees(p, kx, position, key0 + j)) s[j >> 5][j & 31] = 0xff800000u;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 128; ++j) top = fmaxf(top, __uint_as_float(s[j >> 5][j & 31]));
+      top *= p.scale_log2;  // > 0: -inf stays
+      const bool grow = top > m + LAZY || (m == -INFINITY && top > m);
+      if (__any_sync(0xffffffffu, grow)) {
+        const float now = grow ? top : m, fix = grow ? ex2(m - now) : 1.f;
+        if (n > 0) {
+          ok = __all_sync(0xffffffffu, wait_bounded(&ofull[x], (n - 1) & 1, p.timeout_ns));
+          if (!ok) break;
+          tmem_fence_after();
+#pragma unroll
+          for (int j = 0; j < HD / 32; ++j) {
+            uint32_t o[32];
+            tmem_ld32(ot + 32 * j, o);
+#pragma unroll
+            for (int d = 0; d < 32; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * fix);
+            tmem_st32(ot + 32 * j, o);
+          }
+        }
+        l *= fix;
+        m = now;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t w[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const int e = 64 * h + 2 * j;
+          const uint32_t sa = s[e >> 5][e & 31], sb = s[(e + 1) >> 5][(e + 1) & 31];
+          const float a = ex2(fmaf(__uint_as_float(sa), p.scale_log2, -base));
+          const float b = ex2(fmaf(__uint_as_float(sb), p.scale_log2, -base));
+          sum[j & 3] += a + b;
+          w[j] = Half16<DT>::pack(a, b);
+        }
+        tmem_st32(st + 32 * h, w);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_wait_st();
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pfull[x]);
+      ++n;
+    }
+    // epilogue
+    if (n > 0 && ok) {
+      ok = __all_sync(0xffffffffu, wait_bounded(&ofull[x], (n - 1) & 1, p.timeout_ns));
+      tmem_fence_after();
+    }
+    if (!ok && lane == 0) atomicCAS(p.error, 0, 0x214);
+    const int r = r0 + row, t = r / p.group;
+    char* out = (char*)p.out + 2 * ((long long)(sh.first_row + t) * p.o_row +
+                                    (long long)(sh.kvh * p.group + r - t * p.group) * p.o_head);
+    auto scale_of = [](float ls) { return ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls); };  // nothing seen: zero; NaN stays
+    auto write = [&](const float (&o)[32], int j, float inv) {
+#pragma unroll
+      for (int d = 0; d < 32; d += 8)
+        *reinterpret_cast<uint4*>(out + 2 * (32 * j + d)) =
+            make_uint4(Half16<DT>::pack(o[d] * inv, o[d + 1] * inv), Half16<DT>::pack(o[d + 2] * inv, o[d + 3] * inv),
+                       Half16<DT>::pack(o[d + 4] * inv, o[d + 5] * inv), Half16<DT>::pack(o[d + 6] * inv, o[d + 7] * inv));
+    };
+    constexpr int PART = CT * (HD + 2);  // [HD / 4][256 rows] float4, then (maximum, total) of each row
+    float* part = p.parts + (size_t)(sh.part + sh.split) * PART;
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j) {
+      uint32_t u[32];
+      float o[32];
+#pragma unroll
+      for (int d = 0; d < 32; ++d) u[d] = 0u;
+      if (n > 0 && ok) tmem_ld32(ot + 32 * j, u);  // warp-uniform
+#pragma unroll
+      for (int d = 0; d < 32; ++d) o[d] = __uint_as_float(u[d]);
+      if (sh.splits > 1) {
+#pragma unroll
+        for (int d = 0; d < 32; d += 4)
+          __stcg(reinterpret_cast<float4*>(part + ((size_t)(8 * j + d / 4) * CT + row) * 4),
+                 make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]));
+      } else if (r <= r1) {
+        write(o, j, scale_of(l));
+      }
+    }
+    if (sh.splits > 1) {
+      __stcg(reinterpret_cast<float2*>(part + (size_t)CT * HD) + row, make_float2(m, l));
+      __threadfence();
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      __shared__ int last;
+      if (threadIdx.x == 0) {
+        last = atomicAdd(p.tickets + sh.ticket, 1u) == (unsigned)sh.splits - 1;
+        if (last) p.tickets[sh.ticket] = 0;
+        __threadfence();
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (last && r <= r1) {
+        const float* parts = p.parts + (size_t)sh.part * PART;
+        float top = -INFINITY, ls = 0.f;
+        for (int k = 0; k < sh.splits; ++k)
+          top = fmaxf(top, __ldcg(reinterpret_cast<const float2*>(parts + (size_t)k * PART + CT * HD) + row).x);
+        const float base = top == -INFINITY ? 0.f : top;
+        for (int k = 0; k < sh.splits; ++k) {
+          const float2 ml = __ldcg(reinterpret_cast<const float2*>(parts + (size_t)k * PART + CT * HD) + row);
+          ls += ex2(ml.x - base) * ml.y;
+        }
+        const float inv = scale_of(ls);
+        for (int j = 0; j < HD / 32; ++j) {
+          float o[32];
+#pragma unroll
+          for (int d = 0; d < 32; ++d) o[d] = 0.f;
+          for (int k = 0; k < sh.splits; ++k) {
+            const float* at = parts + (size_t)k * PART;
+            const float f = ex2(__ldcg(reinterpret_cast<const float2*>(at + CT * HD) + row).x - base);
+#pragma unroll
+            for (int d = 0; d < 32; d += 4) {
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(at + ((size_t)(8 * j + d / 4) * CT + row) * 4));
+              o[d] += f * v.x;
+              o[d + 1] += f * v.y;
+              o[d + 2] += f * v.z;
+              o[d + 3] += f * v.w;
+            }
+          }
+          write(o, j, inv);
+        }
+      }
+    }
+    tmem_fence_before();
+  }
+  __syncthreads();
+  if (warp == 9) {
+    wait_bounded(done, 0, p.timeout_ns);  // no MMA may still write
+    tmem_fence_after();
+    tmem_free(*tmem_slot, 512);
+  }
+}
+
 // ---- host ----------------------------------------------------------------------------------------
 bool encode_pages(CUtensorMap* m, const void* base, int dtype, int head_dim, int page_rows, int kv_heads, int pages,
                   long long row, long long head, long long page, int box_rows) {
@@ -356,6 +737,7 @@ bool encode_pages(CUtensorMap* m, const void* base, int dtype, int head_dim, int
 }
 
 struct Plan {
+  bool chunk;
   int mt, kt, slots, max_parts;
   long long grid;
   size_t bytes;
@@ -370,9 +752,11 @@ bool plan_of(const mkx_attend_inputs& a, int sms, Plan& pl) {
   if (a.head_dim != 64 && a.head_dim != 128) return false;
   const long long group = a.heads / a.kv_heads;
   const long long most = a.max_rows < a.rows ? a.max_rows : a.rows;
-  pl.mt = MT;
-  pl.kt = 8192 / a.head_dim;
-  pl.slots = 2 * sms;
+  // rows of one K/V head and episode beyond one 16-row tile would read the pages again: chunk_kernel
+  pl.chunk = most * group > MT;
+  pl.mt = pl.chunk ? CT : MT;
+  pl.kt = pl.chunk ? CK : 8192 / a.head_dim;
+  pl.slots = pl.chunk ? sms : 2 * sms;
   // tiles <= the rows' tiles plus one per episode, and <= episodes x the tiles of the largest
   long long tiles = (a.rows * group) / pl.mt + a.B;
   const long long by_most = a.B * ((most * group + pl.mt - 1) / pl.mt);
@@ -383,18 +767,22 @@ bool plan_of(const mkx_attend_inputs& a, int sms, Plan& pl) {
   return pl.grid < (1ll << 31);
 }
 
-template <int DT, int HD>
-bool launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const AttendParams& p, long long grid, int device,
-                 cudaStream_t stream) {
-  static bool sized[MAX_DEVICES] = {};  // the attribute of this kernel is set once per device
-  if (!sized[device]) {
-    if (!mkxc::cuda_ok(cudaFuncSetAttribute(rows_kernel<DT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            RowShape<HD>::SMEM)))
-      return false;
+template <typename Kernel>
+bool launch(Kernel kernel, bool (&sized)[MAX_DEVICES], int threads, int smem, const CUtensorMap& tk, const CUtensorMap& tv,
+            const AttendParams& p, long long grid, int device, cudaStream_t stream) {
+  if (!sized[device]) {  // the attribute of a kernel is set once per device
+    if (!mkxc::cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))) return false;
     sized[device] = true;
   }
-  rows_kernel<DT, HD><<<(unsigned)grid, ROW_THREADS, RowShape<HD>::SMEM, stream>>>(tk, tv, p);
+  kernel<<<(unsigned)grid, threads, smem, stream>>>(tk, tv, p);
   return mkxc::cuda_ok(cudaGetLastError());
+}
+template <int DT, int HD>
+bool launch_typed(bool chunk, const CUtensorMap& tk, const CUtensorMap& tv, const AttendParams& p, long long grid, int device,
+                  cudaStream_t stream) {
+  static bool rows_sized[MAX_DEVICES] = {}, chunk_sized[MAX_DEVICES] = {};
+  return chunk ? launch(chunk_kernel<DT, HD>, chunk_sized, CHUNK_THREADS, ChunkShape<HD>::SMEM, tk, tv, p, grid, device, stream)
+               : launch(rows_kernel<DT, HD>, rows_sized, ROW_THREADS, RowShape<HD>::SMEM, tk, tv, p, grid, device, stream);
 }
 
 }  // namespace
@@ -468,14 +856,18 @@ extern "C" mkx_status mkx_cache_attend(const mkx_attend_inputs* in, size_t works
   p.causal = a.causal != 0;
   p.window = a.window < MAX_KEYS ? a.window : MAX_KEYS;
   p.sinks = a.sinks < MAX_KEYS ? a.sinks : MAX_KEYS;
-  p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
+  p.scale_log2 = a.scale == 0.f ? 1.f : (float)(std::fabs((double)a.scale) * 1.4426950408889634);
+  p.q_and = a.scale == 0.f ? 0u : ~0u;
+  p.q_xor = a.scale < 0.f ? 0x80008000u : 0u;
   p.slots = pl.slots;
   p.min_blocks = 2;
   p.max_parts = pl.max_parts;
   p.timeout_ns = 2000000000ull;
-  const bool ok = a.head_dim == 64 ? (a.dtype == MKX_BF16 ? launch_rows<MKX_BF16, 64>(tk, tv, p, pl.grid, device, stream)
-                                                          : launch_rows<MKX_FP16, 64>(tk, tv, p, pl.grid, device, stream))
-                                   : (a.dtype == MKX_BF16 ? launch_rows<MKX_BF16, 128>(tk, tv, p, pl.grid, device, stream)
-                                                          : launch_rows<MKX_FP16, 128>(tk, tv, p, pl.grid, device, stream));
+  const bool ok =
+      a.head_dim == 64
+          ? (a.dtype == MKX_BF16 ? launch_typed<MKX_BF16, 64>(pl.chunk, tk, tv, p, pl.grid, device, stream)
+                                 : launch_typed<MKX_FP16, 64>(pl.chunk, tk, tv, p, pl.grid, device, stream))
+          : (a.dtype == MKX_BF16 ? launch_typed<MKX_BF16, 128>(pl.chunk, tk, tv, p, pl.grid, device, stream)
+                                 : launch_typed<MKX_FP16, 128>(pl.chunk, tk, tv, p, pl.grid, device, stream));
   return ok ? MKX_OK : MKX_ERR_CUDA;
 }

@@ -22,7 +22,8 @@ struct AttendParams {
   long long q_row, q_head, o_row, o_head;
   int rows, B, heads, kv_heads, group, pages, shift, table_width, max_rows;
   int causal, window, sinks;
-  float scale_log2;  // scale * log2(e): scores are kept in powers of two
+  float scale_log2;       // |scale| * log2(e): scores are kept in powers of two
+  uint32_t q_and, q_xor;  // q's words as they enter: the sign of a negative scale, nothing for scale 0
   int slots;         // blocks that the call's work is meant to be spread over
   int min_blocks;    // key blocks that a part has at least
   int max_parts;
@@ -204,6 +205,8 @@ __device__ __forceinline__ int page_of(const AttendParams& p, const Keys& k, int
   const int id = p.table[(size_t)b * p.table_width + page];
   return id >= 0 && id < p.pages ? id : -1;
 }
+
+__device__ __forceinline__ uint32_t signed_q(const AttendParams& p, uint32_t v) { return (v & p.q_and) ^ p.q_xor; }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
