@@ -190,12 +190,16 @@ __global__ void __launch_bounds__(ROW_THREADS)
       }
     const bool whole = whole_block<KT>(p, ks, block_key<KT>(ks, i));
     float top[2] = {-INFINITY, -INFINITY};
+    uint32_t seen[2] = {~0u, ~0u};  // of this thread's columns 8 j + 2 c + (0, 1)
+    if (!whole)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) seen[x] = seen_mask(p, ks, pos[x], key0) >> (2 * c);
 #pragma unroll
     for (int j = 0; j < KW / 8; ++j)
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         float v = sc[j][x] * p.scale_log2;
-        if (!whole && !sees(p, ks, pos[x >> 1], key0 + 8 * j + 2 * c + (x & 1))) v = -INFINITY;
+        if (!((seen[x >> 1] >> (8 * j + (x & 1))) & 1u)) v = -INFINITY;
         sc[j][x] = v;
         top[x >> 1] = fmaxf(top[x >> 1], v);
       }
@@ -584,8 +588,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       for (int j = 0; j < 4; ++j) tmem_ld32(st + 32 * j, s[j]);
       if (!whole_block<CK>(p, kx, key0)) {
 #pragma unroll
-        for (int j = 0; j < 128; ++j)
-          if (!sees(p, kx, position, key0 + j)) s[j >> 5][j & 31] = 0xff800000u;
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t seen = seen_mask(p, kx, position, key0 + 32 * j);
+#pragma unroll
+          for (int d = 0; d < 32; ++d)
+            if (!((seen >> d) & 1u)) s[j][d] = 0xff800000u;
+        }
       }
       float top = -INFINITY;
 #pragma unroll

@@ -193,9 +193,12 @@ __device__ __forceinline__ bool whole_block(const AttendParams& p, const Keys& k
   if (key0 + KT > k.hi || (p.causal && key0 + KT - 1 > k.p_first)) return false;
   return !p.window || key0 > k.p_last - p.window || key0 + KT <= p.sinks;
 }
-__device__ __forceinline__ bool sees(const AttendParams& p, const Keys& k, int position, int key) {
-  if (key >= k.hi || (p.causal && key > position)) return false;
-  return !p.window || key > position - p.window || key < p.sinks;
+// Bit d: whether a row at `position` sees key0 + d, d < 32.
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; }
+__device__ __forceinline__ uint32_t seen_mask(const AttendParams& p, const Keys& k, int position, int key0) {
+  uint32_t m = below((p.causal ? min(k.hi, position + 1) : k.hi) - key0);
+  if (p.window) m &= ~below(position - p.window + 1 - key0) | below(p.sinks - key0);
+  return m;
 }
 // The page that holds keys [page << shift, ..), or -1 (its rows read as zero) where no row sees any.
 __device__ __forceinline__ int page_of(const AttendParams& p, const Keys& k, int b, int page) {
