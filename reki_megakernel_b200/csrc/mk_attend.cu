@@ -26,6 +26,7 @@ constexpr int MAX_KEYS = 1 << 30;  // rows of an episode: keys and positions are
 constexpr int ROW_WARPS = 4;
 constexpr int ROW_THREADS = 32 * (ROW_WARPS + 1);
 constexpr int ROW_STAGES = 3;
+constexpr int JOIN_AT_ONCE = 12;  // parts that one block joins
 
 template <int HD>
 struct RowShape {
@@ -33,7 +34,9 @@ struct RowShape {
   static constexpr int KW = KT / ROW_WARPS;          // keys of a warp
   static constexpr int HALF = KT * 128;              // bytes of a 64-dim half of K or V
   static constexpr int STAGE = 2 * KT * HD * 2;
-  static constexpr int SMEM = ROW_STAGES * STAGE + 1024 + 256;
+  static constexpr int JOIN = HD / 4 + 2;            // floats of a row in the join of the warps
+  static constexpr int QROW = HD * 2 + 16;           // bytes of a row of Q: fragments without bank conflicts
+  static constexpr int SMEM = ROW_STAGES * STAGE + ROW_WARPS * MT * (JOIN * 4 + 8) + MT * QROW + 1024 + 128;
 };
 
 template <int DT>
@@ -67,282 +70,327 @@ __device__ __forceinline__ void row_barrier() { asm volatile("bar.sync 1, %0;" :
 extern __shared__ __align__(1024) char asmem[];
 
 template <int DT, int HD>
-__global__ void __launch_bounds__(ROW_THREADS)
+__global__ void __launch_bounds__(ROW_THREADS, 2)
     rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                 const __grid_constant__ AttendParams p) {
   using S = RowShape<HD>;
-  constexpr int KT = S::KT, KW = S::KW;
+  constexpr int KT = S::KT, KW = S::KW, PART = MT * (HD + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   char* ring = asmem + ((1024u - (smem_u32(asmem) & 1023u)) & 1023u);
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + ROW_STAGES * S::STAGE);
+  float* os = reinterpret_cast<float*>(ring + ROW_STAGES * S::STAGE);  // [4 warps][16 rows][S::JOIN]
+  float2* ml = reinterpret_cast<float2*>(os + ROW_WARPS * MT * S::JOIN);  // [4][16]
+  uint64_t* full = reinterpret_cast<uint64_t*>(ml + ROW_WARPS * MT);
   uint64_t* empty = full + ROW_STAGES;
+  uint64_t* qfull = empty + ROW_STAGES;  // the next tile's rows of Q, copied ahead
+  uint64_t* qempty = qfull + 1;
+  char* qs = reinterpret_cast<char*>(qempty + 1);  // [16 rows][S::QROW]
   if (threadIdx.x == 0) {
     for (int s = 0; s < ROW_STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], ROW_WARPS);
     }
+    mbar_init(qfull, 1);
+    mbar_init(qempty, ROW_WARPS);
     fence_mbar_init();
   }
-  Share sh;
-  if (!find_share<MT, KT, ROW_THREADS>(p, blockIdx.x, sh)) return;  // its barriers publish the mbarriers too
-  const int total = sh.fresh * p.group, r0 = sh.tile * MT, r1 = min(r0 + MT, total) - 1;
-  const Keys ks = keys_of<KT>(p, sh, r0, r1);
-  const int i0 = (int)((long long)ks.blocks * sh.split / sh.splits);
-  const int i1 = (int)((long long)ks.blocks * (sh.split + 1) / sh.splits);
+  Line line;
+  if (!find_line<MT, KT, ROW_THREADS>(p, line)) return;  // its barriers publish the mbarriers too
+  Walk<MT, KT> walk(p, line);
+  Segment sg;
+  int n = 0, tiles = 0;  // blocks of keys and tiles since the start: n % ROW_STAGES is a block's stage
 
   if (warp == ROW_WARPS) {
     // producer: lane j fetches the j-th page of each block
     const int rows_box = min(1 << p.shift, KT), boxes = KT / rows_box;
-    int id = -1;
-    auto page_at = [&](int i) {
-      return lane < boxes ? page_of(p, ks, sh.b, (block_key<KT>(ks, i) >> p.shift) + lane) : -1;
-    };
-    if (i0 < i1) id = page_at(i0);
     bool ok = true;
-    int issued = i0;
-    for (int i = i0; i < i1; ++i) {
-      const int n = i - i0, s = n % ROW_STAGES;
-      const int next = i + 1 < i1 ? page_at(i + 1) : -1;
-      if (n >= ROW_STAGES && !wait_bounded(&empty[s], ((n / ROW_STAGES) & 1) ^ 1, p.timeout_ns)) {
-        atomicCAS(p.error, 0, 0x201);
-        ok = false;
-      }
-      if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane == 0) mbar_expect_tx(&full[s], (uint32_t)S::STAGE);
+    while (ok && walk.next(sg)) {
+      const int r0 = sg.tile * MT, r1 = min(r0 + MT, sg.fresh * p.group) - 1;
+      const Keys ks = keys_of<KT>(p, sg, r0, r1);
+      const int i0 = (int)((long long)ks.blocks * sg.v0 / sg.units), i1 = (int)((long long)ks.blocks * sg.v1 / sg.units);
+      auto page_at = [&](int i) {
+        return lane < boxes ? page_of(p, ks, sg.b, (block_key<KT>(ks, i) >> p.shift) + lane) : -1;
+      };
+      if (i0 >= i1) continue;
+      int id = page_at(i0);
+      if (tiles >= 1) ok = wait_bounded(qempty, (tiles & 1) ^ 1, p.timeout_ns);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane == 0) mbar_expect_tx(qfull, (uint32_t)((r1 - r0 + 1) * HD * 2));
       __syncwarp();
-      if (lane < boxes) {
-        const int row = block_key<KT>(ks, i) & ((1 << p.shift) - 1);
-        char* at = ring + s * S::STAGE + lane * rows_box * 128;
-#pragma unroll
-        for (int h = 0; h < HD / 64; ++h) {
-          tma_load_4d(at + h * S::HALF, &tk, 64 * h, boxes > 1 ? 0 : row, sh.kvh, id, &full[s]);
-          tma_load_4d(at + KT * HD * 2 + h * S::HALF, &tv, 64 * h, boxes > 1 ? 0 : row, sh.kvh, id, &full[s]);
-        }
+      if (lane <= r1 - r0) {
+        const int r = r0 + lane, t = r / p.group;
+        bulk_g2s(qs + lane * S::QROW,
+                 (const char*)p.q + 2 * ((long long)(sg.first_row + t) * p.q_row +
+                                         (long long)(sg.kvh * p.group + r - t * p.group) * p.q_head),
+                 HD * 2, qfull);
       }
-      issued = i + 1;
-      id = next;
+      ++tiles;
+      for (int i = i0; i < i1; ++i, ++n) {
+        const int s = n % ROW_STAGES;
+        const int next = i + 1 < i1 ? page_at(i + 1) : -1;
+        if (n >= ROW_STAGES) ok = wait_bounded(&empty[s], ((n / ROW_STAGES) & 1) ^ 1, p.timeout_ns);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(&full[s], (uint32_t)S::STAGE);
+        __syncwarp();
+        if (lane < boxes) {
+          const int row = boxes > 1 ? 0 : block_key<KT>(ks, i) & ((1 << p.shift) - 1);
+          char* at = ring + s * S::STAGE + lane * rows_box * 128;
+#pragma unroll
+          for (int h = 0; h < HD / 64; ++h) {
+            tma_load_4d(at + h * S::HALF, &tk, 64 * h, row, sg.kvh, id, &full[s]);
+            tma_load_4d(at + KT * HD * 2 + h * S::HALF, &tv, 64 * h, row, sg.kvh, id, &full[s]);
+          }
+        }
+        id = next;
+      }
     }
-    if (lane == 0 && issued < i1)  // a wait ran out: let what is in flight land before the block ends
-      for (int i = max(i0, issued - ROW_STAGES); i < issued; ++i)
-        wait_bounded(&full[(i - i0) % ROW_STAGES], ((i - i0) / ROW_STAGES) & 1, p.timeout_ns);
+    if (!ok && lane == 0) {  // a wait ran out: let what is in flight land before the block ends
+      atomicCAS(p.error, 0, 0x201);
+      for (int k = max(0, n - ROW_STAGES); k < n; ++k)
+        wait_bounded(&full[k % ROW_STAGES], (k / ROW_STAGES) & 1, p.timeout_ns);
+      if (tiles > 0) wait_bounded(qfull, (tiles - 1) & 1, p.timeout_ns);
+    }
     return;
   }
 
-  // queries: A fragments of the 16 rows, read once
   const int g = lane >> 2, c = lane & 3;
-  uint32_t qf[HD / 16][4];
-  int pos[2];
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int r = r0 + g + 8 * x;
-    const bool live = r <= r1;
-    const int t = r / p.group;
-    pos[x] = sh.past + t;
-    const char* q = (const char*)p.q + 2 * ((long long)(sh.first_row + t) * p.q_row +
-                                            (long long)(sh.kvh * p.group + r - t * p.group) * p.q_head);
-#pragma unroll
-    for (int kk = 0; kk < HD / 16; ++kk) {
-      qf[kk][x] = live ? signed_q(p, __ldg(reinterpret_cast<const uint32_t*>(q + 32 * kk + 4 * c))) : 0u;
-      qf[kk][x + 2] = live ? signed_q(p, __ldg(reinterpret_cast<const uint32_t*>(q + 32 * kk + 16 + 4 * c))) : 0u;
-    }
-  }
-  float o[HD / 8][4];
-#pragma unroll
-  for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   // ldmatrix: lane's row and 16-byte chunk of the four 8x8 parts
   const int krow = (lane & 7) + ((lane >> 4) << 3), kchunk = (lane >> 3) & 1;   // keys 0-7, 0-7, 8-15, 8-15
   const int vrow = (lane & 7) + (((lane >> 3) & 1) << 3), vchunk = lane >> 4;   // keys 0-7, 8-15, 0-7, 8-15
   bool ok = true;
-  for (int i = i0; i < i1; ++i) {
-    const int n = i - i0, s = n % ROW_STAGES;
-    if (!__all_sync(0xffffffffu, wait_bounded(&full[s], (n / ROW_STAGES) & 1, p.timeout_ns))) {
-      if (lane == 0) atomicCAS(p.error, 0, 0x202);
-      ok = false;
-      break;
-    }
-    const int key0 = block_key<KT>(ks, i) + warp * KW;
-    char* kt = ring + s * S::STAGE;
-    char* vt = kt + KT * HD * 2;
-    const bool ragged = key0 + KW > ks.hi;
-    if (ragged) {  // rows behind the last key may hold anything, and 0 * NaN is not 0
-      for (int e = lane; e < KW * (HD / 8); e += 32) {
-        const int row = e / (HD / 8), ch = e % (HD / 8);
-        if (key0 + row >= ks.hi)
-          *reinterpret_cast<uint4*>(vt + (ch >> 3) * S::HALF + (warp * KW + row) * 128 + (ch & 7) * 16) =
-              make_uint4(0, 0, 0, 0);
+  while (walk.next(sg)) {
+    const int r0 = sg.tile * MT, r1 = min(r0 + MT, sg.fresh * p.group) - 1;
+    const Keys ks = keys_of<KT>(p, sg, r0, r1);
+    const int i0 = (int)((long long)ks.blocks * sg.v0 / sg.units), i1 = (int)((long long)ks.blocks * sg.v1 / sg.units);
+    // queries: A fragments of the 16 rows (rows that are not there hold anything: no row touches another)
+    uint32_t qf[HD / 16][4];
+    int pos[2];
+    if (i0 < i1) {
+      ok = ok && __all_sync(0xffffffffu, wait_bounded(qfull, tiles & 1, p.timeout_ns));
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        pos[x] = sg.past + (r0 + g + 8 * x) / p.group;
+        const char* q = qs + (g + 8 * x) * S::QROW + 4 * c;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          qf[kk][x] = signed_q(p, *reinterpret_cast<const uint32_t*>(q + 32 * kk));
+          qf[kk][x + 2] = signed_q(p, *reinterpret_cast<const uint32_t*>(q + 32 * kk + 16));
+        }
       }
       __syncwarp();
+      if (lane == 0) mbar_arrive(qempty);
+      ++tiles;
     }
-    const uint32_t ka = smem_u32(kt), va = smem_u32(vt);
-    float sc[KW / 8][4];
+    float o[HD / 8][4];
 #pragma unroll
-    for (int j = 0; j < KW / 8; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+    for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int i = i0; i < i1 && ok; ++i, ++n) {
+      const int s = n % ROW_STAGES;
+      ok = __all_sync(0xffffffffu, wait_bounded(&full[s], (n / ROW_STAGES) & 1, p.timeout_ns));
+      if (!ok) break;
+      const int key0 = block_key<KT>(ks, i) + warp * KW;
+      char* kt = ring + s * S::STAGE;
+      char* vt = kt + KT * HD * 2;
+      const bool ragged = key0 + KW > ks.hi;
+      if (ragged) {  // rows behind the last key may hold anything, and 0 * NaN is not 0
+        for (int e = lane; e < KW * (HD / 8); e += 32) {
+          const int row = e / (HD / 8), ch = e % (HD / 8);
+          if (key0 + row >= ks.hi)
+            *reinterpret_cast<uint4*>(vt + (ch >> 3) * S::HALF + (warp * KW + row) * 128 + (ch & 7) * 16) =
+                make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+      }
+      const uint32_t ka = smem_u32(kt), va = smem_u32(vt);
+      float sc[KW / 8][4];
 #pragma unroll
-    for (int kk = 0; kk < HD / 16; ++kk)
+      for (int j = 0; j < KW / 8; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+        for (int j = 0; j < KW / 16; ++j) {
+          const int row = warp * KW + 16 * j + krow, ch = 2 * (kk & 3) + kchunk;
+          uint32_t b[4];
+          ldsm4(b, ka + (kk >> 2) * S::HALF + row * 128 + ((ch ^ (row & 7)) << 4));
+          mma16<DT>(sc[2 * j], qf[kk], b[0], b[1]);
+          mma16<DT>(sc[2 * j + 1], qf[kk], b[2], b[3]);
+        }
+      float top[2] = {-INFINITY, -INFINITY};
+      uint32_t seen[2] = {~0u, ~0u};  // of this thread's columns 8 j + 2 c + (0, 1)
+      if (!whole_block<KT>(p, ks, block_key<KT>(ks, i)))
+#pragma unroll
+        for (int x = 0; x < 2; ++x) seen[x] = seen_mask(p, ks, pos[x], key0) >> (2 * c);
+#pragma unroll
+      for (int j = 0; j < KW / 8; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float v = sc[j][x] * p.scale_log2;
+          if (!((seen[x >> 1] >> (8 * j + (x & 1))) & 1u)) v = -INFINITY;
+          sc[j][x] = v;
+          top[x >> 1] = fmaxf(top[x >> 1], v);
+        }
+      float fix[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
+        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
+        const float now = fmaxf(m[x], top[x]), safe = now == -INFINITY ? 0.f : now;
+        fix[x] = ex2(m[x] - safe);
+        m[x] = now;
+        top[x] = safe;
+        l[x] *= fix[x];
+      }
+#pragma unroll
+      for (int j = 0; j < HD / 8; ++j) {
+        o[j][0] *= fix[0];
+        o[j][1] *= fix[0];
+        o[j][2] *= fix[1];
+        o[j][3] *= fix[1];
+      }
 #pragma unroll
       for (int j = 0; j < KW / 16; ++j) {
-        const int row = warp * KW + 16 * j + krow, ch = 2 * (kk & 3) + kchunk;
-        uint32_t b[4];
-        ldsm4(b, ka + (kk >> 2) * S::HALF + row * 128 + ((ch ^ (row & 7)) << 4));
-        mma16<DT>(sc[2 * j], qf[kk], b[0], b[1]);
-        mma16<DT>(sc[2 * j + 1], qf[kk], b[2], b[3]);
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {  // A fragment words: (row g, keys 0-7), (g + 8, 0-7), (g, 8-15), (g + 8, 8-15)
+          const int t = 2 * j + (y >> 1), x = y & 1;
+          const float a = ex2(sc[t][2 * x] - top[x]), b = ex2(sc[t][2 * x + 1] - top[x]);
+          l[x] += a + b;
+          hi[y] = Half16<DT>::pack(a, b);
+          const float2 h = Half16<DT>::unpack(hi[y]);
+          lo[y] = Half16<DT>::pack(a - h.x, b - h.y);
+        }
+#pragma unroll
+        for (int n16 = 0; n16 < HD / 16; ++n16) {
+          const int row = warp * KW + 16 * j + vrow, ch = 2 * (n16 & 3) + vchunk;
+          uint32_t b[4];
+          ldsm4_t(b, va + (n16 >> 2) * S::HALF + row * 128 + ((ch ^ (row & 7)) << 4));
+          mma16<DT>(o[2 * n16], hi, b[0], b[1]);
+          mma16<DT>(o[2 * n16 + 1], hi, b[2], b[3]);
+          mma16<DT>(o[2 * n16], lo, b[0], b[1]);
+          mma16<DT>(o[2 * n16 + 1], lo, b[2], b[3]);
+        }
       }
-    const bool whole = whole_block<KT>(p, ks, block_key<KT>(ks, i));
-    float top[2] = {-INFINITY, -INFINITY};
-    uint32_t seen[2] = {~0u, ~0u};  // of this thread's columns 8 j + 2 c + (0, 1)
-    if (!whole)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) seen[x] = seen_mask(p, ks, pos[x], key0) >> (2 * c);
-#pragma unroll
-    for (int j = 0; j < KW / 8; ++j)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        float v = sc[j][x] * p.scale_log2;
-        if (!((seen[x >> 1] >> (8 * j + (x & 1))) & 1u)) v = -INFINITY;
-        sc[j][x] = v;
-        top[x >> 1] = fmaxf(top[x >> 1], v);
-      }
-    float fix[2];
+      if (ragged) fence_proxy_async();  // the zeros above, before the next copy into this stage
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+    }
+
+    // join the four warps, a quarter of the dims at a time (the copies of the next tile own the ring):
+    // 8 threads per row, HD / 32 neighbouring dims each
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
-      top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
-      const float now = fmaxf(m[x], top[x]), safe = now == -INFINITY ? 0.f : now;
-      fix[x] = ex2(m[x] - safe);
-      m[x] = now;
-      top[x] = safe;
-      l[x] *= fix[x];
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
     }
-#pragma unroll
-    for (int n8 = 0; n8 < HD / 8; ++n8) {
-      o[n8][0] *= fix[0];
-      o[n8][1] *= fix[0];
-      o[n8][2] *= fix[1];
-      o[n8][3] *= fix[1];
+    if (c == 0) {
+      ml[warp * MT + g] = make_float2(m[0], l[0]);
+      ml[warp * MT + g + 8] = make_float2(m[1], l[1]);
     }
+    constexpr int D = HD / 32;
+    const int row = threadIdx.x >> 3, q = threadIdx.x & 7;
+    float acc[4][D], mx = -INFINITY, ls = 0.f, f[ROW_WARPS];
 #pragma unroll
-    for (int j = 0; j < KW / 16; ++j) {
-      uint32_t hi[4], lo[4];
+    for (int quarter = 0; quarter < 4; ++quarter) {
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {  // A fragment words: (row g, keys 0-7), (g + 8, 0-7), (g, 8-15), (g + 8, 8-15)
-        const int t = 2 * j + (y >> 1), x = y & 1;
-        const float a = ex2(sc[t][2 * x] - top[x]), b = ex2(sc[t][2 * x + 1] - top[x]);
-        l[x] += a + b;
-        hi[y] = Half16<DT>::pack(a, b);
-        const float2 h = Half16<DT>::unpack(hi[y]);
-        lo[y] = Half16<DT>::pack(a - h.x, b - h.y);
+      for (int j = 0; j < D; ++j) {
+        *reinterpret_cast<float2*>(os + (warp * MT + g) * S::JOIN + 8 * j + 2 * c) =
+            make_float2(o[quarter * D + j][0], o[quarter * D + j][1]);
+        *reinterpret_cast<float2*>(os + (warp * MT + g + 8) * S::JOIN + 8 * j + 2 * c) =
+            make_float2(o[quarter * D + j][2], o[quarter * D + j][3]);
+      }
+      row_barrier();
+      if (quarter == 0) {
+#pragma unroll
+        for (int w = 0; w < ROW_WARPS; ++w) mx = fmaxf(mx, ml[w * MT + row].x);
+        const float safe = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int w = 0; w < ROW_WARPS; ++w) {
+          const float2 t = ml[w * MT + row];
+          f[w] = ex2(t.x - safe);
+          ls += f[w] * t.y;
+        }
       }
 #pragma unroll
-      for (int n16 = 0; n16 < HD / 16; ++n16) {
-        const int row = warp * KW + 16 * j + vrow, ch = 2 * (n16 & 3) + vchunk;
-        uint32_t b[4];
-        ldsm4_t(b, va + (n16 >> 2) * S::HALF + row * 128 + ((ch ^ (row & 7)) << 4));
-        mma16<DT>(o[2 * n16], hi, b[0], b[1]);
-        mma16<DT>(o[2 * n16 + 1], hi, b[2], b[3]);
-        mma16<DT>(o[2 * n16], lo, b[0], b[1]);
-        mma16<DT>(o[2 * n16 + 1], lo, b[2], b[3]);
+      for (int d = 0; d < D; ++d) {
+        acc[quarter][d] = 0.f;
+#pragma unroll
+        for (int w = 0; w < ROW_WARPS; ++w) acc[quarter][d] += f[w] * os[(w * MT + row) * S::JOIN + q * D + d];
       }
+      row_barrier();
     }
-    if (ragged) fence_proxy_async();  // the zeros above, before the next copy into this stage
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[s]);
-  }
-  (void)ok;
-
-  // join the four warps: every stage has been read, the ring is free for their sums
+    const int r = r0 + row;
+    if (sg.parts > 1) {
+      auto keep = [&](int k) {  // dims of a thread: quarter * HD / 4 + q * D + d
+        if (r > r1) return;
+        float* part = p.parts + (size_t)part_place(sg, k) * PART;
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-  }
-  row_barrier();
-  constexpr int LD = HD + 4;
-  float* os = reinterpret_cast<float*>(ring);        // [4][16][LD]
-  float2* ml = reinterpret_cast<float2*>(os + ROW_WARPS * MT * LD);  // [4][16]
+        for (int quarter = 0; quarter < 4; ++quarter)
 #pragma unroll
-  for (int n8 = 0; n8 < HD / 8; ++n8) {
-    *reinterpret_cast<float2*>(os + (warp * MT + g) * LD + 8 * n8 + 2 * c) = make_float2(o[n8][0], o[n8][1]);
-    *reinterpret_cast<float2*>(os + (warp * MT + g + 8) * LD + 8 * n8 + 2 * c) = make_float2(o[n8][2], o[n8][3]);
-  }
-  if (c == 0) {
-    ml[warp * MT + g] = make_float2(m[0], l[0]);
-    ml[warp * MT + g + 8] = make_float2(m[1], l[1]);
-  }
-  row_barrier();
-  // 8 threads per row, HD / 8 dims each, as float4 q, q + 8, ...
-  const int row = threadIdx.x >> 3, q = threadIdx.x & 7;
-  float4 acc[HD / 32];
-  float mx = -INFINITY, ls = 0.f;
+          for (int d = 0; d < D; d += 2)
+            __stcg(reinterpret_cast<float2*>(part + row * HD + quarter * (HD / 4) + q * D + d),
+                   make_float2(acc[quarter][d], acc[quarter][d + 1]));
+        if (q == 0) __stcg(reinterpret_cast<float2*>(part + MT * HD) + row, make_float2(mx, ls));
+      };
+      keep(blockIdx.x - sg.lead);
+      // sums of parts first, first + step, ..., `count` of them, into acc, mx, ls
+      auto add_up = [&](int first, int step, int count) {
+        if (r > r1) return;
+        mx = -INFINITY;
+        for (int k = 0; k < count; ++k)
+          mx = fmaxf(mx, __ldcg(reinterpret_cast<const float2*>(
+                             p.parts + (size_t)part_place(sg, first + k * step) * PART + MT * HD) + row).x);
+        const float safe = mx == -INFINITY ? 0.f : mx;
+        ls = 0.f;
 #pragma unroll
-  for (int w = 0; w < ROW_WARPS; ++w) mx = fmaxf(mx, ml[w * MT + row].x);
-  const float safe = mx == -INFINITY ? 0.f : mx;
+        for (int quarter = 0; quarter < 4; ++quarter)
 #pragma unroll
-  for (int d = 0; d < HD / 32; ++d) acc[d] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int w = 0; w < ROW_WARPS; ++w) {
-    const float2 t = ml[w * MT + row];
-    const float f = ex2(t.x - safe);
-    ls += f * t.y;
-#pragma unroll
-    for (int d = 0; d < HD / 32; ++d) {
-      const float4 v = *reinterpret_cast<const float4*>(os + (w * MT + row) * LD + 4 * (q + 8 * d));
-      acc[d].x += f * v.x;
-      acc[d].y += f * v.y;
-      acc[d].z += f * v.z;
-      acc[d].w += f * v.w;
-    }
-  }
-  if (sh.splits > 1) {
-    float* part = p.parts + (size_t)(sh.part + sh.split) * MT * (HD + 2);
-#pragma unroll
-    for (int d = 0; d < HD / 32; ++d) __stcg(reinterpret_cast<float4*>(part + row * HD + 4 * (q + 8 * d)), acc[d]);
-    if (q == 0) __stcg(reinterpret_cast<float2*>(part + MT * HD) + row, make_float2(mx, ls));
-    __threadfence();
-    row_barrier();
-    __shared__ int last;
-    if (threadIdx.x == 0) {
-      last = atomicAdd(p.tickets + sh.ticket, 1u) == (unsigned)sh.splits - 1;
-      if (last) p.tickets[sh.ticket] = 0;
-      __threadfence();
-    }
-    row_barrier();
-    if (!last) return;
-    const float* parts = p.parts + (size_t)sh.part * MT * (HD + 2);
-    mx = -INFINITY;
-    for (int k = 0; k < sh.splits; ++k)
-      mx = fmaxf(mx, __ldcg(reinterpret_cast<const float2*>(parts + (size_t)k * MT * (HD + 2) + MT * HD) + row).x);
-    const float top = mx == -INFINITY ? 0.f : mx;
-    ls = 0.f;
-#pragma unroll
-    for (int d = 0; d < HD / 32; ++d) acc[d] = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int d = 0; d < D; ++d) acc[quarter][d] = 0.f;
 #pragma unroll 4
-    for (int k = 0; k < sh.splits; ++k) {
-      const float* at = parts + (size_t)k * MT * (HD + 2);
-      const float2 t = __ldcg(reinterpret_cast<const float2*>(at + MT * HD) + row);
-      const float f = ex2(t.x - top);
-      ls += f * t.y;
+        for (int k = 0; k < count; ++k) {
+          const float* at = p.parts + (size_t)part_place(sg, first + k * step) * PART;
+          const float2 t = __ldcg(reinterpret_cast<const float2*>(at + MT * HD) + row);
+          const float w = ex2(t.x - safe);
+          ls += w * t.y;
 #pragma unroll
-      for (int d = 0; d < HD / 32; ++d) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(at + row * HD + 4 * (q + 8 * d)));
-        acc[d].x += f * v.x;
-        acc[d].y += f * v.y;
-        acc[d].z += f * v.z;
-        acc[d].w += f * v.w;
+          for (int quarter = 0; quarter < 4; ++quarter)
+#pragma unroll
+            for (int d = 0; d < D; d += 2) {
+              const float2 v = __ldcg(reinterpret_cast<const float2*>(at + row * HD + quarter * (HD / 4) + q * D + d));
+              acc[quarter][d] += w * v.x;
+              acc[quarter][d + 1] += w * v.y;
+            }
+        }
+      };
+      // many parts are joined in two levels, so that no block reads more than a few
+      int step = 1, groups = sg.parts;
+      if (sg.parts > JOIN_AT_ONCE) {
+        step = JOIN_AT_ONCE;
+        groups = ceil_div(sg.parts, step);
+        const int first = (int)(blockIdx.x - sg.lead) / step * step, count = min(step, sg.parts - first);
+        if (!last_of<32 * ROW_WARPS>(p.tickets + p.slots + part_place(sg, first), count)) continue;
+        add_up(first, 1, count);
+        row_barrier();  // the group's first part has been read: the group's sums take its place
+        keep(first);
       }
+      if (!last_of<32 * ROW_WARPS>(p.tickets + sg.lead, groups)) continue;
+      add_up(0, step, groups);
+    }
+    if (r <= r1) {
+      const int t = r / p.group;
+      char* out = (char*)p.out + 2 * ((long long)(sg.first_row + t) * p.o_row +
+                                      (long long)(sg.kvh * p.group + r - t * p.group) * p.o_head + q * D);
+      const float inv = ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls);  // nothing seen: zero; NaN stays
+#pragma unroll
+      for (int quarter = 0; quarter < 4; ++quarter)
+#pragma unroll
+        for (int d = 0; d < D; d += 2)
+          *reinterpret_cast<uint32_t*>(out + 2 * (quarter * (HD / 4) + d)) =
+              Half16<DT>::pack(acc[quarter][d] * inv, acc[quarter][d + 1] * inv);
     }
   }
-  const int r = r0 + row;
-  if (r <= r1) {
-    const int t = r / p.group;
-    char* out = (char*)p.out + 2 * ((long long)(sh.first_row + t) * p.o_row +
-                                    (long long)(sh.kvh * p.group + r - t * p.group) * p.o_head);
-    const float inv = ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls);  // nothing seen: zero; NaN stays
-#pragma unroll
-    for (int d = 0; d < HD / 32; ++d)
-      *reinterpret_cast<uint2*>(out + 8 * (q + 8 * d)) =
-          make_uint2(Half16<DT>::pack(acc[d].x * inv, acc[d].y * inv), Half16<DT>::pack(acc[d].z * inv, acc[d].w * inv));
-  }
+  if (!ok && lane == 0) atomicCAS(p.error, 0, 0x202);
 }
 
 // ---- chunks ----------------------------------------------------------------------------------------
@@ -357,9 +405,9 @@ __global__ void __launch_bounds__(ROW_THREADS)
 constexpr int CT = 256;
 constexpr int CK = 128;
 constexpr int CHUNK_THREADS = 384;  // warps 0-3 tile A, 4-7 tile B, 8 TMA, 9 MMA, 10 and 11 only make 8 and 9 a warpgroup
-// Registers per thread: 384 x 168 at launch; the warps of the tiles, a row of scores each, take 224, the others 56
-// (256 x 224 + 128 x 56 = 384 x 168).
-constexpr int TILE_REGS = 224, OTHER_REGS = 56;
+// Registers per thread: 384 x 168 at launch; the warps of the tiles, a row of scores each, take 216, the others 72
+// (256 x 216 + 128 x 72 = 384 x 168).
+constexpr int TILE_REGS = 216, OTHER_REGS = 72;
 constexpr int MAX_SLOTS = 8;
 constexpr float LAZY = 8.f;  // log2 of the growth that is let pass
 
@@ -397,6 +445,37 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// The rows and key blocks of a segment, for both tiles together and for each: tile x computes the blocks i < to with
+// i < sinks or i >= from; those of whole_from .. whole_to - 1 need no mask.
+struct Tile {
+  int sinks, from, to, whole_from, whole_to;
+  __device__ __forceinline__ bool uses(int i) const { return i < to && (i < sinks || i >= from); }
+};
+struct Tiles {
+  int r0, r1, i0, i1;  // rows (inclusive), key blocks taken here
+  Keys all;
+  __device__ __forceinline__ Tiles(const AttendParams& p, const Segment& sg) {
+    r0 = sg.tile * CT;
+    r1 = min(r0 + CT, sg.fresh * p.group) - 1;
+    all = keys_of<CK>(p, sg, r0, r1);
+    i0 = (int)((long long)all.blocks * sg.v0 / sg.units);
+    i1 = (int)((long long)all.blocks * sg.v1 / sg.units);
+  }
+  __device__ __forceinline__ Tile tile(const AttendParams& p, const Segment& sg, int x) const {
+    Tile t;
+    const int a = r0 + 128 * x;
+    if (a > r1) return Tile{0, 0, 0, 0, 0};
+    const Keys k = keys_of<CK>(p, sg, a, min(a + 127, r1));
+    const int skip = all.sink_blocks - all.lo_block / CK;  // block i of the main range holds keys (i - skip) * CK ..
+    t.from = skip + k.lo / CK;
+    t.to = k.hi > 0 ? skip + ceil_div(k.hi, CK) : 0;
+    t.sinks = p.window ? max(all.sink_blocks, skip + ceil_div(p.sinks, CK)) : 0;
+    t.whole_from = p.window ? skip + max(k.p_last - p.window + CK, 0) / CK : 0;
+    t.whole_to = skip + max(p.causal ? min(k.hi, k.p_first + 1) : k.hi, 0) / CK;
+    return t;
+  }
+};
+
 template <int DT, int HD>
 __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -409,7 +488,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(qs + CT * HD * 2);
   uint64_t* empty = full + MAX_SLOTS;
   uint64_t* raw = empty + MAX_SLOTS;
-  uint64_t* sfull = raw + 1;   // [2] scores of a tile are in TMEM
+  uint64_t* qfull = raw + 1;    // [2] a tile's rows of Q are in shared memory
+  uint64_t* sfull = qfull + 2;  // [2] its scores are in TMEM
   uint64_t* pfull = sfull + 2;  // [2] its probabilities are
   uint64_t* ofull = pfull + 2;  // [2] its sums include them
   uint64_t* done = ofull + 2;
@@ -421,6 +501,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     }
     mbar_init(raw, 1);
     for (int x = 0; x < 2; ++x) {
+      mbar_init(&qfull[x], 4);
       mbar_init(&sfull[x], 1);
       mbar_init(&pfull[x], 4);
       mbar_init(&ofull[x], 1);
@@ -428,295 +509,289 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     mbar_init(done, 1);
     fence_mbar_init();
   }
-  Share sh;
-  if (!find_share<CT, CK, CHUNK_THREADS>(p, blockIdx.x, sh)) return;
-  sh.tile = (int)(((long long)sh.fresh * p.group + CT - 1) / CT) - 1 - sh.tile;  // the longest ones first
-  const int total = sh.fresh * p.group, r0 = sh.tile * CT, r1 = min(r0 + CT, total) - 1;
-  const Keys ks = keys_of<CK>(p, sh, r0, r1);
-  const int i0 = (int)((long long)ks.blocks * sh.split / sh.splits);
-  const int i1 = (int)((long long)ks.blocks * (sh.split + 1) / sh.splits);
-  // the keys that tile A and tile B see by themselves: blocks outside are not computed
-  const Keys ka = keys_of<CK>(p, sh, r0, min(r0 + 127, r1));
-  const bool has_b = r0 + 128 <= r1;
-  const Keys kb = has_b ? keys_of<CK>(p, sh, r0 + 128, r1) : ka;
-  auto uses = [&](int x, int i) {
-    const Keys& k = x ? kb : ka;
-    if (x && !has_b) return false;
-    const int key0 = block_key<CK>(ks, i);
-    return key0 < k.hi && (key0 + CK > k.lo || key0 < p.sinks);
-  };
+  Line line;
+  if (!find_line<CT, CK, CHUNK_THREADS>(p, line)) return;
+  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Walk<CT, CK> walk(p, line);
+  Segment sg;
 
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-  if (warp == 8) {
-    // producer: slots hold K, V, K, V, ... of blocks i0, i0 + 1, ...; lane j fetches the j-th page
-    const int rows_box = min(1 << p.shift, CK), boxes = CK / rows_box;
-    auto page_at = [&](int i) {
-      return lane < boxes ? page_of(p, ks, sh.b, (block_key<CK>(ks, i) >> p.shift) + lane) : -1;
-    };
-    int id = i0 < i1 ? page_at(i0) : -1;
-    bool ok = true;
-    int issued = 0;
-    for (int i = i0; i < i1 && ok; ++i) {
-      const int next = i + 1 < i1 ? page_at(i + 1) : -1;
-      const int key0 = block_key<CK>(ks, i), row = boxes > 1 ? 0 : key0 & ((1 << p.shift) - 1);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+    if (warp == 8) {
+      // producer: slots hold K, V, K, V, ... of the blocks in order; lane j fetches the j-th page
+      const int rows_box = min(1 << p.shift, CK), boxes = CK / rows_box;
+      bool ok = true;
+      int n = 0, raws = 0;
+      while (ok && walk.next(sg)) {
+        const Tiles tl(p, sg);
+        auto page_at = [&](int i) {
+          return lane < boxes ? page_of(p, tl.all, sg.b, (block_key<CK>(tl.all, i) >> p.shift) + lane) : -1;
+        };
+        int id = tl.i0 < tl.i1 ? page_at(tl.i0) : -1;
+        for (int i = tl.i0; i < tl.i1 && ok; ++i) {
+          const int next = i + 1 < tl.i1 ? page_at(i + 1) : -1;
+          const int key0 = block_key<CK>(tl.all, i), row = boxes > 1 ? 0 : key0 & ((1 << p.shift) - 1);
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const int n = 2 * (i - i0) + kv, s = n % SLOTS;
-        if (n >= SLOTS && !wait_bounded(&empty[s], ((n / SLOTS) & 1) ^ 1, p.timeout_ns)) {
-          atomicCAS(p.error, 0, 0x211);
-          ok = false;
-        }
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        // rows of V behind the last key may hold anything, and 0 * NaN is not 0: they are zeroed here
-        const bool ragged = kv == 1 && key0 + CK > ks.hi;
-        uint64_t* bar = ragged ? raw : &full[s];
-        if (lane == 0) mbar_expect_tx(bar, (uint32_t)S::TILE);
-        __syncwarp();
-        char* at = ring + s * S::TILE;
-        if (lane < boxes)
+          for (int kv = 0; kv < 2; ++kv, ++n) {
+            const int s = n % SLOTS;
+            if (n >= SLOTS) ok = wait_bounded(&empty[s], ((n / SLOTS) & 1) ^ 1, p.timeout_ns);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            // rows of V behind the last key may hold anything, and 0 * NaN is not 0: they are zeroed here
+            const bool ragged = kv == 1 && key0 + CK > tl.all.hi;
+            uint64_t* bar = ragged ? raw : &full[s];
+            if (lane == 0) mbar_expect_tx(bar, (uint32_t)S::TILE);
+            __syncwarp();
+            char* at = ring + s * S::TILE;
+            if (lane < boxes)
 #pragma unroll
-          for (int h = 0; h < HD / 64; ++h)
-            tma_load_4d(at + h * S::HALF + lane * rows_box * 128, kv ? &tv : &tk, 64 * h, row, sh.kvh, id, bar);
-        issued = n + 1;
-        if (ragged) {  // only the last block
-          ok = __all_sync(0xffffffffu, wait_bounded(raw, 0, p.timeout_ns));
-          if (!ok) {
-            if (lane == 0) atomicCAS(p.error, 0, 0x212);
-            break;
+              for (int h = 0; h < HD / 64; ++h)
+                tma_load_4d(at + h * S::HALF + lane * rows_box * 128, kv ? &tv : &tk, 64 * h, row, sg.kvh, id, bar);
+            if (ragged) {  // a tile's last block
+              ok = __all_sync(0xffffffffu, wait_bounded(raw, raws & 1, p.timeout_ns));
+              ++raws;
+              for (int e = lane + (tl.all.hi - key0) * (HD / 8); e < CK * (HD / 8); e += 32) {
+                const int r = e / (HD / 8), ch = e % (HD / 8);
+                *reinterpret_cast<uint4*>(at + (ch >> 3) * S::HALF + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+              }
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&full[s]);
+            }
           }
-          for (int e = lane + (ks.hi - key0) * (HD / 8); e < CK * (HD / 8); e += 32) {
-            const int r = e / (HD / 8), ch = e % (HD / 8);
-            *reinterpret_cast<uint4*>(at + (ch >> 3) * S::HALF + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full[s]);
+          id = next;
         }
       }
-      id = next;
-    }
-    if (!ok && lane == 0)  // let what is in flight land before the block ends
-      for (int n = max(0, issued - SLOTS); n < issued; ++n)
-        wait_bounded(&full[n % SLOTS], (n / SLOTS) & 1, p.timeout_ns);
-  } else if (warp == 9) {
-    tmem_alloc(tmem_slot, 512);
-    asm volatile("bar.sync 2, 288;" ::: "memory");  // Q is in shared memory
-    tmem_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    if (lane == 0) {
+      if (!ok && lane == 0) {  // a wait ran out: let what is in flight land before the block ends
+        atomicCAS(p.error, 0, 0x211);
+        for (int k = max(0, n - SLOTS); k < n; ++k) wait_bounded(&full[k % SLOTS], (k / SLOTS) & 1, p.timeout_ns);
+      }
+    } else if (warp == 9 && lane == 0) {
       constexpr uint32_t fmt = DT == MKX_BF16 ? 1u : 0u;
       const uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(128 >> 4) << 24);
       const uint32_t id_qk = base | ((uint32_t)(CK >> 3) << 17);
       const uint32_t id_pv = base | ((uint32_t)(HD >> 3) << 17) | (1u << 16);  // V: dims contiguous
-      int uses_of[2] = {0, 0};
-      bool pending[2] = {false, false}, ok = true;
-      for (int i = i0; i <= i1 && ok; ++i) {
-        const int nk = 2 * (i - i0), nv = nk - 1;  // places of K(i) and V(i - 1)
+      int uses_of[2] = {0, 0}, segments[2] = {0, 0}, place = 0;
+      bool ok = true;
+      while (ok && walk.next(sg)) {
+        const Tiles tl(p, sg);
+        const Tile tx[2] = {tl.tile(p, sg, 0), tl.tile(p, sg, 1)};
+        bool pending[2] = {false, false}, begun[2] = {false, false}, asked[2] = {false, false};
+        for (int i = tl.i0; i <= tl.i1 && ok; ++i) {
+          const int nk = place + 2 * (i - tl.i0), nv = nk - 1;  // places of K(i) and V(i - 1)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const uint32_t st = tmem + 128 * x, ot = tmem + 256 + 128 * x;
-          if (pending[x] && ok) {
-            ok = wait_bounded(&pfull[x], (uses_of[x] - 1) & 1, p.timeout_ns) &&
-                 wait_bounded(&full[nv % SLOTS], (nv / SLOTS) & 1, p.timeout_ns);
-            if (!ok) break;
-            tmem_fence_after();
-            const uint32_t v = smem_u32(ring + (nv % SLOTS) * S::TILE);
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t st = tmem + 128 * x, ot = tmem + 256 + 128 * x;
+            if (pending[x] && ok) {
+              ok = wait_bounded(&pfull[x], (uses_of[x] - 1) & 1, p.timeout_ns) &&
+                   wait_bounded(&full[nv % SLOTS], (nv / SLOTS) & 1, p.timeout_ns);
+              if (!ok) break;
+              tmem_fence_after();
+              const uint32_t v = smem_u32(ring + (nv % SLOTS) * S::TILE);
 #pragma unroll
-            for (int kk = 0; kk < CK / 16; ++kk)
-              umma_ts(ot, st + 8 * kk, sw128_mn_desc(v + 2048 * kk, S::HALF), id_pv, (uses_of[x] > 1 || kk > 0) ? 1u : 0u);
-            umma_commit(&ofull[x]);
-            pending[x] = false;
+              for (int kk = 0; kk < CK / 16; ++kk)
+                umma_ts(ot, st + 8 * kk, sw128_mn_desc(v + 2048 * kk, S::HALF), id_pv, (begun[x] || kk > 0) ? 1u : 0u);
+              umma_commit(&ofull[x]);
+              pending[x] = false;
+              begun[x] = true;
+            }
+            if (x == 1 && i > tl.i0) umma_commit(&empty[nv % SLOTS]);
+            if (i < tl.i1 && tx[x].uses(i)) {
+              if (!asked[x]) ok = wait_bounded(&qfull[x], segments[x]++ & 1, p.timeout_ns);
+              asked[x] = true;
+              ok = ok && wait_bounded(&full[nk % SLOTS], (nk / SLOTS) & 1, p.timeout_ns);
+              if (!ok) break;
+              tmem_fence_after();
+              const uint32_t k = smem_u32(ring + (nk % SLOTS) * S::TILE), q = smem_u32(qs) + x * 128 * 128;
+#pragma unroll
+              for (int kk = 0; kk < HD / 16; ++kk)
+                umma_bf16(st, sw128_desc(q + (kk >> 2) * S::QHALF + 32 * (kk & 3)),
+                          sw128_desc(k + (kk >> 2) * S::HALF + 32 * (kk & 3)), id_qk, kk > 0 ? 1u : 0u);
+              umma_commit(&sfull[x]);
+              pending[x] = true;
+              ++uses_of[x];
+            }
           }
-          if (x == 1 && i > i0) umma_commit(&empty[nv % SLOTS]);
-          if (i < i1 && uses(x, i)) {
-            ok = wait_bounded(&full[nk % SLOTS], (nk / SLOTS) & 1, p.timeout_ns);
-            if (!ok) break;
-            tmem_fence_after();
-            const uint32_t k = smem_u32(ring + (nk % SLOTS) * S::TILE), q = smem_u32(qs) + x * 128 * 128;
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk)
-              umma_bf16(st, sw128_desc(q + (kk >> 2) * S::QHALF + 32 * (kk & 3)),
-                        sw128_desc(k + (kk >> 2) * S::HALF + 32 * (kk & 3)), id_qk, kk > 0 ? 1u : 0u);
-            umma_commit(&sfull[x]);
-            pending[x] = true;
-            ++uses_of[x];
-          }
+          if (i < tl.i1) umma_commit(&empty[nk % SLOTS]);
         }
-        if (i < i1) umma_commit(&empty[nk % SLOTS]);
+        place += 2 * (tl.i1 - tl.i0);
       }
       if (!ok) atomicCAS(p.error, 0, 0x213);
       umma_commit(done);
     }
     __syncwarp();
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TILE_REGS));
-    // Q into shared memory, coalesced: 16-byte chunks of a row by neighbouring threads
-    for (int e = threadIdx.x; e < CT * (HD / 8); e += 256) {
-      const int row = e / (HD / 8), ch = e % (HD / 8), r = r0 + row;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r <= r1) {
-        const int t = r / p.group;
-        v = __ldg(reinterpret_cast<const uint4*>((const char*)p.q +
-                                                 2 * ((long long)(sh.first_row + t) * p.q_row +
-                                                      (long long)(sh.kvh * p.group + r - t * p.group) * p.q_head + 8 * ch)));
-        v = make_uint4(signed_q(p, v.x), signed_q(p, v.y), signed_q(p, v.z), signed_q(p, v.w));
-      }
-      *reinterpret_cast<uint4*>(qs + (ch >> 3) * S::QHALF + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = v;
-    }
-    fence_proxy_async();
-    asm volatile("bar.sync 2, 288;" ::: "memory");
-    tmem_fence_after();
     const int x = warp >> 2, row = threadIdx.x;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t st = *tmem_slot + lanes + 128 * x, ot = *tmem_slot + lanes + 256 + 128 * x;
-    const Keys& kx = x ? kb : ka;
-    const int position = sh.past + (r0 + row) / p.group;
-    float m = -INFINITY, l = 0.f;
-    int n = 0;
+    const uint32_t st = tmem + lanes + 128 * x, ot = tmem + lanes + 256 + 128 * x;
+    int n = 0;  // blocks of this tile since the start
     bool ok = true;
-    for (int i = i0; i < i1; ++i) {
-      if (!uses(x, i)) continue;
-      ok = __all_sync(0xffffffffu, wait_bounded(&sfull[x], n & 1, p.timeout_ns));
-      if (!ok) break;
-      tmem_fence_after();
-      const int key0 = block_key<CK>(ks, i);
-      uint32_t s[4][32];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) tmem_ld32(st + 32 * j, s[j]);
-      if (!whole_block<CK>(p, kx, key0)) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t seen = seen_mask(p, kx, position, key0 + 32 * j);
-#pragma unroll
-          for (int d = 0; d < 32; ++d)
-            if (!((seen >> d) & 1u)) s[j][d] = 0xff800000u;
+    while (walk.next(sg)) {
+      const Tiles tl(p, sg);
+      const Tile tile = tl.tile(p, sg, x);
+      const int position = sg.past + (tl.r0 + row) / p.group;
+      float m = -INFINITY, l = 0.f;
+      bool begun = false;
+      const int n0 = n;
+      for (int i = tl.i0; i < tl.i1 && ok; ++i) {
+        if (!tile.uses(i)) continue;
+        if (!begun) {
+          // the tile's Q into shared memory, coalesced: 16-byte chunks of a row by neighbouring threads. Only for a
+          // tile with work in this segment: warps without any run ahead, by more phases than a barrier tells apart
+          for (int e = threadIdx.x - 128 * x; e < 128 * (HD / 8); e += 128) {
+            const int qr = 128 * x + e / (HD / 8), ch = e % (HD / 8), r = tl.r0 + qr;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r <= tl.r1) {
+              const int t = r / p.group;
+              v = __ldg(reinterpret_cast<const uint4*>((const char*)p.q +
+                                                       2 * ((long long)(sg.first_row + t) * p.q_row +
+                                                            (long long)(sg.kvh * p.group + r - t * p.group) * p.q_head + 8 * ch)));
+              v = make_uint4(signed_q(p, v.x), signed_q(p, v.y), signed_q(p, v.z), signed_q(p, v.w));
+            }
+            *reinterpret_cast<uint4*>(qs + (ch >> 3) * S::QHALF + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4)) = v;
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&qfull[x]);
+          begun = true;
         }
-      }
-      float top = -INFINITY;
+        ok = __all_sync(0xffffffffu, wait_bounded(&sfull[x], n & 1, p.timeout_ns));
+        if (!ok) break;
+        tmem_fence_after();
+        uint32_t s[4][32];
 #pragma unroll
-      for (int j = 0; j < 128; ++j) top = fmaxf(top, __uint_as_float(s[j >> 5][j & 31]));
-      top *= p.scale_log2;  // > 0: -inf stays
-      const bool grow = top > m + LAZY || (m == -INFINITY && top > m);
-      if (__any_sync(0xffffffffu, grow)) {
-        const float now = grow ? top : m, fix = grow ? ex2(m - now) : 1.f;
-        if (n > 0) {
-          ok = __all_sync(0xffffffffu, wait_bounded(&ofull[x], (n - 1) & 1, p.timeout_ns));
-          if (!ok) break;
-          tmem_fence_after();
+        for (int j = 0; j < 4; ++j) tmem_ld32(st + 32 * j, s[j]);
+        if (i < tile.whole_from || i >= tile.whole_to) {
+          const int key0 = block_key<CK>(tl.all, i);
 #pragma unroll
-          for (int j = 0; j < HD / 32; ++j) {
-            uint32_t o[32];
-            tmem_ld32(ot + 32 * j, o);
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t seen = seen_mask(p, tl.all, position, key0 + 32 * j);
 #pragma unroll
-            for (int d = 0; d < 32; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * fix);
-            tmem_st32(ot + 32 * j, o);
+            for (int d = 0; d < 32; ++d)
+              if (!((seen >> d) & 1u)) s[j][d] = 0xff800000u;
           }
         }
-        l *= fix;
-        m = now;
-      }
-      const float base = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        float top = -INFINITY;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t w[32];
+        for (int j = 0; j < 128; ++j) top = fmaxf(top, __uint_as_float(s[j >> 5][j & 31]));
+        top *= p.scale_log2;  // > 0: -inf stays
+        const bool grow = top > m + LAZY || (m == -INFINITY && top > m);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float now = grow ? top : m, fix = grow ? ex2(m - now) : 1.f;
+          if (n > n0) {
+            ok = __all_sync(0xffffffffu, wait_bounded(&ofull[x], (n - 1) & 1, p.timeout_ns));
+            if (!ok) break;
+            tmem_fence_after();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const int e = 64 * h + 2 * j;
-          const uint32_t sa = s[e >> 5][e & 31], sb = s[(e + 1) >> 5][(e + 1) & 31];
-          const float a = ex2(fmaf(__uint_as_float(sa), p.scale_log2, -base));
-          const float b = ex2(fmaf(__uint_as_float(sb), p.scale_log2, -base));
-          sum[j & 3] += a + b;
-          w[j] = Half16<DT>::pack(a, b);
-        }
-        tmem_st32(st + 32 * h, w);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_wait_st();
-      tmem_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&pfull[x]);
-      ++n;
-    }
-    // epilogue
-    if (n > 0 && ok) {
-      ok = __all_sync(0xffffffffu, wait_bounded(&ofull[x], (n - 1) & 1, p.timeout_ns));
-      tmem_fence_after();
-    }
-    if (!ok && lane == 0) atomicCAS(p.error, 0, 0x214);
-    const int r = r0 + row, t = r / p.group;
-    char* out = (char*)p.out + 2 * ((long long)(sh.first_row + t) * p.o_row +
-                                    (long long)(sh.kvh * p.group + r - t * p.group) * p.o_head);
-    auto scale_of = [](float ls) { return ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls); };  // nothing seen: zero; NaN stays
-    auto write = [&](const float (&o)[32], int j, float inv) {
+            for (int j = 0; j < HD / 32; ++j) {
+              uint32_t o[32];
+              tmem_ld32(ot + 32 * j, o);
 #pragma unroll
-      for (int d = 0; d < 32; d += 8)
-        *reinterpret_cast<uint4*>(out + 2 * (32 * j + d)) =
-            make_uint4(Half16<DT>::pack(o[d] * inv, o[d + 1] * inv), Half16<DT>::pack(o[d + 2] * inv, o[d + 3] * inv),
-                       Half16<DT>::pack(o[d + 4] * inv, o[d + 5] * inv), Half16<DT>::pack(o[d + 6] * inv, o[d + 7] * inv));
-    };
-    constexpr int PART = CT * (HD + 2);  // [HD / 4][256 rows] float4, then (maximum, total) of each row
-    float* part = p.parts + (size_t)(sh.part + sh.split) * PART;
-#pragma unroll
-    for (int j = 0; j < HD / 32; ++j) {
-      uint32_t u[32];
-      float o[32];
-#pragma unroll
-      for (int d = 0; d < 32; ++d) u[d] = 0u;
-      if (n > 0 && ok) tmem_ld32(ot + 32 * j, u);  // warp-uniform
-#pragma unroll
-      for (int d = 0; d < 32; ++d) o[d] = __uint_as_float(u[d]);
-      if (sh.splits > 1) {
-#pragma unroll
-        for (int d = 0; d < 32; d += 4)
-          __stcg(reinterpret_cast<float4*>(part + ((size_t)(8 * j + d / 4) * CT + row) * 4),
-                 make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]));
-      } else if (r <= r1) {
-        write(o, j, scale_of(l));
-      }
-    }
-    if (sh.splits > 1) {
-      __stcg(reinterpret_cast<float2*>(part + (size_t)CT * HD) + row, make_float2(m, l));
-      __threadfence();
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      __shared__ int last;
-      if (threadIdx.x == 0) {
-        last = atomicAdd(p.tickets + sh.ticket, 1u) == (unsigned)sh.splits - 1;
-        if (last) p.tickets[sh.ticket] = 0;
-        __threadfence();
-      }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (last && r <= r1) {
-        const float* parts = p.parts + (size_t)sh.part * PART;
-        float top = -INFINITY, ls = 0.f;
-        for (int k = 0; k < sh.splits; ++k)
-          top = fmaxf(top, __ldcg(reinterpret_cast<const float2*>(parts + (size_t)k * PART + CT * HD) + row).x);
-        const float base = top == -INFINITY ? 0.f : top;
-        for (int k = 0; k < sh.splits; ++k) {
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(parts + (size_t)k * PART + CT * HD) + row);
-          ls += ex2(ml.x - base) * ml.y;
-        }
-        const float inv = scale_of(ls);
-        for (int j = 0; j < HD / 32; ++j) {
-          float o[32];
-#pragma unroll
-          for (int d = 0; d < 32; ++d) o[d] = 0.f;
-          for (int k = 0; k < sh.splits; ++k) {
-            const float* at = parts + (size_t)k * PART;
-            const float f = ex2(__ldcg(reinterpret_cast<const float2*>(at + CT * HD) + row).x - base);
-#pragma unroll
-            for (int d = 0; d < 32; d += 4) {
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(at + ((size_t)(8 * j + d / 4) * CT + row) * 4));
-              o[d] += f * v.x;
-              o[d + 1] += f * v.y;
-              o[d + 2] += f * v.z;
-              o[d + 3] += f * v.w;
+              for (int d = 0; d < 32; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * fix);
+              tmem_st32(ot + 32 * j, o);
             }
           }
-          write(o, j, inv);
+          l *= fix;
+          m = now;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int e = 64 * h + 2 * j;
+            const uint32_t sa = s[e >> 5][e & 31], sb = s[(e + 1) >> 5][(e + 1) & 31];
+            const float a = ex2(fmaf(__uint_as_float(sa), p.scale_log2, -base));
+            const float b = ex2(fmaf(__uint_as_float(sb), p.scale_log2, -base));
+            sum[j & 3] += a + b;
+            w[j] = Half16<DT>::pack(a, b);
+          }
+          tmem_st32(st + 32 * h, w);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pfull[x]);
+        ++n;
+      }
+      // the tile's sums: out, or into this block's part
+      const bool any = n > n0;
+      if (any && ok) {
+        ok = __all_sync(0xffffffffu, wait_bounded(&ofull[x], (n - 1) & 1, p.timeout_ns));
+        tmem_fence_after();
+      }
+      if (!ok && lane == 0) atomicCAS(p.error, 0, 0x214);
+      const int r = tl.r0 + row, t = r / p.group;
+      char* out = (char*)p.out + 2 * ((long long)(sg.first_row + t) * p.o_row +
+                                      (long long)(sg.kvh * p.group + r - t * p.group) * p.o_head);
+      auto scale_of = [](float ls) { return ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls); };  // nothing seen: zero; NaN stays
+      auto write = [&](const float (&o)[32], int j, float inv) {
+#pragma unroll
+        for (int d = 0; d < 32; d += 8)
+          *reinterpret_cast<uint4*>(out + 2 * (32 * j + d)) =
+              make_uint4(Half16<DT>::pack(o[d] * inv, o[d + 1] * inv), Half16<DT>::pack(o[d + 2] * inv, o[d + 3] * inv),
+                         Half16<DT>::pack(o[d + 4] * inv, o[d + 5] * inv), Half16<DT>::pack(o[d + 6] * inv, o[d + 7] * inv));
+      };
+      constexpr int PART = CT * (HD + 2);  // [HD / 4][256 rows] float4, then (maximum, total) of each row
+      float* part = p.parts + (size_t)part_place(sg, blockIdx.x - sg.lead) * PART;
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) {
+        uint32_t u[32];
+        float o[32];
+#pragma unroll
+        for (int d = 0; d < 32; ++d) u[d] = 0u;
+        if (any && ok) tmem_ld32(ot + 32 * j, u);  // warp-uniform
+#pragma unroll
+        for (int d = 0; d < 32; ++d) o[d] = __uint_as_float(u[d]);
+        if (sg.parts > 1) {
+#pragma unroll
+          for (int d = 0; d < 32; d += 4)
+            __stcg(reinterpret_cast<float4*>(part + ((size_t)(8 * j + d / 4) * CT + row) * 4),
+                   make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]));
+        } else if (r <= tl.r1) {
+          write(o, j, scale_of(l));
+        }
+      }
+      tmem_fence_before();
+      if (sg.parts > 1) {
+        __stcg(reinterpret_cast<float2*>(part + (size_t)CT * HD) + row, make_float2(m, l));
+        if (last_of<256>(p.tickets + sg.lead, sg.parts) && r <= tl.r1) {
+          float top = -INFINITY, ls = 0.f;
+          auto ml_of = [&](int k) {
+            return __ldcg(reinterpret_cast<const float2*>(p.parts + (size_t)part_place(sg, k) * PART + CT * HD) + row);
+          };
+          for (int k = 0; k < sg.parts; ++k) top = fmaxf(top, ml_of(k).x);
+          const float base = top == -INFINITY ? 0.f : top;
+          for (int k = 0; k < sg.parts; ++k) {
+            const float2 ml = ml_of(k);
+            ls += ex2(ml.x - base) * ml.y;
+          }
+          const float inv = scale_of(ls);
+          for (int j = 0; j < HD / 32; ++j) {
+            float o[32];
+#pragma unroll
+            for (int d = 0; d < 32; ++d) o[d] = 0.f;
+            for (int k = 0; k < sg.parts; ++k) {
+              const float* at = p.parts + (size_t)part_place(sg, k) * PART;
+              const float f = ex2(ml_of(k).x - base);
+#pragma unroll
+              for (int d = 0; d < 32; d += 4) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(at + ((size_t)(8 * j + d / 4) * CT + row) * 4));
+                o[d] += f * v.x;
+                o[d + 1] += f * v.y;
+                o[d + 2] += f * v.z;
+                o[d + 3] += f * v.w;
+              }
+            }
+            write(o, j, inv);
+          }
         }
       }
     }
@@ -726,7 +801,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   if (warp == 9) {
     wait_bounded(done, 0, p.timeout_ns);  // no MMA may still write
     tmem_fence_after();
-    tmem_free(*tmem_slot, 512);
+    tmem_free(tmem, 512);
   }
 }
 
@@ -746,8 +821,8 @@ bool encode_pages(CUtensorMap* m, const void* base, int dtype, int head_dim, int
 
 struct Plan {
   bool chunk;
-  int mt, kt, slots, max_parts;
-  long long grid;
+  int kt;     // key blocks
+  int slots;  // blocks of the grid
   size_t bytes;
 };
 
@@ -762,35 +837,28 @@ bool plan_of(const mkx_attend_inputs& a, int sms, Plan& pl) {
   const long long most = a.max_rows < a.rows ? a.max_rows : a.rows;
   // rows of one K/V head and episode beyond one 16-row tile would read the pages again: chunk_kernel
   pl.chunk = most * group > MT;
-  pl.mt = pl.chunk ? CT : MT;
   pl.kt = pl.chunk ? CK : 8192 / a.head_dim;
   pl.slots = pl.chunk ? sms : 2 * sms;
-  // tiles <= the rows' tiles plus one per episode, and <= episodes x the tiles of the largest
-  long long tiles = (a.rows * group) / pl.mt + a.B;
-  const long long by_most = a.B * ((most * group + pl.mt - 1) / pl.mt);
-  if (by_most < tiles) tiles = by_most;
-  pl.grid = tiles * a.kv_heads + pl.slots;
-  pl.max_parts = 2 * pl.slots + 2;
-  pl.bytes = MKX_ATTEND_TICKETS * 4 + (size_t)pl.max_parts * pl.mt * (a.head_dim + 2) * 4;
-  return pl.grid < (1ll << 31);
+  pl.bytes = MKX_ATTEND_TICKETS * 4 + (size_t)2 * pl.slots * (pl.chunk ? CT : MT) * (a.head_dim + 2) * 4;
+  return 3 * pl.slots <= MKX_ATTEND_TICKETS && (long long)a.rows * group < MAX_KEYS;
 }
 
 template <typename Kernel>
 bool launch(Kernel kernel, bool (&sized)[MAX_DEVICES], int threads, int smem, const CUtensorMap& tk, const CUtensorMap& tv,
-            const AttendParams& p, long long grid, int device, cudaStream_t stream) {
+            const AttendParams& p, int device, cudaStream_t stream) {
   if (!sized[device]) {  // the attribute of a kernel is set once per device
     if (!mkxc::cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))) return false;
     sized[device] = true;
   }
-  kernel<<<(unsigned)grid, threads, smem, stream>>>(tk, tv, p);
+  kernel<<<(unsigned)p.slots, threads, smem, stream>>>(tk, tv, p);
   return mkxc::cuda_ok(cudaGetLastError());
 }
 template <int DT, int HD>
-bool launch_typed(bool chunk, const CUtensorMap& tk, const CUtensorMap& tv, const AttendParams& p, long long grid, int device,
+bool launch_typed(bool chunk, const CUtensorMap& tk, const CUtensorMap& tv, const AttendParams& p, int device,
                   cudaStream_t stream) {
   static bool rows_sized[MAX_DEVICES] = {}, chunk_sized[MAX_DEVICES] = {};
-  return chunk ? launch(chunk_kernel<DT, HD>, chunk_sized, CHUNK_THREADS, ChunkShape<HD>::SMEM, tk, tv, p, grid, device, stream)
-               : launch(rows_kernel<DT, HD>, rows_sized, ROW_THREADS, RowShape<HD>::SMEM, tk, tv, p, grid, device, stream);
+  return chunk ? launch(chunk_kernel<DT, HD>, chunk_sized, CHUNK_THREADS, ChunkShape<HD>::SMEM, tk, tv, p, device, stream)
+               : launch(rows_kernel<DT, HD>, rows_sized, ROW_THREADS, RowShape<HD>::SMEM, tk, tv, p, device, stream);
 }
 
 }  // namespace
@@ -868,14 +936,14 @@ extern "C" mkx_status mkx_cache_attend(const mkx_attend_inputs* in, size_t works
   p.q_and = a.scale == 0.f ? 0u : ~0u;
   p.q_xor = a.scale < 0.f ? 0x80008000u : 0u;
   p.slots = pl.slots;
-  p.min_blocks = 2;
-  p.max_parts = pl.max_parts;
+  p.min_units = 2;
+  p.snap = 2;
   p.timeout_ns = 2000000000ull;
   const bool ok =
       a.head_dim == 64
-          ? (a.dtype == MKX_BF16 ? launch_typed<MKX_BF16, 64>(pl.chunk, tk, tv, p, pl.grid, device, stream)
-                                 : launch_typed<MKX_FP16, 64>(pl.chunk, tk, tv, p, pl.grid, device, stream))
-          : (a.dtype == MKX_BF16 ? launch_typed<MKX_BF16, 128>(pl.chunk, tk, tv, p, pl.grid, device, stream)
-                                 : launch_typed<MKX_FP16, 128>(pl.chunk, tk, tv, p, pl.grid, device, stream));
+          ? (a.dtype == MKX_BF16 ? launch_typed<MKX_BF16, 64>(pl.chunk, tk, tv, p, device, stream)
+                                 : launch_typed<MKX_FP16, 64>(pl.chunk, tk, tv, p, device, stream))
+          : (a.dtype == MKX_BF16 ? launch_typed<MKX_BF16, 128>(pl.chunk, tk, tv, p, device, stream)
+                                 : launch_typed<MKX_FP16, 128>(pl.chunk, tk, tv, p, device, stream));
   return ok ? MKX_OK : MKX_ERR_CUDA;
 }

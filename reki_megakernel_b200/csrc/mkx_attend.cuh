@@ -1,5 +1,5 @@
-// What the attention kernels of the paged episode cache share: which share of the work a block takes,
-// which keys its rows see, the tensor maps of the pages, and the join of the parts of a split tile.
+// What the attention kernels of the paged episode cache share: which stretch of the work a block takes,
+// which keys its rows see, and the exchange between blocks that share a tile.
 #pragma once
 #include <stdint.h>
 #include <cuda_runtime.h>
@@ -17,42 +17,34 @@ struct AttendParams {
   void* out;
   const int *table, *length, *start;
   unsigned* tickets;  // [MKX_ATTEND_TICKETS], zero between calls
-  float* parts;       // [max_parts][tile rows][HD + 2]: unnormalised sums, then (maximum, total)
+  float* parts;       // [2 slots][tile rows x (HD + 2)]: unnormalised sums, then (maximum, total) of each row
   int* error;
   long long q_row, q_head, o_row, o_head;
   int rows, B, heads, kv_heads, group, pages, shift, table_width, max_rows;
   int causal, window, sinks;
   float scale_log2;       // |scale| * log2(e): scores are kept in powers of two
   uint32_t q_and, q_xor;  // q's words as they enter: the sign of a negative scale, nothing for scale 0
-  int slots;         // blocks that the call's work is meant to be spread over
-  int min_blocks;    // key blocks that a part has at least
-  int max_parts;
+  int slots;      // blocks of the grid
+  int min_units;  // key blocks that one block takes at least
+  int snap;       // units by which a cut may move to a tile's end
   unsigned long long timeout_ns;
-};
-
-// One block's share: part `split` of `splits` of the key blocks of row tile `tile` of (episode, head).
-struct Share {
-  int b, kvh, tile, split, splits;
-  int first_row, fresh, length, past;  // of the episode: row of q, new rows, rows held, position of row 0
-  int part, ticket;                    // of the tile (splits > 1)
 };
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
+// An episode's new rows, its row tiles (MT rows of (new row, head of the group)) and the most key blocks
+// (KT keys) that one of its tiles sees.
 struct Episode {
-  int first_row, fresh, length, past, tiles, blocks;
+  int first_row, fresh, length, past, tiles, units;
 };
 
-// An episode's new rows, row tiles (MT rows of (new row, head of the group)) and the most key blocks
-// (KT keys) that one of its tiles sees.
 template <int MT, int KT>
-__device__ __forceinline__ Episode episode_of(const AttendParams& p, int b) {
+__device__ __forceinline__ Episode episode_from(const AttendParams& p, int first_row, int next, int length) {
   Episode e;
-  e.first_row = p.start[b];
-  const int next = p.start[b + 1];
-  e.length = max(p.length[b], 0);
-  e.past = e.length - max(next - e.first_row, 0);
-  e.fresh = (e.first_row < 0 || next > p.rows) ? 0 : min(max(next - e.first_row, 0), p.max_rows);
+  e.first_row = first_row;
+  e.length = max(length, 0);
+  e.past = e.length - max(next - first_row, 0);
+  e.fresh = (first_row < 0 || next > p.rows) ? 0 : min(max(next - first_row, 0), p.max_rows);
   e.tiles = (int)(((long long)e.fresh * p.group + MT - 1) / MT);
   const long long keys = min((long long)e.length, (long long)p.table_width << p.shift);
   long long blocks = (keys + KT - 1) / KT;
@@ -60,104 +52,188 @@ __device__ __forceinline__ Episode episode_of(const AttendParams& p, int b) {
     const long long span = (long long)p.window + min(e.fresh, MT / p.group + 2);
     blocks = min(blocks, (span + KT - 1) / KT + 1 + ((long long)p.sinks + KT - 1) / KT);
   }
-  e.blocks = (int)max(blocks, 1ll);
+  e.units = (int)max(blocks, 1ll);
   return e;
 }
+template <int MT, int KT>
+__device__ __forceinline__ Episode episode_of(const AttendParams& p, int b) {
+  return episode_from<MT, KT>(p, p.start[b], p.start[b + 1], p.length[b]);
+}
 
-// Every block works out its share by itself from the B lengths. The work is cut into parts of at most
-// `cut` key blocks, cut = all key blocks of all tiles / slots, so that a call with few tiles (single rows,
-// few heads) still fills the GPU, and one with many is not split at all. Splits are the same for all
-// tiles of an episode: a part is found by a prefix over the episodes.
-// NTH threads, all call. Returns false if there is no share left for this block.
+// The work of a call is a line of units, one for each key block of each row tile, K/V head and episode.
+// Block c of the grid takes the units from cut c to cut c + 1; the cuts divide the line evenly, but one
+// within `snap` units of a tile's end moves there, because a tile in two parts has to be joined, which
+// costs about as much as that many units. So tiles of any lengths fill the GPU evenly, short ones stay
+// whole, and a long one alone is spread over all blocks. The last block of a tile to finish joins its
+// parts. Each role of a block walks the line by itself: no exchange, and the copies run ahead of the
+// arithmetic across tiles.
+struct Segment {
+  int b, kvh, tile;
+  int first_row, fresh, length, past;  // of the episode
+  int v0, v1, units;                   // units of the tile taken here
+  int lead, parts;                     // first block of the tile, number of blocks (parts > 1: to be joined)
+};
+
+struct Line {
+  long long total, at, begin, end;  // units; first unit of the episode that the stretch begins in; the stretch
+  int blocks, b;                    // blocks that the line is cut for; that episode
+};
+
+__device__ __forceinline__ long long snapped(long long u, long long at, int units, int snap) {
+  const int v = (int)((unsigned long long)(u - at) % (unsigned)units);
+  return v <= snap ? u - v : units - v <= snap ? u + (units - v) : u;
+}
+
+// All threads of the block call this; false if the block has nothing to do.
 template <int MT, int KT, int NTH>
-__device__ __forceinline__ bool find_share(const AttendParams& p, long long item, Share& out) {
+__device__ __forceinline__ bool find_line(const AttendParams& p, Line& out) {
   constexpr int W = NTH / 32;
-  __shared__ long long sums[W];
-  __shared__ int3 warp_sums[W];
-  __shared__ Share found;
+  __shared__ long long sums[2][W];
+  __shared__ Line line;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long all = 0;
+  Episode e;
+  long long all = 0, mine = 0;
   for (int b = threadIdx.x; b < p.B; b += NTH) {
-    const Episode e = episode_of<MT, KT>(p, b);
-    all += (long long)e.tiles * p.kv_heads * e.blocks;
+    const Episode x = episode_of<MT, KT>(p, b);
+    const long long units = (long long)x.tiles * p.kv_heads * x.units;
+    all += units;
+    if (b == (int)threadIdx.x) {
+      e = x;
+      mine = units;
+    }
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
-  if (lane == 0) sums[warp] = all;
-  if (threadIdx.x == 0) found.b = -1;
+  if (lane == 0) sums[0][warp] = all;
   __syncthreads();
   all = 0;
 #pragma unroll
-  for (int w = 0; w < W; ++w) all += sums[w];
-  const int cut = (int)max((long long)p.min_blocks, (all + p.slots - 1) / p.slots);
-  int3 before = make_int3(0, 0, 0);  // items, parts of split tiles, split tiles of earlier episodes
-  for (int b0 = 0; b0 < p.B; b0 += NTH) {
+  for (int w = 0; w < W; ++w) all += sums[0][w];
+  const int blocks = (int)min((long long)p.slots, all / p.min_units + 1);
+  if (all == 0 || (int)blockIdx.x >= blocks) return false;
+  const long long u0 = all * blockIdx.x / blocks, u1 = all * (blockIdx.x + 1) / blocks;
+  if (threadIdx.x == 0) line.end = all;
+  long long before = 0;
+  for (int b0 = 0;; b0 += NTH) {  // ends: u0 < all
     const int b = b0 + threadIdx.x;
-    Episode e;
-    e.tiles = 0;
-    int splits = 1;
-    int3 v = make_int3(0, 0, 0);
-    if (b < p.B) {
-      e = episode_of<MT, KT>(p, b);
-      splits = ceil_div(e.blocks, cut);
-      v.x = e.tiles * p.kv_heads * splits;
-      if (splits > 1) {
-        v.y = v.x;
-        v.z = e.tiles * p.kv_heads;
+    if (b0 > 0) {
+      mine = 0;
+      if (b < p.B) {
+        e = episode_of<MT, KT>(p, b);
+        mine = (long long)e.tiles * p.kv_heads * e.units;
       }
     }
-    int3 inc = v;
+    long long inc = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, inc.x, d), y = __shfl_up_sync(0xffffffffu, inc.y, d),
-                z = __shfl_up_sync(0xffffffffu, inc.z, d);
-      if (lane >= d) {
-        inc.x += x;
-        inc.y += y;
-        inc.z += z;
-      }
+      const long long o = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += o;
     }
-    if (lane == 31) warp_sums[warp] = inc;
+    if (b0 > 0) __syncthreads();  // the sums have been read
+    if (lane == 31) sums[1][warp] = inc;
     __syncthreads();
-    int3 base = before;
+    long long at = before + inc - mine;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const int3 s = warp_sums[w];
-      if (w < warp) {
-        base.x += s.x;
-        base.y += s.y;
-        base.z += s.z;
-      }
-      before.x += s.x;
-      before.y += s.y;
-      before.z += s.z;
+      if (w < warp) at += sums[1][w];
+      before += sums[1][w];
     }
-    const int mine = base.x + inc.x - v.x;
-    if (item >= mine && item < mine + v.x) {
-      const int local = (int)(item - mine);
-      Share s;
-      s.b = b;
-      s.kvh = local % p.kv_heads;
-      const int rest = local / p.kv_heads;
-      s.split = rest % splits;
-      s.tile = rest / splits;
-      s.splits = splits;
-      s.first_row = e.first_row;
-      s.fresh = e.fresh;
-      s.length = e.length;
-      s.past = e.past;
-      const int t = s.tile * p.kv_heads + s.kvh;
-      s.part = base.y + inc.y - v.y + t * splits;
-      s.ticket = base.z + inc.z - v.z + t;
-      found = s;
+    if (u0 >= at && u0 < at + mine) {
+      line.total = all;
+      line.at = at;
+      line.begin = snapped(u0, at, e.units, p.snap);
+      line.blocks = blocks;
+      line.b = b;
     }
-    __syncthreads();
-    if (before.x > item) break;
+    if (u1 >= at && u1 < at + mine) line.end = snapped(u1, at, e.units, p.snap);
+    if (before > u1 || before >= all) break;
   }
-  out = found;
-  // (a `start` that is no prefix could ask for more parts than there are: those tiles stay unwritten)
-  return out.b >= 0 && (out.splits == 1 || ((unsigned)(out.part + out.splits) <= (unsigned)p.max_parts &&
-                                            (unsigned)out.ticket < MKX_ATTEND_TICKETS));
+  __syncthreads();
+  out = line;
+  return out.begin < out.end;
+}
+
+template <int MT, int KT>
+struct Walk {
+  const AttendParams& p;
+  long long total, left, tile_at;  // units of the line; units left of the stretch; first unit of the tile
+  int blocks, b, kvh, tile, v;     // place: unit v of the tile
+  Episode e;
+  int n_first, n_next, n_length;   // of episode b + 1, asked for ahead
+
+  __device__ __forceinline__ Walk(const AttendParams& params, const Line& l)
+      : p(params), total(l.total), left(l.end - l.begin), blocks(l.blocks), b(l.b) {
+    e = episode_of<MT, KT>(p, b);
+    ask();
+    // the stretch may begin behind the episode's last unit: then the first next() goes on
+    const long long local = l.begin - l.at, t = local / e.units;
+    v = (int)(local - t * e.units);
+    tile_at = l.begin - v;
+    kvh = (int)(t / e.tiles);
+    tile = e.tiles - 1 - (int)(t - (long long)kvh * e.tiles);
+  }
+  __device__ __forceinline__ void ask() {
+    const int n = min(b + 1, p.B - 1);
+    n_first = p.start[n];
+    n_next = p.start[n + 1];
+    n_length = p.length[n];
+  }
+  // The last block whose cut lies at or before `unit`.
+  __device__ __forceinline__ int block_at(long long unit) const { return (int)(((unit + 1) * blocks - 1) / total); }
+  __device__ __forceinline__ bool next(Segment& s) {
+    if (left <= 0) return false;
+    while (kvh >= p.kv_heads || e.tiles == 0) {
+      if (++b >= p.B) return false;
+      e = episode_from<MT, KT>(p, n_first, n_next, n_length);
+      ask();
+      kvh = 0;
+      tile = e.tiles - 1;
+    }
+    s.b = b;
+    s.kvh = kvh;
+    s.tile = tile;
+    s.first_row = e.first_row;
+    s.fresh = e.fresh;
+    s.length = e.length;
+    s.past = e.past;
+    s.units = e.units;
+    s.v0 = v;
+    s.v1 = (int)min((long long)e.units, v + left);
+    s.lead = blockIdx.x;
+    s.parts = 1;
+    if (s.v0 > 0 || s.v1 < s.units) {
+      s.lead = block_at(tile_at + min(p.snap, s.units - 1));
+      s.parts = block_at(tile_at + s.units - p.snap - 1) - s.lead + 1;
+    }
+    left -= s.v1 - s.v0;
+    tile_at += s.units;
+    v = 0;
+    if (--tile < 0) {
+      tile = e.tiles - 1;
+      ++kvh;
+    }
+    return true;
+  }
+};
+
+// A block keeps at most two parts: of the tile its stretch begins inside of, and of the one it ends inside of.
+__device__ __forceinline__ int part_place(const Segment& s, int k) { return 2 * (s.lead + k) + (k == 0); }
+
+// Called by all NTH threads (named barrier 1) after they wrote their part k of a split tile with __stcg: whether
+// this block is the last of the parts [k0, k0 + n) under ticket `ticket`, which is left at zero. The others' parts are
+// then visible through __ldcg.
+template <int NTH>
+__device__ __forceinline__ bool last_of(unsigned* ticket, int n) {
+  __shared__ int last;
+  __threadfence();
+  asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");
+  if (threadIdx.x == 0) {
+    last = atomicAdd(ticket, 1u) == (unsigned)n - 1;
+    if (last) *ticket = 0;
+    __threadfence();
+  }
+  asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");
+  return last;
 }
 
 // The keys that the rows of a tile see: blocks of KT keys, first those of the sinks, then from the
@@ -171,7 +247,7 @@ struct Keys {
 };
 
 template <int KT>
-__device__ __forceinline__ Keys keys_of(const AttendParams& p, const Share& s, int r0, int r1) {
+__device__ __forceinline__ Keys keys_of(const AttendParams& p, const Segment& s, int r0, int r1) {
   Keys k;
   k.p_first = s.past + r0 / p.group;
   k.p_last = s.past + r1 / p.group;
