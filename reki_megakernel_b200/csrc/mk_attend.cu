@@ -404,11 +404,12 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
 // tiles, whose products take 1024), by both alike at 128.
 constexpr int CT = 256;
 constexpr int CK = 128;
-constexpr int CHUNK_THREADS = 384;  // warps 0-3 tile A, 4-7 tile B, 8 TMA, 9 MMA, 10 and 11 only make 8 and 9 a warpgroup
+constexpr int CHUNK_THREADS = 384;  // warps 0-3 tile A, 4-7 tile B, 8 TMA, 9 MMA, 10 walks the line, 11 fills the warpgroup
 // Registers per thread: 384 x 168 at launch; the warps of the tiles, a row of scores each, take 216, the others 72
 // (256 x 216 + 128 x 72 = 384 x 168).
 constexpr int TILE_REGS = 216, OTHER_REGS = 72;
 constexpr int MAX_SLOTS = 8;
+constexpr bool POLY = true;
 constexpr float LAZY = 8.f;  // log2 of the growth that is let pass
 
 template <int HD>
@@ -417,7 +418,7 @@ struct ChunkShape {
   static constexpr int HALF = CK * 128;                 // its 64-dim half
   static constexpr int SLOTS = HD == 128 ? 5 : 8;
   static constexpr int QHALF = CT * 128;
-  static constexpr int SMEM = SLOTS * TILE + CT * HD * 2 + 1024 + 256;
+  static constexpr int SMEM = SLOTS * TILE + CT * HD * 2 + 1024 + 320;
 };
 
 // A 64-dim half of V is 128 keys x 128 bytes, 128-byte swizzle, dims contiguous ("MN-major" B operand):
@@ -433,6 +434,41 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, 
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(d),
       "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
 }
+// Lanes 32 (warp % 4) .. + 31, 128 columns: a row of scores per thread.
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&v)[128]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, "
+      "%38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, "
+      "%56, %57, %58, %59, %60, %61, %62, %63, %64, %65, %66, %67, %68, %69, %70, %71, %72, %73, "
+      "%74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, "
+      "%92, %93, %94, %95, %96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, "
+      "%108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, "
+      "%123, %124, %125, %126, %127 "
+      "}, [%128];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
+        "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+        "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]), "=r"(v[32]), "=r"(v[33]), "=r"(v[34]),
+        "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]), "=r"(v[40]), "=r"(v[41]),
+        "=r"(v[42]), "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]), "=r"(v[48]),
+        "=r"(v[49]), "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]),
+        "=r"(v[56]), "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]),
+        "=r"(v[63]), "=r"(v[64]), "=r"(v[65]), "=r"(v[66]), "=r"(v[67]), "=r"(v[68]), "=r"(v[69]),
+        "=r"(v[70]), "=r"(v[71]), "=r"(v[72]), "=r"(v[73]), "=r"(v[74]), "=r"(v[75]), "=r"(v[76]),
+        "=r"(v[77]), "=r"(v[78]), "=r"(v[79]), "=r"(v[80]), "=r"(v[81]), "=r"(v[82]), "=r"(v[83]),
+        "=r"(v[84]), "=r"(v[85]), "=r"(v[86]), "=r"(v[87]), "=r"(v[88]), "=r"(v[89]), "=r"(v[90]),
+        "=r"(v[91]), "=r"(v[92]), "=r"(v[93]), "=r"(v[94]), "=r"(v[95]), "=r"(v[96]), "=r"(v[97]),
+        "=r"(v[98]), "=r"(v[99]), "=r"(v[100]), "=r"(v[101]), "=r"(v[102]), "=r"(v[103]),
+        "=r"(v[104]), "=r"(v[105]), "=r"(v[106]), "=r"(v[107]), "=r"(v[108]), "=r"(v[109]),
+        "=r"(v[110]), "=r"(v[111]), "=r"(v[112]), "=r"(v[113]), "=r"(v[114]), "=r"(v[115]),
+        "=r"(v[116]), "=r"(v[117]), "=r"(v[118]), "=r"(v[119]), "=r"(v[120]), "=r"(v[121]),
+        "=r"(v[122]), "=r"(v[123]), "=r"(v[124]), "=r"(v[125]), "=r"(v[126]), "=r"(v[127])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -445,36 +481,89 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// The rows and key blocks of a segment, for both tiles together and for each: tile x computes the blocks i < to with
-// i < sinks or i >= from; those of whole_from .. whole_to - 1 need no mask.
+// Two floats at a time on the fp32 pipe.
+__device__ __forceinline__ uint64_t f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unf2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x of two floats without the exponential unit, for x <= 126: 2^x = 2^n 2^f with n the nearest integer (adding
+// 1.5 * 2^23 leaves it in the low bits), |f| <= 1/2, and 2^f by a polynomial whose relative error is the smallest
+// possible with constant term 1 (so that x = -inf, taken as -127, gives 0): 1.0e-4 in degree 3, a fortieth of half a
+// bf16 step, 2.8e-6 in degree 4, for fp16.
+template <int DT>
+__device__ __forceinline__ float2 exp2_pair(uint64_t x2) {
+  const float2 x = unf2(x2);
+  x2 = f2(fmaxf(x.x, -127.f), fmaxf(x.y, -127.f));
+  const uint64_t magic = f2(12582912.f, 12582912.f);
+  const uint64_t r2 = add2(x2, magic);
+  const uint64_t f = fma2(add2(r2, f2(-12582912.f, -12582912.f)), f2(-1.f, -1.f), x2);
+  uint64_t y;
+  if constexpr (DT == MKX_BF16) {
+    y = fma2(f2(0.05500893294811249f, 0.05500893294811249f), f, f2(0.24221095442771912f, 0.24221095442771912f));
+    y = fma2(y, f, f2(0.6932829022407532f, 0.6932829022407532f));
+  } else {
+    y = fma2(f2(0.009582852944731712f, 0.009582852944731712f), f, f2(0.055906426161527634f, 0.055906426161527634f));
+    y = fma2(y, f, f2(0.24024099111557007f, 0.24024099111557007f));
+    y = fma2(y, f, f2(0.6931241750717163f, 0.6931241750717163f));
+  }
+  const float2 v = unf2(fma2(y, f, f2(1.f, 1.f))), r = unf2(r2);
+  return make_float2(__int_as_float(__float_as_int(v.x) + (__float_as_int(r.x) << 23)),
+                     __int_as_float(__float_as_int(v.y) + (__float_as_int(r.y) << 23)));
+}
+
+// What every role needs to know of a segment, worked out once by a warp of its own and handed on in shared memory.
+// Tile x computes the blocks i < to with i < sinks or i >= from; those of whole_from .. whole_to - 1 need no mask.
 struct Tile {
   int sinks, from, to, whole_from, whole_to;
   __device__ __forceinline__ bool uses(int i) const { return i < to && (i < sinks || i >= from); }
 };
-struct Tiles {
-  int r0, r1, i0, i1;  // rows (inclusive), key blocks taken here
-  Keys all;
-  __device__ __forceinline__ Tiles(const AttendParams& p, const Segment& sg) {
-    r0 = sg.tile * CT;
-    r1 = min(r0 + CT, sg.fresh * p.group) - 1;
-    all = keys_of<CK>(p, sg, r0, r1);
-    i0 = (int)((long long)all.blocks * sg.v0 / sg.units);
-    i1 = (int)((long long)all.blocks * sg.v1 / sg.units);
-  }
-  __device__ __forceinline__ Tile tile(const AttendParams& p, const Segment& sg, int x) const {
-    Tile t;
-    const int a = r0 + 128 * x;
-    if (a > r1) return Tile{0, 0, 0, 0, 0};
-    const Keys k = keys_of<CK>(p, sg, a, min(a + 127, r1));
-    const int skip = all.sink_blocks - all.lo_block / CK;  // block i of the main range holds keys (i - skip) * CK ..
-    t.from = skip + k.lo / CK;
-    t.to = k.hi > 0 ? skip + ceil_div(k.hi, CK) : 0;
-    t.sinks = p.window ? max(all.sink_blocks, skip + ceil_div(p.sinks, CK)) : 0;
-    t.whole_from = p.window ? skip + max(k.p_last - p.window + CK, 0) / CK : 0;
-    t.whole_to = skip + max(p.causal ? min(k.hi, k.p_first + 1) : k.hi, 0) / CK;
-    return t;
-  }
+struct Job {
+  Segment sg;
+  int r0, r1, i0, i1;  // rows (inclusive), key blocks taken here; i0 < 0: no more jobs
+  Keys keys;           // of both tiles together
+  Tile tile[2];
 };
+__device__ __forceinline__ void fill(const AttendParams& p, Job& job, const Segment& sg) {
+  const int r0 = sg.tile * CT, r1 = min(r0 + CT, sg.fresh * p.group) - 1;
+  const Keys all = keys_of<CK>(p, sg, r0, r1);
+  job.sg = sg;
+  job.r0 = r0;
+  job.r1 = r1;
+  job.i0 = (int)((long long)all.blocks * sg.v0 / sg.units);
+  job.i1 = (int)((long long)all.blocks * sg.v1 / sg.units);
+  job.keys = all;
+  for (int x = 0; x < 2; ++x) {
+    Tile t{0, 0, 0, 0, 0};
+    const int a = r0 + 128 * x;
+    if (a <= r1) {
+      const Keys k = keys_of<CK>(p, sg, a, min(a + 127, r1));
+      const int skip = all.sink_blocks - all.lo_block / CK;  // block i of the main range holds keys (i - skip) * CK ..
+      t.from = skip + k.lo / CK;
+      t.to = k.hi > 0 ? skip + ceil_div(k.hi, CK) : 0;
+      t.sinks = p.window ? max(all.sink_blocks, skip + ceil_div(p.sinks, CK)) : 0;
+      t.whole_from = p.window ? skip + max(k.p_last - p.window + CK, 0) / CK : 0;
+      t.whole_to = skip + max(p.causal ? min(k.hi, k.p_first + 1) : k.hi, 0) / CK;
+    }
+    job.tile[x] = t;
+  }
+}
+constexpr int JOBS = 4;
 
 template <int DT, int HD>
 __global__ void __launch_bounds__(CHUNK_THREADS, 1)
@@ -490,10 +579,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   uint64_t* raw = empty + MAX_SLOTS;
   uint64_t* qfull = raw + 1;    // [2] a tile's rows of Q are in shared memory
   uint64_t* sfull = qfull + 2;  // [2] its scores are in TMEM
-  uint64_t* pfull = sfull + 2;  // [2] its probabilities are
-  uint64_t* ofull = pfull + 2;  // [2] its sums include them
+  uint64_t* pfull = sfull + 2;  // [2][2] the first, the second half of its probabilities are
+  uint64_t* ofull = pfull + 4;  // [2] its sums include them
   uint64_t* done = ofull + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* jfull = done + 1;      // [JOBS]
+  uint64_t* jempty = jfull + JOBS;  // [JOBS]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(jempty + JOBS);
+  __shared__ Job jobs[JOBS];
   if (threadIdx.x == 0) {
     for (int s = 0; s < SLOTS; ++s) {
       mbar_init(&full[s], 1);
@@ -503,10 +595,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     for (int x = 0; x < 2; ++x) {
       mbar_init(&qfull[x], 4);
       mbar_init(&sfull[x], 1);
-      mbar_init(&pfull[x], 4);
+      mbar_init(&pfull[2 * x], 4);
+      mbar_init(&pfull[2 * x + 1], 4);
       mbar_init(&ofull[x], 1);
     }
     mbar_init(done, 1);
+    for (int j = 0; j < JOBS; ++j) {
+      mbar_init(&jfull[j], 1);
+      mbar_init(&jempty[j], 10);  // the producer, the MMA warp, the eight warps of the tiles
+    }
     fence_mbar_init();
   }
   Line line;
@@ -515,8 +612,6 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Walk<CT, CK> walk(p, line);
-  Segment sg;
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
@@ -525,15 +620,22 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       const int rows_box = min(1 << p.shift, CK), boxes = CK / rows_box;
       bool ok = true;
       int n = 0, raws = 0;
-      while (ok && walk.next(sg)) {
-        const Tiles tl(p, sg);
+      for (int jn = 0; ok; ++jn) {
+        ok = __all_sync(0xffffffffu, wait_bounded(&jfull[jn % JOBS], (jn / JOBS) & 1, p.timeout_ns));
+        if (!ok) break;
+        const Job& job = jobs[jn % JOBS];
+        const int i0 = job.i0, i1 = job.i1, b = job.sg.b, kvh = job.sg.kvh;
+        const Keys ks = job.keys;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&jempty[jn % JOBS]);
+        if (i0 < 0) break;
         auto page_at = [&](int i) {
-          return lane < boxes ? page_of(p, tl.all, sg.b, (block_key<CK>(tl.all, i) >> p.shift) + lane) : -1;
+          return lane < boxes ? page_of(p, ks, b, (block_key<CK>(ks, i) >> p.shift) + lane) : -1;
         };
-        int id = tl.i0 < tl.i1 ? page_at(tl.i0) : -1;
-        for (int i = tl.i0; i < tl.i1 && ok; ++i) {
-          const int next = i + 1 < tl.i1 ? page_at(i + 1) : -1;
-          const int key0 = block_key<CK>(tl.all, i), row = boxes > 1 ? 0 : key0 & ((1 << p.shift) - 1);
+        int id = i0 < i1 ? page_at(i0) : -1;
+        for (int i = i0; i < i1 && ok; ++i) {
+          const int next = i + 1 < i1 ? page_at(i + 1) : -1;
+          const int key0 = block_key<CK>(ks, i), row = boxes > 1 ? 0 : key0 & ((1 << p.shift) - 1);
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv, ++n) {
             const int s = n % SLOTS;
@@ -541,7 +643,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             // rows of V behind the last key may hold anything, and 0 * NaN is not 0: they are zeroed here
-            const bool ragged = kv == 1 && key0 + CK > tl.all.hi;
+            const bool ragged = kv == 1 && key0 + CK > ks.hi;
             uint64_t* bar = ragged ? raw : &full[s];
             if (lane == 0) mbar_expect_tx(bar, (uint32_t)S::TILE);
             __syncwarp();
@@ -549,11 +651,11 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             if (lane < boxes)
 #pragma unroll
               for (int h = 0; h < HD / 64; ++h)
-                tma_load_4d(at + h * S::HALF + lane * rows_box * 128, kv ? &tv : &tk, 64 * h, row, sg.kvh, id, bar);
+                tma_load_4d(at + h * S::HALF + lane * rows_box * 128, kv ? &tv : &tk, 64 * h, row, kvh, id, bar);
             if (ragged) {  // a tile's last block
               ok = __all_sync(0xffffffffu, wait_bounded(raw, raws & 1, p.timeout_ns));
               ++raws;
-              for (int e = lane + (tl.all.hi - key0) * (HD / 8); e < CK * (HD / 8); e += 32) {
+              for (int e = lane + (ks.hi - key0) * (HD / 8); e < CK * (HD / 8); e += 32) {
                 const int r = e / (HD / 8), ch = e % (HD / 8);
                 *reinterpret_cast<uint4*>(at + (ch >> 3) * S::HALF + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
               }
@@ -576,30 +678,39 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       const uint32_t id_pv = base | ((uint32_t)(HD >> 3) << 17) | (1u << 16);  // V: dims contiguous
       int uses_of[2] = {0, 0}, segments[2] = {0, 0}, place = 0;
       bool ok = true;
-      while (ok && walk.next(sg)) {
-        const Tiles tl(p, sg);
-        const Tile tx[2] = {tl.tile(p, sg, 0), tl.tile(p, sg, 1)};
+      for (int jn = 0; ok; ++jn) {
+        ok = wait_bounded(&jfull[jn % JOBS], (jn / JOBS) & 1, p.timeout_ns);
+        if (!ok) break;
+        const Job& job = jobs[jn % JOBS];
+        const int i0 = job.i0, i1 = job.i1;
+        const Tile tiles[2] = {job.tile[0], job.tile[1]};
+        mbar_arrive(&jempty[jn % JOBS]);
+        if (i0 < 0) break;
         bool pending[2] = {false, false}, begun[2] = {false, false}, asked[2] = {false, false};
-        for (int i = tl.i0; i <= tl.i1 && ok; ++i) {
-          const int nk = place + 2 * (i - tl.i0), nv = nk - 1;  // places of K(i) and V(i - 1)
+        for (int i = i0; i <= i1 && ok; ++i) {
+          const int nk = place + 2 * (i - i0), nv = nk - 1;  // places of K(i) and V(i - 1)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const uint32_t st = tmem + 128 * x, ot = tmem + 256 + 128 * x;
             if (pending[x] && ok) {
-              ok = wait_bounded(&pfull[x], (uses_of[x] - 1) & 1, p.timeout_ns) &&
-                   wait_bounded(&full[nv % SLOTS], (nv / SLOTS) & 1, p.timeout_ns);
-              if (!ok) break;
-              tmem_fence_after();
+              ok = wait_bounded(&full[nv % SLOTS], (nv / SLOTS) & 1, p.timeout_ns);
               const uint32_t v = smem_u32(ring + (nv % SLOTS) * S::TILE);
 #pragma unroll
-              for (int kk = 0; kk < CK / 16; ++kk)
-                umma_ts(ot, st + 8 * kk, sw128_mn_desc(v + 2048 * kk, S::HALF), id_pv, (begun[x] || kk > 0) ? 1u : 0u);
+              for (int half = 0; half < 2; ++half) {
+                ok = ok && wait_bounded(&pfull[2 * x + half], (uses_of[x] - 1) & 1, p.timeout_ns);
+                if (!ok) break;
+                tmem_fence_after();
+#pragma unroll
+                for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                  umma_ts(ot, st + 8 * kk, sw128_mn_desc(v + 2048 * kk, S::HALF), id_pv, (begun[x] || kk > 0) ? 1u : 0u);
+              }
+              if (!ok) break;
               umma_commit(&ofull[x]);
               pending[x] = false;
               begun[x] = true;
             }
-            if (x == 1 && i > tl.i0) umma_commit(&empty[nv % SLOTS]);
-            if (i < tl.i1 && tx[x].uses(i)) {
+            if (x == 1 && i > i0) umma_commit(&empty[nv % SLOTS]);
+            if (i < i1 && tiles[x].uses(i)) {
               if (!asked[x]) ok = wait_bounded(&qfull[x], segments[x]++ & 1, p.timeout_ns);
               asked[x] = true;
               ok = ok && wait_bounded(&full[nk % SLOTS], (nk / SLOTS) & 1, p.timeout_ns);
@@ -615,12 +726,27 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
               ++uses_of[x];
             }
           }
-          if (i < tl.i1) umma_commit(&empty[nk % SLOTS]);
+          if (i < i1) umma_commit(&empty[nk % SLOTS]);
         }
-        place += 2 * (tl.i1 - tl.i0);
+        place += 2 * (i1 - i0);
       }
       if (!ok) atomicCAS(p.error, 0, 0x213);
       umma_commit(done);
+    } else if (warp == 10 && lane == 0) {
+      // walks the line
+      Walk<CT, CK> walk(p, line);
+      Segment sg;
+      for (int jn = 0;; ++jn) {
+        const bool more = walk.next(sg);
+        if (jn >= JOBS && !wait_bounded(&jempty[jn % JOBS], ((jn / JOBS) & 1) ^ 1, p.timeout_ns)) {
+          atomicCAS(p.error, 0, 0x215);
+          break;
+        }
+        if (more) fill(p, jobs[jn % JOBS], sg);
+        else jobs[jn % JOBS].i0 = -1;
+        mbar_arrive(&jfull[jn % JOBS]);
+        if (!more) break;
+      }
     }
     __syncwarp();
   } else {
@@ -628,28 +754,31 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     const int x = warp >> 2, row = threadIdx.x;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t st = tmem + lanes + 128 * x, ot = tmem + lanes + 256 + 128 * x;
+    const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
     int n = 0;  // blocks of this tile since the start
     bool ok = true;
-    while (walk.next(sg)) {
-      const Tiles tl(p, sg);
-      const Tile tile = tl.tile(p, sg, x);
-      const int position = sg.past + (tl.r0 + row) / p.group;
+    for (int jn = 0; ok; ++jn) {
+      ok = __all_sync(0xffffffffu, wait_bounded(&jfull[jn % JOBS], (jn / JOBS) & 1, p.timeout_ns));
+      if (!ok) break;
+      const Job& job = jobs[jn % JOBS];
+      const int i0 = job.i0, i1 = job.i1;
+      if (i0 < 0) break;
+      const Tile tile = job.tile[x];
       float m = -INFINITY, l = 0.f;
-      bool begun = false;
       const int n0 = n;
-      for (int i = tl.i0; i < tl.i1 && ok; ++i) {
+      for (int i = i0; i < i1 && ok; ++i) {
         if (!tile.uses(i)) continue;
-        if (!begun) {
+        if (n == n0) {
           // the tile's Q into shared memory, coalesced: 16-byte chunks of a row by neighbouring threads. Only for a
           // tile with work in this segment: warps without any run ahead, by more phases than a barrier tells apart
           for (int e = threadIdx.x - 128 * x; e < 128 * (HD / 8); e += 128) {
-            const int qr = 128 * x + e / (HD / 8), ch = e % (HD / 8), r = tl.r0 + qr;
+            const int qr = 128 * x + e / (HD / 8), ch = e % (HD / 8), r = job.r0 + qr;
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (r <= tl.r1) {
+            if (r <= job.r1) {
               const int t = r / p.group;
-              v = __ldg(reinterpret_cast<const uint4*>((const char*)p.q +
-                                                       2 * ((long long)(sg.first_row + t) * p.q_row +
-                                                            (long long)(sg.kvh * p.group + r - t * p.group) * p.q_head + 8 * ch)));
+              v = __ldg(reinterpret_cast<const uint4*>(
+                  (const char*)p.q + 2 * ((long long)(job.sg.first_row + t) * p.q_row +
+                                          (long long)(job.sg.kvh * p.group + r - t * p.group) * p.q_head + 8 * ch)));
               v = make_uint4(signed_q(p, v.x), signed_q(p, v.y), signed_q(p, v.z), signed_q(p, v.w));
             }
             *reinterpret_cast<uint4*>(qs + (ch >> 3) * S::QHALF + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4)) = v;
@@ -657,28 +786,33 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) mbar_arrive(&qfull[x]);
-          begun = true;
         }
         ok = __all_sync(0xffffffffu, wait_bounded(&sfull[x], n & 1, p.timeout_ns));
         if (!ok) break;
         tmem_fence_after();
-        uint32_t s[4][32];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) tmem_ld32(st + 32 * j, s[j]);
+        uint32_t s[128];
+        tmem_ld128(st, s);
         if (i < tile.whole_from || i >= tile.whole_to) {
-          const int key0 = block_key<CK>(tl.all, i);
+          const int key0 = block_key<CK>(job.keys, i), position = job.sg.past + (job.r0 + row) / p.group;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint32_t seen = seen_mask(p, tl.all, position, key0 + 32 * j);
+            const uint32_t seen = seen_mask(p, job.keys, position, key0 + 32 * j);
 #pragma unroll
             for (int d = 0; d < 32; ++d)
-              if (!((seen >> d) & 1u)) s[j][d] = 0xff800000u;
+              if (!((seen >> d) & 1u)) s[32 * j + d] = 0xff800000u;
           }
         }
-        float top = -INFINITY;
+        float tops[8];
 #pragma unroll
-        for (int j = 0; j < 128; ++j) top = fmaxf(top, __uint_as_float(s[j >> 5][j & 31]));
-        top *= p.scale_log2;  // > 0: -inf stays
+        for (int k = 0; k < 8; ++k) tops[k] = fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 8]));
+#pragma unroll
+        for (int j = 16; j < 128; j += 16)
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            tops[k] = fmaxf(fmaxf(tops[k], __uint_as_float(s[j + k])), __uint_as_float(s[j + k + 8]));
+        const float top = p.scale_log2 *  // > 0: -inf stays
+                          fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
+                                fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
         const bool grow = top > m + LAZY || (m == -INFINITY && top > m);
         if (__any_sync(0xffffffffu, grow)) {
           const float now = grow ? top : m, fix = grow ? ex2(m - now) : 1.f;
@@ -699,26 +833,33 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           m = now;
         }
         const float base = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t base2 = f2(-base, -base);
+        uint64_t sums[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int half = 0; half < 2; ++half) {
           uint32_t w[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const int e = 64 * h + 2 * j;
-            const uint32_t sa = s[e >> 5][e & 31], sb = s[(e + 1) >> 5][(e + 1) & 31];
-            const float a = ex2(fmaf(__uint_as_float(sa), p.scale_log2, -base));
-            const float b = ex2(fmaf(__uint_as_float(sb), p.scale_log2, -base));
-            sum[j & 3] += a + b;
-            w[j] = Half16<DT>::pack(a, b);
+            const int e = 64 * half + 2 * j;
+            const uint64_t y = fma2(f2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, base2);
+            float2 v;
+            if ((j & 3) == 3 && POLY) {
+              v = exp2_pair<DT>(y);
+            } else {
+              v = unf2(y);
+              v = make_float2(ex2(v.x), ex2(v.y));
+            }
+            sums[j & 3] = add2(sums[j & 3], f2(v.x, v.y));
+            w[j] = Half16<DT>::pack(v.x, v.y);
           }
-          tmem_st32(st + 32 * h, w);
+          tmem_st32(st + 32 * half, w);
+          tmem_wait_st();
+          tmem_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pfull[2 * x + half]);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_wait_st();
-        tmem_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&pfull[x]);
+        const float2 total = unf2(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+        l += total.x + total.y;
         ++n;
       }
       // the tile's sums: out, or into this block's part
@@ -727,8 +868,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         ok = __all_sync(0xffffffffu, wait_bounded(&ofull[x], (n - 1) & 1, p.timeout_ns));
         tmem_fence_after();
       }
-      if (!ok && lane == 0) atomicCAS(p.error, 0, 0x214);
-      const int r = tl.r0 + row, t = r / p.group;
+      const Segment sg = job.sg;
+      const int r1 = job.r1, r = job.r0 + row, t = r / p.group;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&jempty[jn % JOBS]);
       char* out = (char*)p.out + 2 * ((long long)(sg.first_row + t) * p.o_row +
                                       (long long)(sg.kvh * p.group + r - t * p.group) * p.o_head);
       auto scale_of = [](float ls) { return ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls); };  // nothing seen: zero; NaN stays
@@ -755,14 +898,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           for (int d = 0; d < 32; d += 4)
             __stcg(reinterpret_cast<float4*>(part + ((size_t)(8 * j + d / 4) * CT + row) * 4),
                    make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]));
-        } else if (r <= tl.r1) {
+        } else if (r <= r1) {
           write(o, j, scale_of(l));
         }
       }
       tmem_fence_before();
       if (sg.parts > 1) {
         __stcg(reinterpret_cast<float2*>(part + (size_t)CT * HD) + row, make_float2(m, l));
-        if (last_of<256>(p.tickets + sg.lead, sg.parts) && r <= tl.r1) {
+        if (last_of<256>(p.tickets + sg.lead, sg.parts) && r <= r1) {
           float top = -INFINITY, ls = 0.f;
           auto ml_of = [&](int k) {
             return __ldcg(reinterpret_cast<const float2*>(p.parts + (size_t)part_place(sg, k) * PART + CT * HD) + row);
@@ -795,6 +938,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         }
       }
     }
+    if (!ok && lane == 0) atomicCAS(p.error, 0, 0x214);
     tmem_fence_before();
   }
   __syncthreads();
