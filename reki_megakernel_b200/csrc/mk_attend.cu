@@ -421,19 +421,47 @@ struct ChunkShape {
   static constexpr int SMEM = SLOTS * TILE + CT * HD * 2 + 1024 + 320;
 };
 
-// A 64-dim half of V is 128 keys x 128 bytes, 128-byte swizzle, dims contiguous ("MN-major" B operand):
-// 8-key groups are 1024 bytes apart (stride offset), the 64-dim halves HALF bytes (leading offset).
-__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t addr, uint32_t half_bytes) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(half_bytes >> 4) << 16) | ((uint64_t)64 << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Shared-memory matrix descriptors in two words: the low one (address and leading offset, both / 16) changes from
+// product to product by additions, the high one (stride offset 1024 between 8-row groups, version 1, 128-byte
+// swizzle) is one constant. Q and K are K-major (leading offset unused). A 64-dim half of V is 128 keys x 128 bytes with
+// the dims contiguous ("MN-major" B operand): 8-key groups are a stride offset apart, the halves a leading offset.
+constexpr uint32_t DESC_HIGH = 64u | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t leading) {
+  return ((addr >> 4) & 0x3FFFu) | ((leading >> 4) << 16);
+}
+// The MMA warp stays converged, so that descriptors live in uniform registers (one thread by itself moves six
+// registers per product, 100 clocks for a product of 64): the instruction is predicated on its one elected lane.
+// D[tmem] (+)= A[smem] * B[smem]^T, K = 16.
+__device__ __forceinline__ void umma_ss(uint32_t lead, uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 a, {%1, %6};\n\tmov.b64 b, {%2, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(lead), "n"(DESC_HIGH));
 }
 // D[tmem] (+)= A[tmem] * B[smem]: A is 128 lanes x 16 16-bit values in 8 columns.
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b_low, uint32_t idesc,
+                                        uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 b, {%2, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(lead), "n"(DESC_HIGH));
 }
+__device__ __forceinline__ void commit_by(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 // Lanes 32 (warp % 4) .. + 31, 128 columns: a row of scores per thread.
 __device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&v)[128]) {
   asm volatile(
@@ -671,67 +699,85 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         atomicCAS(p.error, 0, 0x211);
         for (int k = max(0, n - SLOTS); k < n; ++k) wait_bounded(&full[k % SLOTS], (k / SLOTS) & 1, p.timeout_ns);
       }
-    } else if (warp == 9 && lane == 0) {
+    } else if (warp == 9) {
       constexpr uint32_t fmt = DT == MKX_BF16 ? 1u : 0u;
-      const uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(128 >> 4) << 24);
-      const uint32_t id_qk = base | ((uint32_t)(CK >> 3) << 17);
-      const uint32_t id_pv = base | ((uint32_t)(HD >> 3) << 17) | (1u << 16);  // V: dims contiguous
-      int uses_of[2] = {0, 0}, segments[2] = {0, 0}, place = 0;
+      constexpr uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(128 >> 4) << 24);
+      constexpr uint32_t id_qk = base | ((uint32_t)(CK >> 3) << 17);
+      constexpr uint32_t id_pv = base | ((uint32_t)(HD >> 3) << 17) | (1u << 16);  // V: dims contiguous
+      const uint32_t lead = elect_one(), tm = (uint32_t)uniform((int)tmem);
+      const uint32_t q_low = desc_low(smem_u32(qs), 0), k_low = desc_low(smem_u32(ring), 0),
+                     v_low = desc_low(smem_u32(ring), S::HALF);
+      auto wait = [&](uint64_t* bar, int parity) {
+        return __all_sync(0xffffffffu, wait_bounded(bar, (uint32_t)parity, p.timeout_ns)) != 0;
+      };
+      int uses_of[2] = {0, 0}, segments[2] = {0, 0};
+      int slot = 0, turn = 0;  // of K(i): slot and its phase
       bool ok = true;
       for (int jn = 0; ok; ++jn) {
-        ok = wait_bounded(&jfull[jn % JOBS], (jn / JOBS) & 1, p.timeout_ns);
+        ok = wait(&jfull[jn % JOBS], (jn / JOBS) & 1);
         if (!ok) break;
         const Job& job = jobs[jn % JOBS];
-        const int i0 = job.i0, i1 = job.i1;
-        const Tile tiles[2] = {job.tile[0], job.tile[1]};
-        mbar_arrive(&jempty[jn % JOBS]);
+        const int i0 = uniform(job.i0), i1 = uniform(job.i1);
+        Tile tiles[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          tiles[x].sinks = uniform(job.tile[x].sinks);
+          tiles[x].from = uniform(job.tile[x].from);
+          tiles[x].to = uniform(job.tile[x].to);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&jempty[jn % JOBS]);
         if (i0 < 0) break;
         bool pending[2] = {false, false}, begun[2] = {false, false}, asked[2] = {false, false};
+        int v_slot = 0, v_turn = 0;  // of V(i - 1)
         for (int i = i0; i <= i1 && ok; ++i) {
-          const int nk = place + 2 * (i - i0), nv = nk - 1;  // places of K(i) and V(i - 1)
+          const uint32_t v = v_low + v_slot * (S::TILE >> 4), k = k_low + slot * (S::TILE >> 4);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const uint32_t st = tmem + 128 * x, ot = tmem + 256 + 128 * x;
+            const uint32_t st = tm + 128 * x, ot = tm + 256 + 128 * x, q = q_low + x * (128 * 128 >> 4);
             if (pending[x] && ok) {
-              ok = wait_bounded(&full[nv % SLOTS], (nv / SLOTS) & 1, p.timeout_ns);
-              const uint32_t v = smem_u32(ring + (nv % SLOTS) * S::TILE);
+              ok = wait(&full[v_slot], v_turn);
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
-                ok = ok && wait_bounded(&pfull[2 * x + half], (uses_of[x] - 1) & 1, p.timeout_ns);
+                ok = ok && wait(&pfull[2 * x + half], (uses_of[x] - 1) & 1);
                 if (!ok) break;
                 tmem_fence_after();
 #pragma unroll
                 for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                  umma_ts(ot, st + 8 * kk, sw128_mn_desc(v + 2048 * kk, S::HALF), id_pv, (begun[x] || kk > 0) ? 1u : 0u);
+                  umma_ts(lead, ot, st + 8 * kk, v + kk * (2048 >> 4), id_pv, kk > 0 ? 1u : (begun[x] ? 1u : 0u));
               }
               if (!ok) break;
-              umma_commit(&ofull[x]);
+              commit_by(lead, &ofull[x]);
               pending[x] = false;
               begun[x] = true;
             }
-            if (x == 1 && i > i0) umma_commit(&empty[nv % SLOTS]);
+            if (x == 1 && i > i0) commit_by(lead, &empty[v_slot]);
             if (i < i1 && tiles[x].uses(i)) {
-              if (!asked[x]) ok = wait_bounded(&qfull[x], segments[x]++ & 1, p.timeout_ns);
+              if (!asked[x]) ok = wait(&qfull[x], segments[x]++ & 1);
               asked[x] = true;
-              ok = ok && wait_bounded(&full[nk % SLOTS], (nk / SLOTS) & 1, p.timeout_ns);
+              ok = ok && wait(&full[slot], turn);
               if (!ok) break;
               tmem_fence_after();
-              const uint32_t k = smem_u32(ring + (nk % SLOTS) * S::TILE), q = smem_u32(qs) + x * 128 * 128;
 #pragma unroll
               for (int kk = 0; kk < HD / 16; ++kk)
-                umma_bf16(st, sw128_desc(q + (kk >> 2) * S::QHALF + 32 * (kk & 3)),
-                          sw128_desc(k + (kk >> 2) * S::HALF + 32 * (kk & 3)), id_qk, kk > 0 ? 1u : 0u);
-              umma_commit(&sfull[x]);
+                umma_ss(lead, st, q + (kk >> 2) * (S::QHALF >> 4) + 2 * (kk & 3), k + (kk >> 2) * (S::HALF >> 4) + 2 * (kk & 3),
+                        id_qk, kk > 0 ? 1u : 0u);
+              commit_by(lead, &sfull[x]);
               pending[x] = true;
               ++uses_of[x];
             }
           }
-          if (i < i1) umma_commit(&empty[nk % SLOTS]);
+          if (i < i1) {
+            commit_by(lead, &empty[slot]);
+            if (++slot == SLOTS) slot = 0, turn ^= 1;
+            v_slot = slot;
+            v_turn = turn;
+            if (++slot == SLOTS) slot = 0, turn ^= 1;
+          }
         }
-        place += 2 * (i1 - i0);
       }
-      if (!ok) atomicCAS(p.error, 0, 0x213);
-      umma_commit(done);
+      if (!ok && lane == 0) atomicCAS(p.error, 0, 0x213);
+      commit_by(lead, done);
     } else if (warp == 10 && lane == 0) {
       // walks the line
       Walk<CT, CK> walk(p, line);
