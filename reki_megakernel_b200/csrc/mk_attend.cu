@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
       if (lane == 0) mbar_expect_tx(qfull, (uint32_t)((r1 - r0 + 1) * HD * 2));
       __syncwarp();
       if (lane <= r1 - r0) {
-        const int r = r0 + lane, t = r / p.group;
+        const int r = r0 + lane, t = by_group(p, r);
         bulk_g2s(qs + lane * S::QROW,
                  (const char*)p.q + 2 * ((long long)(sg.first_row + t) * p.q_row +
                                          (long long)(sg.kvh * p.group + r - t * p.group) * p.q_head),
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
       ok = ok && __all_sync(0xffffffffu, wait_bounded(qfull, tiles & 1, p.timeout_ns));
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        pos[x] = sg.past + (r0 + g + 8 * x) / p.group;
+        pos[x] = sg.past + by_group(p, r0 + g + 8 * x);
         const char* q = qs + (g + 8 * x) * S::QROW + 4 * c;
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
       add_up(0, step, groups);
     }
     if (r <= r1) {
-      const int t = r / p.group;
+      const int t = by_group(p, r);
       char* out = (char*)p.out + 2 * ((long long)(sg.first_row + t) * p.o_row +
                                       (long long)(sg.kvh * p.group + r - t * p.group) * p.o_head + q * D);
       const float inv = ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls);  // nothing seen: zero; NaN stays
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
 // tiles, whose products take 1024), by both alike at 128.
 constexpr int CT = 256;
 constexpr int CK = 128;
-constexpr int CHUNK_THREADS = 384;  // warps 0-3 tile A, 4-7 tile B, 8 TMA, 9 MMA, 10 walks the line, 11 fills the warpgroup
+constexpr int CHUNK_THREADS = 384;  // warps 0-3 tile A, 4-7 tile B, 8 TMA, 9 and 11 MMA, 10 walks the line
 // Registers per thread: 384 x 168 at launch; the warps of the tiles, a row of scores each, take 216, the others 72
 // (256 x 216 + 128 x 72 = 384 x 168).
 constexpr int TILE_REGS = 216, OTHER_REGS = 72;
@@ -429,7 +429,7 @@ constexpr uint32_t DESC_HIGH = 64u | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t leading) {
   return ((addr >> 4) & 0x3FFFu) | ((leading >> 4) << 16);
 }
-// The MMA warp stays converged, so that descriptors live in uniform registers (one thread by itself moves six
+// An MMA warp stays converged, so that descriptors live in uniform registers (one thread by itself moves six
 // registers per product, 100 clocks for a product of 64): the instruction is predicated on its one elected lane.
 // D[tmem] (+)= A[smem] * B[smem]^T, K = 16.
 __device__ __forceinline__ void umma_ss(uint32_t lead, uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc,
@@ -610,14 +610,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   uint64_t* pfull = sfull + 2;  // [2][2] the first, the second half of its probabilities are
   uint64_t* ofull = pfull + 4;  // [2] its sums include them
   uint64_t* done = ofull + 2;
-  uint64_t* jfull = done + 1;      // [JOBS]
+  uint64_t* turns = done + 1;      // [2] the MMA warps' turns
+  uint64_t* jfull = turns + 2;     // [JOBS]
   uint64_t* jempty = jfull + JOBS;  // [JOBS]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(jempty + JOBS);
   __shared__ Job jobs[JOBS];
   if (threadIdx.x == 0) {
     for (int s = 0; s < SLOTS; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], 2);
     }
     mbar_init(raw, 1);
     for (int x = 0; x < 2; ++x) {
@@ -626,11 +627,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       mbar_init(&pfull[2 * x], 4);
       mbar_init(&pfull[2 * x + 1], 4);
       mbar_init(&ofull[x], 1);
+      mbar_init(&turns[x], 1);
     }
-    mbar_init(done, 1);
+    mbar_init(done, 2);
     for (int j = 0; j < JOBS; ++j) {
       mbar_init(&jfull[j], 1);
-      mbar_init(&jempty[j], 10);  // the producer, the MMA warp, the eight warps of the tiles
+      mbar_init(&jempty[j], 11);  // the producer, the two MMA warps, the eight warps of the tiles
     }
     fence_mbar_init();
   }
@@ -699,81 +701,98 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         atomicCAS(p.error, 0, 0x211);
         for (int k = max(0, n - SLOTS); k < n; ++k) wait_bounded(&full[k % SLOTS], (k / SLOTS) & 1, p.timeout_ns);
       }
-    } else if (warp == 9) {
+    } else if (warp != 10) {
+      // the products of tile A (warp 9) and tile B (warp 11). They take turns, a block's step each, so that one tile's
+      // products run under the other's softmax (without turns both do the same at the same time: 281 against 2xx us for
+      // 2011 rows after 6007); two warps, because what one does around a step, a few hundred clocks, then hides behind
+      // the other's products
       constexpr uint32_t fmt = DT == MKX_BF16 ? 1u : 0u;
       constexpr uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(128 >> 4) << 24);
       constexpr uint32_t id_qk = base | ((uint32_t)(CK >> 3) << 17);
       constexpr uint32_t id_pv = base | ((uint32_t)(HD >> 3) << 17) | (1u << 16);  // V: dims contiguous
-      const uint32_t lead = elect_one(), tm = (uint32_t)uniform((int)tmem);
-      const uint32_t q_low = desc_low(smem_u32(qs), 0), k_low = desc_low(smem_u32(ring), 0),
+      const int x = uniform(warp == 11);
+      const uint32_t lead = elect_one(), st = (uint32_t)uniform((int)tmem) + 128 * x, ot = st + 256;
+      const uint32_t q = desc_low(smem_u32(qs), 0) + x * (128 * 128 >> 4), k_low = desc_low(smem_u32(ring), 0),
                      v_low = desc_low(smem_u32(ring), S::HALF);
       auto wait = [&](uint64_t* bar, int parity) {
         return __all_sync(0xffffffffu, wait_bounded(bar, (uint32_t)parity, p.timeout_ns)) != 0;
       };
-      int uses_of[2] = {0, 0}, segments[2] = {0, 0};
-      int slot = 0, turn = 0;  // of K(i): slot and its phase
+      int n = 0, segments = 0, steps = 0;  // blocks and segments of this tile; turns taken
+      int slot = 0, turn = 0;   // of K(i): slot and its phase
       bool ok = true;
       for (int jn = 0; ok; ++jn) {
         ok = wait(&jfull[jn % JOBS], (jn / JOBS) & 1);
         if (!ok) break;
         const Job& job = jobs[jn % JOBS];
         const int i0 = uniform(job.i0), i1 = uniform(job.i1);
-        Tile tiles[2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          tiles[x].sinks = uniform(job.tile[x].sinks);
-          tiles[x].from = uniform(job.tile[x].from);
-          tiles[x].to = uniform(job.tile[x].to);
-        }
+        Tile tile;
+        tile.sinks = uniform(job.tile[x].sinks);
+        tile.from = uniform(job.tile[x].from);
+        tile.to = uniform(job.tile[x].to);
         __syncwarp();
         if (lane == 0) mbar_arrive(&jempty[jn % JOBS]);
         if (i0 < 0) break;
-        bool pending[2] = {false, false}, begun[2] = {false, false}, asked[2] = {false, false};
+        bool pending = false, mine = false;
+        const int n0 = n;
+        auto my_turn = [&]() {
+          const bool got = mine || wait(&turns[x], (steps & 1) ^ (1 - x));
+          mine = true;
+          return got;
+        };
         int v_slot = 0, v_turn = 0;  // of V(i - 1)
-        for (int i = i0; i <= i1 && ok; ++i) {
-          const uint32_t v = v_low + v_slot * (S::TILE >> 4), k = k_low + slot * (S::TILE >> 4);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const uint32_t st = tm + 128 * x, ot = tm + 256 + 128 * x, q = q_low + x * (128 * 128 >> 4);
-            if (pending[x] && ok) {
-              ok = wait(&full[v_slot], v_turn);
+        for (int i = i0; i <= i1; ++i) {
+          if (i > i0) {
+            ok = wait(&full[v_slot], v_turn);
+            if (!ok) break;
+            if (pending) {
+              const uint32_t v = v_low + v_slot * (S::TILE >> 4);
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
-                ok = ok && wait(&pfull[2 * x + half], (uses_of[x] - 1) & 1);
-                if (!ok) break;
+                ok = ok && wait(&pfull[2 * x + half], (n - 1) & 1);
+                if (half == 0) ok = ok && my_turn();
                 tmem_fence_after();
 #pragma unroll
                 for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                  umma_ts(lead, ot, st + 8 * kk, v + kk * (2048 >> 4), id_pv, kk > 0 ? 1u : (begun[x] ? 1u : 0u));
+                  umma_ts(lead, ot, st + 8 * kk, v + kk * (2048 >> 4), id_pv, kk > 0 ? 1u : (n - 1 > n0 ? 1u : 0u));
               }
               if (!ok) break;
               commit_by(lead, &ofull[x]);
-              pending[x] = false;
-              begun[x] = true;
+              commit_by(lead, &empty[v_slot]);
+              pending = false;
+            } else if (lane == 0) {
+              mbar_arrive(&empty[v_slot]);
             }
-            if (x == 1 && i > i0) commit_by(lead, &empty[v_slot]);
-            if (i < i1 && tiles[x].uses(i)) {
-              if (!asked[x]) ok = wait(&qfull[x], segments[x]++ & 1);
-              asked[x] = true;
-              ok = ok && wait(&full[slot], turn);
+          }
+          if (i < i1) {
+            ok = wait(&full[slot], turn);
+            if (tile.uses(i)) {
+              if (n == n0) ok = ok && wait(&qfull[x], segments++ & 1);
+              ok = ok && my_turn();
               if (!ok) break;
               tmem_fence_after();
+              const uint32_t k = k_low + slot * (S::TILE >> 4);
 #pragma unroll
               for (int kk = 0; kk < HD / 16; ++kk)
                 umma_ss(lead, st, q + (kk >> 2) * (S::QHALF >> 4) + 2 * (kk & 3), k + (kk >> 2) * (S::HALF >> 4) + 2 * (kk & 3),
                         id_qk, kk > 0 ? 1u : 0u);
               commit_by(lead, &sfull[x]);
-              pending[x] = true;
-              ++uses_of[x];
+              commit_by(lead, &empty[slot]);
+              pending = true;
+              ++n;
+            } else {
+              if (!ok) break;
+              if (lane == 0) mbar_arrive(&empty[slot]);
             }
-          }
-          if (i < i1) {
-            commit_by(lead, &empty[slot]);
             if (++slot == SLOTS) slot = 0, turn ^= 1;
             v_slot = slot;
             v_turn = turn;
             if (++slot == SLOTS) slot = 0, turn ^= 1;
           }
+          ok = my_turn();  // a step without products still takes its turn
+          if (!ok) break;
+          if (lane == 0) mbar_arrive(&turns[1 - x]);
+          ++steps;
+          mine = false;
         }
       }
       if (!ok && lane == 0) atomicCAS(p.error, 0, 0x213);
@@ -817,17 +836,24 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         if (n == n0) {
           // the tile's Q into shared memory, coalesced: 16-byte chunks of a row by neighbouring threads. Only for a
           // tile with work in this segment: warps without any run ahead, by more phases than a barrier tells apart
-          for (int e = threadIdx.x - 128 * x; e < 128 * (HD / 8); e += 128) {
-            const int qr = 128 * x + e / (HD / 8), ch = e % (HD / 8), r = job.r0 + qr;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (r <= job.r1) {
-              const int t = r / p.group;
-              v = __ldg(reinterpret_cast<const uint4*>(
-                  (const char*)p.q + 2 * ((long long)(job.sg.first_row + t) * p.q_row +
-                                          (long long)(job.sg.kvh * p.group + r - t * p.group) * p.q_head + 8 * ch)));
-              v = make_uint4(signed_q(p, v.x), signed_q(p, v.y), signed_q(p, v.z), signed_q(p, v.w));
+          const int first = job.r0 + 128 * x, last = job.r1, head = job.sg.kvh * p.group;
+          const char* rows = (const char*)p.q + 2 * (long long)job.sg.first_row * p.q_row;
+          uint4 v[HD / 8];
+#pragma unroll
+          for (int k = 0; k < HD / 8; ++k) {  // all loads in flight at once
+            const int e = threadIdx.x - 128 * x + 128 * k, r = first + e / (HD / 8), ch = e % (HD / 8);
+            v[k] = make_uint4(0, 0, 0, 0);
+            if (r <= last) {
+              const int t = by_group(p, r);
+              v[k] = __ldg(reinterpret_cast<const uint4*>(
+                  rows + 2 * ((long long)t * p.q_row + (long long)(head + r - t * p.group) * p.q_head + 8 * ch)));
             }
-            *reinterpret_cast<uint4*>(qs + (ch >> 3) * S::QHALF + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4)) = v;
+          }
+#pragma unroll
+          for (int k = 0; k < HD / 8; ++k) {
+            const int e = threadIdx.x - 128 * x + 128 * k, qr = 128 * x + e / (HD / 8), ch = e % (HD / 8);
+            *reinterpret_cast<uint4*>(qs + (ch >> 3) * S::QHALF + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4)) =
+                make_uint4(signed_q(p, v[k].x), signed_q(p, v[k].y), signed_q(p, v[k].z), signed_q(p, v[k].w));
           }
           fence_proxy_async();
           __syncwarp();
@@ -839,7 +865,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         uint32_t s[128];
         tmem_ld128(st, s);
         if (i < tile.whole_from || i >= tile.whole_to) {
-          const int key0 = block_key<CK>(job.keys, i), position = job.sg.past + (job.r0 + row) / p.group;
+          const int key0 = block_key<CK>(job.keys, i), position = job.sg.past + by_group(p, job.r0 + row);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const uint32_t seen = seen_mask(p, job.keys, position, key0 + 32 * j);
@@ -915,7 +941,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         tmem_fence_after();
       }
       const Segment sg = job.sg;
-      const int r1 = job.r1, r = job.r0 + row, t = r / p.group;
+      const int r1 = job.r1, r = job.r0 + row, t = by_group(p, r);
       __syncwarp();
       if (lane == 0) mbar_arrive(&jempty[jn % JOBS]);
       char* out = (char*)p.out + 2 * ((long long)(sg.first_row + t) * p.o_row +
@@ -929,58 +955,87 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                          Half16<DT>::pack(o[d + 4] * inv, o[d + 5] * inv), Half16<DT>::pack(o[d + 6] * inv, o[d + 7] * inv));
       };
       constexpr int PART = CT * (HD + 2);  // [HD / 4][256 rows] float4, then (maximum, total) of each row
-      float* part = p.parts + (size_t)part_place(sg, blockIdx.x - sg.lead) * PART;
-#pragma unroll
-      for (int j = 0; j < HD / 32; ++j) {
+      auto sums_of = [&](int j, float (&o)[32]) {
         uint32_t u[32];
-        float o[32];
 #pragma unroll
         for (int d = 0; d < 32; ++d) u[d] = 0u;
         if (any && ok) tmem_ld32(ot + 32 * j, u);  // warp-uniform
 #pragma unroll
         for (int d = 0; d < 32; ++d) o[d] = __uint_as_float(u[d]);
-        if (sg.parts > 1) {
+      };
+      if (sg.parts == 1) {
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
+          float o[32];
+          sums_of(j, o);
+          if (r <= r1) write(o, j, scale_of(l));
+        }
+        tmem_fence_before();
+        continue;
+      }
+      const int own = blockIdx.x - sg.lead;
+      const bool keep = others_done<256>(p.tickets + sg.lead, sg.parts);
+      if (!keep) {
+        float* part = p.parts + (size_t)part_place(sg, own) * PART;
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
+          float o[32];
+          sums_of(j, o);
 #pragma unroll
           for (int d = 0; d < 32; d += 4)
             __stcg(reinterpret_cast<float4*>(part + ((size_t)(8 * j + d / 4) * CT + row) * 4),
                    make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]));
-        } else if (r <= r1) {
-          write(o, j, scale_of(l));
+        }
+        __stcg(reinterpret_cast<float2*>(part + (size_t)CT * HD) + row, make_float2(m, l));
+        if (!last_of<256>(p.tickets + sg.lead, sg.parts)) {
+          tmem_fence_before();
+          continue;
+        }
+      }
+      // the parts in their order, whoever is last: the same sums every time
+      auto ml_of = [&](int k) {
+        return k == own ? make_float2(m, l)
+                        : __ldcg(reinterpret_cast<const float2*>(p.parts + (size_t)part_place(sg, k) * PART + CT * HD) + row);
+      };
+      float top = -INFINITY, ls = 0.f;
+#pragma unroll 4
+      for (int k = 0; k < sg.parts; ++k) top = fmaxf(top, ml_of(k).x);
+      const float base = top == -INFINITY ? 0.f : top;
+      float acc[HD];
+#pragma unroll
+      for (int d = 0; d < HD; ++d) acc[d] = 0.f;
+      for (int k = 0; k < sg.parts; ++k) {
+        const float2 ml = ml_of(k);
+        const float f = ex2(ml.x - base);
+        ls += f * ml.y;
+        if (k == own) {
+#pragma unroll
+          for (int j = 0; j < HD / 32; ++j) {
+            float o[32];
+            sums_of(j, o);
+#pragma unroll
+            for (int d = 0; d < 32; ++d) acc[32 * j + d] += f * o[d];
+          }
+        } else {
+          const float4* at = reinterpret_cast<const float4*>(p.parts + (size_t)part_place(sg, k) * PART) + row;
+#pragma unroll
+          for (int d = 0; d < HD; d += 4) {
+            const float4 v = __ldcg(at + (size_t)(d / 4) * CT);
+            acc[d] += f * v.x;
+            acc[d + 1] += f * v.y;
+            acc[d + 2] += f * v.z;
+            acc[d + 3] += f * v.w;
+          }
         }
       }
       tmem_fence_before();
-      if (sg.parts > 1) {
-        __stcg(reinterpret_cast<float2*>(part + (size_t)CT * HD) + row, make_float2(m, l));
-        if (last_of<256>(p.tickets + sg.lead, sg.parts) && r <= r1) {
-          float top = -INFINITY, ls = 0.f;
-          auto ml_of = [&](int k) {
-            return __ldcg(reinterpret_cast<const float2*>(p.parts + (size_t)part_place(sg, k) * PART + CT * HD) + row);
-          };
-          for (int k = 0; k < sg.parts; ++k) top = fmaxf(top, ml_of(k).x);
-          const float base = top == -INFINITY ? 0.f : top;
-          for (int k = 0; k < sg.parts; ++k) {
-            const float2 ml = ml_of(k);
-            ls += ex2(ml.x - base) * ml.y;
-          }
-          const float inv = scale_of(ls);
-          for (int j = 0; j < HD / 32; ++j) {
-            float o[32];
+      if (r <= r1) {
 #pragma unroll
-            for (int d = 0; d < 32; ++d) o[d] = 0.f;
-            for (int k = 0; k < sg.parts; ++k) {
-              const float* at = p.parts + (size_t)part_place(sg, k) * PART;
-              const float f = ex2(ml_of(k).x - base);
+        for (int j = 0; j < HD / 32; ++j) {
+          float o[32];
 #pragma unroll
-              for (int d = 0; d < 32; d += 4) {
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(at + ((size_t)(8 * j + d / 4) * CT + row) * 4));
-                o[d] += f * v.x;
-                o[d + 1] += f * v.y;
-                o[d + 2] += f * v.z;
-                o[d + 3] += f * v.w;
-              }
-            }
-            write(o, j, inv);
-          }
+          for (int d = 0; d < 32; ++d) o[d] = acc[32 * j + d];
+          write(o, j, scale_of(ls));
         }
       }
     }
@@ -1115,6 +1170,7 @@ extern "C" mkx_status mkx_cache_attend(const mkx_attend_inputs* in, size_t works
   p.heads = a.heads;
   p.kv_heads = a.kv_heads;
   p.group = a.heads / a.kv_heads;
+  p.group_shift = (p.group & (p.group - 1)) == 0 ? __builtin_ctz(p.group) : -1;
   p.pages = a.pages;
   p.shift = mkxc::page_shift(a.page_rows);
   p.table_width = a.table_width;

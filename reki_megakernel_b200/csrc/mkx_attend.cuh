@@ -20,7 +20,7 @@ struct AttendParams {
   float* parts;       // [2 slots][tile rows x (HD + 2)]: unnormalised sums, then (maximum, total) of each row
   int* error;
   long long q_row, q_head, o_row, o_head;
-  int rows, B, heads, kv_heads, group, pages, shift, table_width, max_rows;
+  int rows, B, heads, kv_heads, group, group_shift, pages, shift, table_width, max_rows;  // group_shift: log2, or -1
   int causal, window, sinks;
   float scale_log2;       // |scale| * log2(e): scores are kept in powers of two
   uint32_t q_and, q_xor;  // q's words as they enter: the sign of a negative scale, nothing for scale 0
@@ -31,6 +31,13 @@ struct AttendParams {
 };
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+__device__ __forceinline__ int by_group(const AttendParams& p, int r) {
+  return p.group_shift >= 0 ? r >> p.group_shift : r / p.group;
+}
+// Quotients of what is nearly always below 2^32: a 64-bit division is a few hundred clocks, at every block's start.
+__device__ __forceinline__ long long quotient(long long a, int b) {
+  return (unsigned long long)a >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
+}
 
 // An episode's new rows, its row tiles (MT rows of (new row, head of the group)) and the most key blocks
 // (KT keys) that one of its tiles sees.
@@ -77,10 +84,11 @@ struct Segment {
 struct Line {
   long long total, at, begin, end;  // units; first unit of the episode that the stretch begins in; the stretch
   int blocks, b;                    // blocks that the line is cut for; that episode
+  Episode e;
 };
 
 __device__ __forceinline__ long long snapped(long long u, long long at, int units, int snap) {
-  const int v = (int)((unsigned long long)(u - at) % (unsigned)units);
+  const int v = (int)(u - at - quotient(u - at, units) * units);
   return v <= snap ? u - v : units - v <= snap ? u + (units - v) : u;
 }
 
@@ -109,9 +117,9 @@ __device__ __forceinline__ bool find_line(const AttendParams& p, Line& out) {
   all = 0;
 #pragma unroll
   for (int w = 0; w < W; ++w) all += sums[0][w];
-  const int blocks = (int)min((long long)p.slots, all / p.min_units + 1);
+  const int blocks = (int)min((long long)p.slots, quotient(all, p.min_units) + 1);
   if (all == 0 || (int)blockIdx.x >= blocks) return false;
-  const long long u0 = all * blockIdx.x / blocks, u1 = all * (blockIdx.x + 1) / blocks;
+  const long long u0 = quotient(all * blockIdx.x, blocks), u1 = quotient(all * (blockIdx.x + 1), blocks);
   if (threadIdx.x == 0) line.end = all;
   long long before = 0;
   for (int b0 = 0;; b0 += NTH) {  // ends: u0 < all
@@ -144,6 +152,7 @@ __device__ __forceinline__ bool find_line(const AttendParams& p, Line& out) {
       line.begin = snapped(u0, at, e.units, p.snap);
       line.blocks = blocks;
       line.b = b;
+      line.e = e;
     }
     if (u1 >= at && u1 < at + mine) line.end = snapped(u1, at, e.units, p.snap);
     if (before > u1 || before >= all) break;
@@ -163,13 +172,13 @@ struct Walk {
 
   __device__ __forceinline__ Walk(const AttendParams& params, const Line& l)
       : p(params), total(l.total), left(l.end - l.begin), blocks(l.blocks), b(l.b) {
-    e = episode_of<MT, KT>(p, b);
+    e = l.e;
     ask();
     // the stretch may begin behind the episode's last unit: then the first next() goes on
-    const long long local = l.begin - l.at, t = local / e.units;
+    const long long local = l.begin - l.at, t = quotient(local, e.units);
     v = (int)(local - t * e.units);
     tile_at = l.begin - v;
-    kvh = (int)(t / e.tiles);
+    kvh = (int)quotient(t, e.tiles);
     tile = e.tiles - 1 - (int)(t - (long long)kvh * e.tiles);
   }
   __device__ __forceinline__ void ask() {
@@ -179,7 +188,10 @@ struct Walk {
     n_length = p.length[n];
   }
   // The last block whose cut lies at or before `unit`.
-  __device__ __forceinline__ int block_at(long long unit) const { return (int)(((unit + 1) * blocks - 1) / total); }
+  __device__ __forceinline__ int block_at(long long unit) const { 
+    const long long a = (unit + 1) * blocks - 1;
+    return (unsigned long long)(a | total) >> 32 ? (int)(a / total) : (int)((unsigned)a / (unsigned)total);
+  }
   __device__ __forceinline__ bool next(Segment& s) {
     if (left <= 0) return false;
     while (kvh >= p.kv_heads || e.tiles == 0) {
@@ -219,6 +231,19 @@ struct Walk {
 // A block keeps at most two parts: of the tile its stretch begins inside of, and of the one it ends inside of.
 __device__ __forceinline__ int part_place(const Segment& s, int k) { return 2 * (s.lead + k) + (k == 0); }
 
+// Whether the other parts - 1 blocks of a tile have all delivered: then this one keeps its part to itself, and joins.
+// Called by all NTH threads (named barrier 1); leaves the ticket at zero if so. The others' parts are then visible
+// through __ldcg.
+template <int NTH>
+__device__ __forceinline__ bool others_done(unsigned* ticket, int parts) {
+  __shared__ int done;
+  if (threadIdx.x == 0) {
+    done = ld_acquire_i32(reinterpret_cast<int*>(ticket)) == parts - 1;
+    if (done) *ticket = 0;
+  }
+  asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");
+  return done;
+}
 // Called by all NTH threads (named barrier 1) after they wrote their part k of a split tile with __stcg: whether
 // this block is the last of the parts [k0, k0 + n) under ticket `ticket`, which is left at zero. The others' parts are
 // then visible through __ldcg.
@@ -249,8 +274,8 @@ struct Keys {
 template <int KT>
 __device__ __forceinline__ Keys keys_of(const AttendParams& p, const Segment& s, int r0, int r1) {
   Keys k;
-  k.p_first = s.past + r0 / p.group;
-  k.p_last = s.past + r1 / p.group;
+  k.p_first = s.past + by_group(p, r0);
+  k.p_last = s.past + by_group(p, r1);
   const int held = (int)min((long long)s.length, (long long)p.table_width << p.shift);
   k.hi = p.causal ? max(min(held, k.p_last + 1), 0) : held;
   k.lo = p.window ? min(max(k.p_first - p.window + 1, 0), k.hi) : 0;
