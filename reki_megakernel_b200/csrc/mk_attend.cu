@@ -93,8 +93,10 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
     mbar_init(qempty, ROW_WARPS);
     fence_mbar_init();
   }
+  __shared__ LineScratch scratch;
+  __shared__ int flag;
   Line line;
-  if (!find_line<MT, KT, ROW_THREADS>(p, line)) return;  // its barriers publish the mbarriers too
+  if (!find_line<MT, KT, ROW_THREADS>(p, scratch, line)) return;  // its barriers publish the mbarriers too
   Walk<MT, KT> walk(p, line);
   Segment sg;
   int n = 0, tiles = 0;  // blocks of keys and tiles since the start: n % ROW_STAGES is a block's stage
@@ -369,12 +371,12 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
         step = JOIN_AT_ONCE;
         groups = ceil_div(sg.parts, step);
         const int first = (int)(blockIdx.x - sg.lead) / step * step, count = min(step, sg.parts - first);
-        if (!last_of<32 * ROW_WARPS>(p.tickets + p.slots + part_place(sg, first), count)) continue;
+        if (!last_of<32 * ROW_WARPS>(p.tickets + p.slots + part_place(sg, first), count, &flag)) continue;
         add_up(first, 1, count);
         row_barrier();  // the group's first part has been read: the group's sums take its place
         keep(first);
       }
-      if (!last_of<32 * ROW_WARPS>(p.tickets + sg.lead, groups)) continue;
+      if (!last_of<32 * ROW_WARPS>(p.tickets + sg.lead, groups, &flag)) continue;
       add_up(0, step, groups);
     }
     if (r <= r1) {
@@ -395,30 +397,38 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
 
 // ---- chunks ----------------------------------------------------------------------------------------
 // chunk_kernel: tiles of 256 rows as two tiles A, B of 128, one CTA per SM. Both products run on
-// tcgen05 (128-key blocks): S = Q K^T from shared memory into TMEM, O += P V with P read from TMEM (it
-// overwrites the scores it came from) and V as TMA left it (dims contiguous). Four warps per tile hold
-// one row per thread: no shuffles, the row's maximum and sum stay in registers. While one tile's warps
-// take exponentials, the tensor cores work for the other. O is rescaled only when a maximum has grown by
-// more than 2^8 since the last time, which is rare after the first blocks: P stays below 2^8, far inside
-// both types. Bound by the exponentials at head_dim 64 (16 a clock per SM: 2048 clocks for two 128 x 128
-// tiles, whose products take 1024), by both alike at 128.
+// tcgen05 (128-key blocks): S = Q K^T from shared memory into TMEM, O += P V with P read from TMEM and V
+// as TMA left it (dims contiguous). Eight warps per tile: two threads share a row, half of the keys of a
+// block each, so that what lies between S and P, which nothing else of the same tile can overlap, is
+// short. They exchange their maxima once a block. O is rescaled only when a maximum has grown by more
+// than 2^8 since the last time, which is rare after the first blocks: P stays below 2^8, far inside both
+// types. At head_dim 128 TMEM is full with two tiles of S and O, and P overwrites the scores it came
+// from: a tile's products wait for its softmax and the other way round, and the two tiles alternate. At
+// head_dim 64 P has columns of its own, and the next scores are there before the last ones are done.
+// Bound by the exponentials at head_dim 64 (16 a clock per SM: 2048 clocks for two 128 x 128 tiles, whose
+// products take 1024), by both alike at 128.
 constexpr int CT = 256;
 constexpr int CK = 128;
-constexpr int CHUNK_THREADS = 384;  // warps 0-3 tile A, 4-7 tile B, 8 TMA, 9 and 11 MMA, 10 walks the line
-// Registers per thread: 384 x 168 at launch; the warps of the tiles, a row of scores each, take 216, the others 72
-// (256 x 216 + 128 x 72 = 384 x 168).
-constexpr int TILE_REGS = 216, OTHER_REGS = 72;
-constexpr int MAX_SLOTS = 8;
+constexpr int TILE_THREADS = 512;                   // warps 0-7 tile A, 8-15 tile B
+constexpr int CHUNK_THREADS = TILE_THREADS + 128;   // 16 TMA, 17 and 19 MMA, 18 walks the line
+// Registers per thread: 640 x 96 at launch; the warps of the tiles, half a row of scores each, take 104, the others 64
+// (512 x 104 + 128 x 64 = 640 x 96).
+constexpr int TILE_REGS = 104, OTHER_REGS = 64;
 constexpr bool POLY = true;
 constexpr float LAZY = 8.f;  // log2 of the growth that is let pass
+constexpr int JOBS = 2;
 
 template <int HD>
 struct ChunkShape {
+  static constexpr bool EARLY = HD == 64;               // P beside S in TMEM
   static constexpr int TILE = CK * HD * 2;              // one K or V block
   static constexpr int HALF = CK * 128;                 // its 64-dim half
   static constexpr int SLOTS = HD == 128 ? 5 : 8;
   static constexpr int QHALF = CT * 128;
-  static constexpr int SMEM = SLOTS * TILE + CT * HD * 2 + 1024 + 320;
+  // TMEM columns of a tile: S, O, P
+  static __device__ __forceinline__ uint32_t s_at(int x) { return 128 * x; }
+  static __device__ __forceinline__ uint32_t o_at(int x) { return 256 + HD * x; }
+  static __device__ __forceinline__ uint32_t p_at(int x) { return EARLY ? 384 + 64 * x : 128 * x; }
 };
 
 // Shared-memory matrix descriptors in two words: the low one (address and leading offset, both / 16) changes from
@@ -462,38 +472,24 @@ __device__ __forceinline__ uint32_t elect_one() {
   return r;
 }
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
-// Lanes 32 (warp % 4) .. + 31, 128 columns: a row of scores per thread.
-__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&v)[128]) {
+// Lanes 32 (warp % 4) .. + 31, 64 columns.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&v)[64]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
       "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
       "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, "
       "%38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, "
-      "%56, %57, %58, %59, %60, %61, %62, %63, %64, %65, %66, %67, %68, %69, %70, %71, %72, %73, "
-      "%74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, "
-      "%92, %93, %94, %95, %96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, "
-      "%108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, "
-      "%123, %124, %125, %126, %127 "
-      "}, [%128];\n\ttcgen05.wait::ld.sync.aligned;"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
-        "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
-        "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]), "=r"(v[32]), "=r"(v[33]), "=r"(v[34]),
-        "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]), "=r"(v[40]), "=r"(v[41]),
-        "=r"(v[42]), "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]), "=r"(v[48]),
-        "=r"(v[49]), "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]),
-        "=r"(v[56]), "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]),
-        "=r"(v[63]), "=r"(v[64]), "=r"(v[65]), "=r"(v[66]), "=r"(v[67]), "=r"(v[68]), "=r"(v[69]),
-        "=r"(v[70]), "=r"(v[71]), "=r"(v[72]), "=r"(v[73]), "=r"(v[74]), "=r"(v[75]), "=r"(v[76]),
-        "=r"(v[77]), "=r"(v[78]), "=r"(v[79]), "=r"(v[80]), "=r"(v[81]), "=r"(v[82]), "=r"(v[83]),
-        "=r"(v[84]), "=r"(v[85]), "=r"(v[86]), "=r"(v[87]), "=r"(v[88]), "=r"(v[89]), "=r"(v[90]),
-        "=r"(v[91]), "=r"(v[92]), "=r"(v[93]), "=r"(v[94]), "=r"(v[95]), "=r"(v[96]), "=r"(v[97]),
-        "=r"(v[98]), "=r"(v[99]), "=r"(v[100]), "=r"(v[101]), "=r"(v[102]), "=r"(v[103]),
-        "=r"(v[104]), "=r"(v[105]), "=r"(v[106]), "=r"(v[107]), "=r"(v[108]), "=r"(v[109]),
-        "=r"(v[110]), "=r"(v[111]), "=r"(v[112]), "=r"(v[113]), "=r"(v[114]), "=r"(v[115]),
-        "=r"(v[116]), "=r"(v[117]), "=r"(v[118]), "=r"(v[119]), "=r"(v[120]), "=r"(v[121]),
-        "=r"(v[122]), "=r"(v[123]), "=r"(v[124]), "=r"(v[125]), "=r"(v[126]), "=r"(v[127])
+      "%56, %57, %58, %59, %60, %61, %62, %63 "
+      "}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),
+        "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]),
+        "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]),
+        "=r"(v[29]), "=r"(v[30]), "=r"(v[31]), "=r"(v[32]), "=r"(v[33]), "=r"(v[34]), "=r"(v[35]),
+        "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]), "=r"(v[40]), "=r"(v[41]), "=r"(v[42]),
+        "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]), "=r"(v[48]), "=r"(v[49]),
+        "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]), "=r"(v[56]),
+        "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63])
       : "r"(taddr)
       : "memory");
 }
@@ -505,6 +501,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
       "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
       "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
       "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -591,7 +595,29 @@ __device__ __forceinline__ void fill(const AttendParams& p, Job& job, const Segm
     job.tile[x] = t;
   }
 }
-constexpr int JOBS = 4;
+
+template <int HD>
+struct ChunkShared {
+  char ring[ChunkShape<HD>::SLOTS * ChunkShape<HD>::TILE];  // K and V blocks
+  char q[CT * HD * 2];                                      // [HD / 64][256 rows][128 bytes], 128-byte swizzle
+  union {
+    LineScratch line;
+    float row[2][2][128];  // [tile][half]: what the two threads of a row tell each other
+  } scratch;
+  uint64_t full[ChunkShape<HD>::SLOTS], empty[ChunkShape<HD>::SLOTS], raw;
+  uint64_t qfull[2];     // a tile's rows of Q are in shared memory
+  uint64_t sfull[2];     // its scores are in TMEM
+  uint64_t sfree[2];     // its scores are in registers (EARLY)
+  uint64_t pfull[2][2];  // the first, the second half of the probabilities of each thread are in TMEM
+  uint64_t ofull[2];     // its sums include them
+  uint64_t done;
+  uint64_t turns[2];     // the MMA warps' turns
+  uint64_t jfull[JOBS], jempty[JOBS];
+  uint32_t tmem;
+  int flag;
+  Job jobs[JOBS];
+};
+static_assert(sizeof(ChunkShared<128>) <= 227 * 1024, "one block's shared memory");
 
 template <int DT, int HD>
 __global__ void __launch_bounds__(CHUNK_THREADS, 1)
@@ -600,64 +626,57 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   using S = ChunkShape<HD>;
   constexpr int SLOTS = S::SLOTS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  char* ring = asmem + ((1024u - (smem_u32(asmem) & 1023u)) & 1023u);
-  char* qs = ring + SLOTS * S::TILE;  // [HD / 64][256 rows][128 bytes], 128-byte swizzle
-  uint64_t* full = reinterpret_cast<uint64_t*>(qs + CT * HD * 2);
-  uint64_t* empty = full + MAX_SLOTS;
-  uint64_t* raw = empty + MAX_SLOTS;
-  uint64_t* qfull = raw + 1;    // [2] a tile's rows of Q are in shared memory
-  uint64_t* sfull = qfull + 2;  // [2] its scores are in TMEM
-  uint64_t* pfull = sfull + 2;  // [2][2] the first, the second half of its probabilities are
-  uint64_t* ofull = pfull + 4;  // [2] its sums include them
-  uint64_t* done = ofull + 2;
-  uint64_t* turns = done + 1;      // [2] the MMA warps' turns
-  uint64_t* jfull = turns + 2;     // [JOBS]
-  uint64_t* jempty = jfull + JOBS;  // [JOBS]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(jempty + JOBS);
-  __shared__ Job jobs[JOBS];
+  auto& sm = *reinterpret_cast<ChunkShared<HD>*>(asmem);
+  char* ring = sm.ring;
+  char* qs = sm.q;
+  if (smem_u32(asmem) & 1023u) {  // (nothing else is in shared memory)
+    if (threadIdx.x == 0) atomicCAS(p.error, 0, 0x210);
+    return;
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < SLOTS; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 2);
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 2);  // both tiles' products have read it
     }
-    mbar_init(raw, 1);
+    mbar_init(&sm.raw, 1);
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&qfull[x], 4);
-      mbar_init(&sfull[x], 1);
-      mbar_init(&pfull[2 * x], 4);
-      mbar_init(&pfull[2 * x + 1], 4);
-      mbar_init(&ofull[x], 1);
-      mbar_init(&turns[x], 1);
+      mbar_init(&sm.qfull[x], 8);
+      mbar_init(&sm.sfull[x], 1);
+      mbar_init(&sm.sfree[x], 8);
+      mbar_init(&sm.pfull[x][0], 8);
+      mbar_init(&sm.pfull[x][1], 8);
+      mbar_init(&sm.ofull[x], 1);
+      mbar_init(&sm.turns[x], 1);
     }
-    mbar_init(done, 2);
+    mbar_init(&sm.done, 2);
     for (int j = 0; j < JOBS; ++j) {
-      mbar_init(&jfull[j], 1);
-      mbar_init(&jempty[j], 11);  // the producer, the two MMA warps, the eight warps of the tiles
+      mbar_init(&sm.jfull[j], 1);
+      mbar_init(&sm.jempty[j], 19);  // the producer, the two MMA warps, the sixteen warps of the tiles
     }
     fence_mbar_init();
   }
   Line line;
-  if (!find_line<CT, CK, CHUNK_THREADS>(p, line)) return;
-  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  if (!find_line<CT, CK, CHUNK_THREADS>(p, sm.scratch.line, line)) return;
+  if (warp == 17) tmem_alloc(&sm.tmem, 512);
   __syncthreads();
   tmem_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = sm.tmem;
 
-  if (warp >= 8) {
+  if (warp >= 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-    if (warp == 8) {
+    if (warp == 16) {
       // producer: slots hold K, V, K, V, ... of the blocks in order; lane j fetches the j-th page
       const int rows_box = min(1 << p.shift, CK), boxes = CK / rows_box;
       bool ok = true;
       int n = 0, raws = 0;
       for (int jn = 0; ok; ++jn) {
-        ok = __all_sync(0xffffffffu, wait_bounded(&jfull[jn % JOBS], (jn / JOBS) & 1, p.timeout_ns));
+        ok = __all_sync(0xffffffffu, wait_bounded(&sm.jfull[jn % JOBS], (jn / JOBS) & 1, p.timeout_ns));
         if (!ok) break;
-        const Job& job = jobs[jn % JOBS];
+        const Job& job = sm.jobs[jn % JOBS];
         const int i0 = job.i0, i1 = job.i1, b = job.sg.b, kvh = job.sg.kvh;
         const Keys ks = job.keys;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&jempty[jn % JOBS]);
+        if (lane == 0) mbar_arrive(&sm.jempty[jn % JOBS]);
         if (i0 < 0) break;
         auto page_at = [&](int i) {
           return lane < boxes ? page_of(p, ks, b, (block_key<CK>(ks, i) >> p.shift) + lane) : -1;
@@ -669,12 +688,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv, ++n) {
             const int s = n % SLOTS;
-            if (n >= SLOTS) ok = wait_bounded(&empty[s], ((n / SLOTS) & 1) ^ 1, p.timeout_ns);
+            if (n >= SLOTS) ok = wait_bounded(&sm.empty[s], ((n / SLOTS) & 1) ^ 1, p.timeout_ns);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             // rows of V behind the last key may hold anything, and 0 * NaN is not 0: they are zeroed here
             const bool ragged = kv == 1 && key0 + CK > ks.hi;
-            uint64_t* bar = ragged ? raw : &full[s];
+            uint64_t* bar = ragged ? &sm.raw : &sm.full[s];
             if (lane == 0) mbar_expect_tx(bar, (uint32_t)S::TILE);
             __syncwarp();
             char* at = ring + s * S::TILE;
@@ -683,7 +702,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
               for (int h = 0; h < HD / 64; ++h)
                 tma_load_4d(at + h * S::HALF + lane * rows_box * 128, kv ? &tv : &tk, 64 * h, row, kvh, id, bar);
             if (ragged) {  // a tile's last block
-              ok = __all_sync(0xffffffffu, wait_bounded(raw, raws & 1, p.timeout_ns));
+              ok = __all_sync(0xffffffffu, wait_bounded(&sm.raw, raws & 1, p.timeout_ns));
               ++raws;
               for (int e = lane + (ks.hi - key0) * (HD / 8); e < CK * (HD / 8); e += 32) {
                 const int r = e / (HD / 8), ch = e % (HD / 8);
@@ -691,7 +710,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
               }
               fence_proxy_async();
               __syncwarp();
-              if (lane == 0) mbar_arrive(&full[s]);
+              if (lane == 0) mbar_arrive(&sm.full[s]);
             }
           }
           id = next;
@@ -699,74 +718,82 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       }
       if (!ok && lane == 0) {  // a wait ran out: let what is in flight land before the block ends
         atomicCAS(p.error, 0, 0x211);
-        for (int k = max(0, n - SLOTS); k < n; ++k) wait_bounded(&full[k % SLOTS], (k / SLOTS) & 1, p.timeout_ns);
+        for (int k = max(0, n - SLOTS); k < n; ++k) wait_bounded(&sm.full[k % SLOTS], (k / SLOTS) & 1, p.timeout_ns);
       }
-    } else if (warp != 10) {
-      // the products of tile A (warp 9) and tile B (warp 11). They take turns, a block's step each, so that one tile's
-      // products run under the other's softmax (without turns both do the same at the same time: 281 against 2xx us for
-      // 2011 rows after 6007); two warps, because what one does around a step, a few hundred clocks, then hides behind
-      // the other's products
+    } else if (warp != 18) {
+      // the products of tile A (warp 17) and tile B (warp 19): two warps, because what one does around a block's
+      // products, a few hundred clocks, then hides behind the other's. Without columns for P beside S they take turns,
+      // so that one tile's products run under the other's softmax (otherwise both do the same at the same time: 281
+      // instead of 239 us for 2011 rows after 6007, 32/8 heads x 128)
       constexpr uint32_t fmt = DT == MKX_BF16 ? 1u : 0u;
       constexpr uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(128 >> 4) << 24);
       constexpr uint32_t id_qk = base | ((uint32_t)(CK >> 3) << 17);
       constexpr uint32_t id_pv = base | ((uint32_t)(HD >> 3) << 17) | (1u << 16);  // V: dims contiguous
-      const int x = uniform(warp == 11);
-      const uint32_t lead = elect_one(), st = (uint32_t)uniform((int)tmem) + 128 * x, ot = st + 256;
+      const int x = uniform(warp == 19);
+      const uint32_t lead = elect_one(), tm = (uint32_t)uniform((int)tmem);
+      const uint32_t st = tm + S::s_at(x), ot = tm + S::o_at(x), pt = tm + S::p_at(x);
       const uint32_t q = desc_low(smem_u32(qs), 0) + x * (128 * 128 >> 4), k_low = desc_low(smem_u32(ring), 0),
                      v_low = desc_low(smem_u32(ring), S::HALF);
       auto wait = [&](uint64_t* bar, int parity) {
         return __all_sync(0xffffffffu, wait_bounded(bar, (uint32_t)parity, p.timeout_ns)) != 0;
       };
       int n = 0, segments = 0, steps = 0;  // blocks and segments of this tile; turns taken
-      int slot = 0, turn = 0;   // of K(i): slot and its phase
+      int slot = 0, turn = 0;              // of K(i): slot and its phase
       bool ok = true;
       for (int jn = 0; ok; ++jn) {
-        ok = wait(&jfull[jn % JOBS], (jn / JOBS) & 1);
+        ok = wait(&sm.jfull[jn % JOBS], (jn / JOBS) & 1);
         if (!ok) break;
-        const Job& job = jobs[jn % JOBS];
+        const Job& job = sm.jobs[jn % JOBS];
         const int i0 = uniform(job.i0), i1 = uniform(job.i1);
         Tile tile;
         tile.sinks = uniform(job.tile[x].sinks);
         tile.from = uniform(job.tile[x].from);
         tile.to = uniform(job.tile[x].to);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&jempty[jn % JOBS]);
+        if (lane == 0) mbar_arrive(&sm.jempty[jn % JOBS]);
         if (i0 < 0) break;
-        bool pending = false, mine = false;
         const int n0 = n;
+        bool mine = S::EARLY;
         auto my_turn = [&]() {
-          const bool got = mine || wait(&turns[x], (steps & 1) ^ (1 - x));
+          const bool got = mine || wait(&sm.turns[x], (steps & 1) ^ (1 - x));
           mine = true;
           return got;
         };
-        int v_slot = 0, v_turn = 0;  // of V(i - 1)
-        for (int i = i0; i <= i1; ++i) {
-          if (i > i0) {
-            ok = wait(&full[v_slot], v_turn);
-            if (!ok) break;
-            if (pending) {
-              const uint32_t v = v_low + v_slot * (S::TILE >> 4);
+        int done = n0;       // blocks whose V product has been issued
+        auto add_pv = [&](int v_slot, int v_turn, bool has) {  // V(i - 1)
+          if (!wait(&sm.full[v_slot], v_turn)) return false;
+          if (!has) {
+            if (lane == 0) mbar_arrive(&sm.empty[v_slot]);
+            return true;
+          }
+          const uint32_t v = v_low + v_slot * (S::TILE >> 4);
 #pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                ok = ok && wait(&pfull[2 * x + half], (n - 1) & 1);
-                if (half == 0) ok = ok && my_turn();
-                tmem_fence_after();
+          for (int part = 0; part < 2; ++part) {
+            if (!wait(&sm.pfull[x][part], done & 1)) return false;
+            if (part == 0 && !my_turn()) return false;
+            tmem_fence_after();
 #pragma unroll
-                for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                  umma_ts(lead, ot, st + 8 * kk, v + kk * (2048 >> 4), id_pv, kk > 0 ? 1u : (n - 1 > n0 ? 1u : 0u));
-              }
-              if (!ok) break;
-              commit_by(lead, &ofull[x]);
-              commit_by(lead, &empty[v_slot]);
-              pending = false;
-            } else if (lane == 0) {
-              mbar_arrive(&empty[v_slot]);
+            for (int k = 0; k < 4; ++k) {
+              const int kk = 4 * (k >> 1) + 2 * part + (k & 1);  // keys 0-31 and 64-95, then the others
+              umma_ts(lead, ot, pt + 8 * kk, v + kk * (2048 >> 4), id_pv, (part > 0 || k > 0) ? 1u : (done > n0 ? 1u : 0u));
             }
           }
+          commit_by(lead, &sm.ofull[x]);
+          commit_by(lead, &sm.empty[v_slot]);
+          ++done;
+          return true;
+        };
+        int v_slot = 0, v_turn = 0;
+        bool last_used = false;
+        for (int i = i0; i <= i1; ++i) {
+          const bool used = i < i1 && tile.uses(i);
+          if (!S::EARLY && i > i0) ok = add_pv(v_slot, v_turn, last_used);
+          if (!ok) break;
           if (i < i1) {
-            ok = wait(&full[slot], turn);
-            if (tile.uses(i)) {
-              if (n == n0) ok = ok && wait(&qfull[x], segments++ & 1);
+            ok = wait(&sm.full[slot], turn);
+            if (used) {
+              if (n == n0) ok = ok && wait(&sm.qfull[x], segments++ & 1);
+              if (S::EARLY && n > 0) ok = ok && wait(&sm.sfree[x], (n - 1) & 1);
               ok = ok && my_turn();
               if (!ok) break;
               tmem_fence_after();
@@ -775,73 +802,89 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
               for (int kk = 0; kk < HD / 16; ++kk)
                 umma_ss(lead, st, q + (kk >> 2) * (S::QHALF >> 4) + 2 * (kk & 3), k + (kk >> 2) * (S::HALF >> 4) + 2 * (kk & 3),
                         id_qk, kk > 0 ? 1u : 0u);
-              commit_by(lead, &sfull[x]);
-              commit_by(lead, &empty[slot]);
-              pending = true;
+              commit_by(lead, &sm.sfull[x]);
+              commit_by(lead, &sm.empty[slot]);
               ++n;
             } else {
               if (!ok) break;
-              if (lane == 0) mbar_arrive(&empty[slot]);
+              if (lane == 0) mbar_arrive(&sm.empty[slot]);
             }
+          }
+          if (S::EARLY && i > i0) ok = add_pv(v_slot, v_turn, last_used);
+          if (!ok) break;
+          if (i < i1) {
             if (++slot == SLOTS) slot = 0, turn ^= 1;
             v_slot = slot;
             v_turn = turn;
             if (++slot == SLOTS) slot = 0, turn ^= 1;
           }
-          ok = my_turn();  // a step without products still takes its turn
-          if (!ok) break;
-          if (lane == 0) mbar_arrive(&turns[1 - x]);
-          ++steps;
-          mine = false;
+          last_used = used;
+          if (!S::EARLY) {
+            ok = my_turn();  // a step without products still takes its turn
+            if (!ok) break;
+            if (lane == 0) mbar_arrive(&sm.turns[1 - x]);
+            ++steps;
+            mine = false;
+          }
         }
       }
       if (!ok && lane == 0) atomicCAS(p.error, 0, 0x213);
-      commit_by(lead, done);
-    } else if (warp == 10 && lane == 0) {
+      commit_by(lead, &sm.done);
+    } else if (lane == 0) {
       // walks the line
       Walk<CT, CK> walk(p, line);
       Segment sg;
       for (int jn = 0;; ++jn) {
         const bool more = walk.next(sg);
-        if (jn >= JOBS && !wait_bounded(&jempty[jn % JOBS], ((jn / JOBS) & 1) ^ 1, p.timeout_ns)) {
+        if (jn >= JOBS && !wait_bounded(&sm.jempty[jn % JOBS], ((jn / JOBS) & 1) ^ 1, p.timeout_ns)) {
           atomicCAS(p.error, 0, 0x215);
           break;
         }
-        if (more) fill(p, jobs[jn % JOBS], sg);
-        else jobs[jn % JOBS].i0 = -1;
-        mbar_arrive(&jfull[jn % JOBS]);
+        if (more) fill(p, sm.jobs[jn % JOBS], sg);
+        else sm.jobs[jn % JOBS].i0 = -1;
+        mbar_arrive(&sm.jfull[jn % JOBS]);
         if (!more) break;
       }
     }
     __syncwarp();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TILE_REGS));
-    const int x = warp >> 2, row = threadIdx.x;
+    // two threads per row: keys 64 h .. of a block, dims HD / 2 * h .. of the sums
+    const int x = warp >> 3, h = (warp >> 2) & 1, row = 32 * (warp & 3) + lane;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t st = tmem + lanes + 128 * x, ot = tmem + lanes + 256 + 128 * x;
+    const uint32_t st = tmem + lanes + S::s_at(x) + 64 * h, ot = tmem + lanes + S::o_at(x) + HD / 2 * h,
+                   pt = tmem + lanes + S::p_at(x) + 32 * h;
+    const int pair = 2 + 4 * x + (warp & 3);  // named barrier of the two warps that share rows
+    auto pair_barrier = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory"); };
     const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
     int n = 0;  // blocks of this tile since the start
+    // After a wait that ran out the warp goes on without waiting: others of its barriers still count on it
     bool ok = true;
-    for (int jn = 0; ok; ++jn) {
-      ok = __all_sync(0xffffffffu, wait_bounded(&jfull[jn % JOBS], (jn / JOBS) & 1, p.timeout_ns));
-      if (!ok) break;
-      const Job& job = jobs[jn % JOBS];
+    auto wait = [&](uint64_t* bar, int parity) {
+      ok = ok && __all_sync(0xffffffffu, wait_bounded(bar, (uint32_t)parity, p.timeout_ns)) != 0;
+    };
+    for (int jn = 0;; ++jn) {
+      if (!__all_sync(0xffffffffu, wait_bounded(&sm.jfull[jn % JOBS], (jn / JOBS) & 1, p.timeout_ns))) {
+        ok = false;
+        break;
+      }
+      const Job& job = sm.jobs[jn % JOBS];
       const int i0 = job.i0, i1 = job.i1;
       if (i0 < 0) break;
       const Tile tile = job.tile[x];
       float m = -INFINITY, l = 0.f;
       const int n0 = n;
-      for (int i = i0; i < i1 && ok; ++i) {
+      for (int i = i0; i < i1; ++i) {
         if (!tile.uses(i)) continue;
         if (n == n0) {
           // the tile's Q into shared memory, coalesced: 16-byte chunks of a row by neighbouring threads. Only for a
           // tile with work in this segment: warps without any run ahead, by more phases than a barrier tells apart
-          const int first = job.r0 + 128 * x, last = job.r1, head = job.sg.kvh * p.group;
+          const int first = job.r0 + 128 * x, last = job.r1, head = job.sg.kvh * p.group, th = threadIdx.x & 255;
           const char* rows = (const char*)p.q + 2 * (long long)job.sg.first_row * p.q_row;
-          uint4 v[HD / 8];
+          uint4 v[HD / 16];
 #pragma unroll
-          for (int k = 0; k < HD / 8; ++k) {  // all loads in flight at once
-            const int e = threadIdx.x - 128 * x + 128 * k, r = first + e / (HD / 8), ch = e % (HD / 8);
+          for (int k = 0; k < HD / 16; ++k) {  // all loads in flight at once
+            const int e = th + 256 * k, r = first + e / (HD / 8), ch = e % (HD / 8);
             v[k] = make_uint4(0, 0, 0, 0);
             if (r <= last) {
               const int t = by_group(p, r);
@@ -850,69 +893,79 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             }
           }
 #pragma unroll
-          for (int k = 0; k < HD / 8; ++k) {
-            const int e = threadIdx.x - 128 * x + 128 * k, qr = 128 * x + e / (HD / 8), ch = e % (HD / 8);
+          for (int k = 0; k < HD / 16; ++k) {
+            const int e = th + 256 * k, qr = 128 * x + e / (HD / 8), ch = e % (HD / 8);
             *reinterpret_cast<uint4*>(qs + (ch >> 3) * S::QHALF + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4)) =
                 make_uint4(signed_q(p, v[k].x), signed_q(p, v[k].y), signed_q(p, v[k].z), signed_q(p, v[k].w));
           }
           fence_proxy_async();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&qfull[x]);
+          if (lane == 0) mbar_arrive(&sm.qfull[x]);
         }
-        ok = __all_sync(0xffffffffu, wait_bounded(&sfull[x], n & 1, p.timeout_ns));
-        if (!ok) break;
+        wait(&sm.sfull[x], n & 1);
         tmem_fence_after();
-        uint32_t s[128];
-        tmem_ld128(st, s);
+        uint32_t s[64];
+        tmem_ld64(st, s);
         if (i < tile.whole_from || i >= tile.whole_to) {
-          const int key0 = block_key<CK>(job.keys, i), position = job.sg.past + by_group(p, job.r0 + row);
+          const int key0 = block_key<CK>(job.keys, i) + 64 * h;
+          const int position = job.sg.past + by_group(p, job.r0 + 128 * x + row);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < 2; ++j) {
             const uint32_t seen = seen_mask(p, job.keys, position, key0 + 32 * j);
 #pragma unroll
             for (int d = 0; d < 32; ++d)
               if (!((seen >> d) & 1u)) s[32 * j + d] = 0xff800000u;
           }
         }
-        float tops[8];
+        float tops[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) tops[k] = fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 8]));
+        for (int k = 0; k < 4; ++k) tops[k] = fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 4]));
 #pragma unroll
-        for (int j = 16; j < 128; j += 16)
+        for (int j = 8; j < 64; j += 8)
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            tops[k] = fmaxf(fmaxf(tops[k], __uint_as_float(s[j + k])), __uint_as_float(s[j + k + 8]));
-        const float top = p.scale_log2 *  // > 0: -inf stays
-                          fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
-                                fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
+          for (int k = 0; k < 4; ++k)
+            tops[k] = fmaxf(fmaxf(tops[k], __uint_as_float(s[j + k])), __uint_as_float(s[j + k + 4]));
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        // the other half's maximum. Its thread has read this word before it lets go of the scores below, so the next
+        // block's does not overtake
+        sm.scratch.row[x][h][row] = top;
+        tmem_fence_before();
+        pair_barrier();
+        tmem_fence_after();  // (the other half's scores are in registers: P may overwrite them)
+        top = p.scale_log2 * fmaxf(top, sm.scratch.row[x][1 - h][row]);  // > 0: -inf stays
+        if (S::EARLY) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.sfree[x]);
+        }
         const bool grow = top > m + LAZY || (m == -INFINITY && top > m);
-        if (__any_sync(0xffffffffu, grow)) {
+        const bool any_grow = __any_sync(0xffffffffu, grow);
+        if ((S::EARLY || any_grow) && n > n0) {  // the last V product: read P (EARLY) and wrote O
+          wait(&sm.ofull[x], (n - 1) & 1);
+          tmem_fence_after();
+        }
+        if (any_grow) {
           const float now = grow ? top : m, fix = grow ? ex2(m - now) : 1.f;
-          if (n > n0) {
-            ok = __all_sync(0xffffffffu, wait_bounded(&ofull[x], (n - 1) & 1, p.timeout_ns));
-            if (!ok) break;
-            tmem_fence_after();
+          if (n > n0)
 #pragma unroll
-            for (int j = 0; j < HD / 32; ++j) {
+            for (int j = 0; j < HD / 64; ++j) {
               uint32_t o[32];
               tmem_ld32(ot + 32 * j, o);
 #pragma unroll
               for (int d = 0; d < 32; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * fix);
               tmem_st32(ot + 32 * j, o);
             }
-          }
           l *= fix;
           m = now;
         }
         const float base = m == -INFINITY ? 0.f : m;
         const uint64_t base2 = f2(-base, -base);
-        uint64_t sums[4] = {0, 0, 0, 0};
+        uint64_t sums[2] = {0, 0};
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t w[32];
+        for (int part = 0; part < 2; ++part) {
+          uint32_t w[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int e = 64 * half + 2 * j;
+          for (int j = 0; j < 16; ++j) {
+            const int e = 32 * part + 2 * j;
             const uint64_t y = fma2(f2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, base2);
             float2 v;
             if ((j & 3) == 3 && POLY) {
@@ -921,31 +974,36 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
               v = unf2(y);
               v = make_float2(ex2(v.x), ex2(v.y));
             }
-            sums[j & 3] = add2(sums[j & 3], f2(v.x, v.y));
+            sums[j & 1] = add2(sums[j & 1], f2(v.x, v.y));
             w[j] = Half16<DT>::pack(v.x, v.y);
           }
-          tmem_st32(st + 32 * half, w);
+          tmem_st16(pt + 16 * part, w);
           tmem_wait_st();
           tmem_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&pfull[2 * x + half]);
+          if (lane == 0) mbar_arrive(&sm.pfull[x][part]);
         }
-        const float2 total = unf2(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+        const float2 total = unf2(add2(sums[0], sums[1]));
         l += total.x + total.y;
         ++n;
       }
       // the tile's sums: out, or into this block's part
       const bool any = n > n0;
-      if (any && ok) {
-        ok = __all_sync(0xffffffffu, wait_bounded(&ofull[x], (n - 1) & 1, p.timeout_ns));
+      if (any) {
+        wait(&sm.ofull[x], (n - 1) & 1);
         tmem_fence_after();
       }
+      pair_barrier();  // the last maxima have been read
+      sm.scratch.row[x][h][row] = l;
+      pair_barrier();
+      l = sm.scratch.row[x][0][row] + sm.scratch.row[x][1][row];
+      pair_barrier();
       const Segment sg = job.sg;
-      const int r1 = job.r1, r = job.r0 + row, t = by_group(p, r);
+      const int r1 = job.r1, trow = 128 * x + row, r = job.r0 + trow, t = by_group(p, r);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&jempty[jn % JOBS]);
+      if (lane == 0) mbar_arrive(&sm.jempty[jn % JOBS]);
       char* out = (char*)p.out + 2 * ((long long)(sg.first_row + t) * p.o_row +
-                                      (long long)(sg.kvh * p.group + r - t * p.group) * p.o_head);
+                                      (long long)(sg.kvh * p.group + r - t * p.group) * p.o_head + HD / 2 * h);
       auto scale_of = [](float ls) { return ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls); };  // nothing seen: zero; NaN stays
       auto write = [&](const float (&o)[32], int j, float inv) {
 #pragma unroll
@@ -965,7 +1023,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       };
       if (sg.parts == 1) {
 #pragma unroll
-        for (int j = 0; j < HD / 32; ++j) {
+        for (int j = 0; j < HD / 64; ++j) {
           float o[32];
           sums_of(j, o);
           if (r <= r1) write(o, j, scale_of(l));
@@ -973,21 +1031,20 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         tmem_fence_before();
         continue;
       }
-      const int own = blockIdx.x - sg.lead;
-      const bool keep = others_done<256>(p.tickets + sg.lead, sg.parts);
-      if (!keep) {
+      const int own = blockIdx.x - sg.lead, at_row = (HD / 8 * h) * CT + trow;
+      if (!others_done<TILE_THREADS>(p.tickets + sg.lead, sg.parts, &sm.flag)) {
         float* part = p.parts + (size_t)part_place(sg, own) * PART;
 #pragma unroll
-        for (int j = 0; j < HD / 32; ++j) {
+        for (int j = 0; j < HD / 64; ++j) {
           float o[32];
           sums_of(j, o);
 #pragma unroll
           for (int d = 0; d < 32; d += 4)
-            __stcg(reinterpret_cast<float4*>(part + ((size_t)(8 * j + d / 4) * CT + row) * 4),
+            __stcg(reinterpret_cast<float4*>(part) + at_row + (8 * j + d / 4) * CT,
                    make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]));
         }
-        __stcg(reinterpret_cast<float2*>(part + (size_t)CT * HD) + row, make_float2(m, l));
-        if (!last_of<256>(p.tickets + sg.lead, sg.parts)) {
+        if (h == 0) __stcg(reinterpret_cast<float2*>(part + (size_t)CT * HD) + trow, make_float2(m, l));
+        if (!last_of<TILE_THREADS>(p.tickets + sg.lead, sg.parts, &sm.flag)) {
           tmem_fence_before();
           continue;
         }
@@ -995,56 +1052,51 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       // the parts in their order, whoever is last: the same sums every time
       auto ml_of = [&](int k) {
         return k == own ? make_float2(m, l)
-                        : __ldcg(reinterpret_cast<const float2*>(p.parts + (size_t)part_place(sg, k) * PART + CT * HD) + row);
+                        : __ldcg(reinterpret_cast<const float2*>(p.parts + (size_t)part_place(sg, k) * PART + CT * HD) + trow);
       };
       float top = -INFINITY, ls = 0.f;
 #pragma unroll 4
       for (int k = 0; k < sg.parts; ++k) top = fmaxf(top, ml_of(k).x);
       const float base = top == -INFINITY ? 0.f : top;
-      float acc[HD];
-#pragma unroll
-      for (int d = 0; d < HD; ++d) acc[d] = 0.f;
+#pragma unroll 4
       for (int k = 0; k < sg.parts; ++k) {
         const float2 ml = ml_of(k);
-        const float f = ex2(ml.x - base);
-        ls += f * ml.y;
-        if (k == own) {
+        ls += ex2(ml.x - base) * ml.y;
+      }
+#pragma unroll 1
+      for (int j = 0; j < HD / 64; ++j) {
+        float acc[32];
 #pragma unroll
-          for (int j = 0; j < HD / 32; ++j) {
-            float o[32];
+        for (int d = 0; d < 32; ++d) acc[d] = 0.f;
+        for (int k = 0; k < sg.parts; ++k) {
+          float o[32];
+          if (k == own) {
             sums_of(j, o);
+          } else {
+            const float4* at = reinterpret_cast<const float4*>(p.parts + (size_t)part_place(sg, k) * PART) + at_row + 8 * j * CT;
 #pragma unroll
-            for (int d = 0; d < 32; ++d) acc[32 * j + d] += f * o[d];
+            for (int d = 0; d < 32; d += 4) {
+              const float4 v = __ldcg(at + (d / 4) * CT);
+              o[d] = v.x;
+              o[d + 1] = v.y;
+              o[d + 2] = v.z;
+              o[d + 3] = v.w;
+            }
           }
-        } else {
-          const float4* at = reinterpret_cast<const float4*>(p.parts + (size_t)part_place(sg, k) * PART) + row;
+          const float f = ex2(ml_of(k).x - base);
 #pragma unroll
-          for (int d = 0; d < HD; d += 4) {
-            const float4 v = __ldcg(at + (size_t)(d / 4) * CT);
-            acc[d] += f * v.x;
-            acc[d + 1] += f * v.y;
-            acc[d + 2] += f * v.z;
-            acc[d + 3] += f * v.w;
-          }
+          for (int d = 0; d < 32; ++d) acc[d] += f * o[d];
         }
+        if (r <= r1) write(acc, j, scale_of(ls));
       }
       tmem_fence_before();
-      if (r <= r1) {
-#pragma unroll
-        for (int j = 0; j < HD / 32; ++j) {
-          float o[32];
-#pragma unroll
-          for (int d = 0; d < 32; ++d) o[d] = acc[32 * j + d];
-          write(o, j, scale_of(ls));
-        }
-      }
     }
     if (!ok && lane == 0) atomicCAS(p.error, 0, 0x214);
     tmem_fence_before();
   }
   __syncthreads();
-  if (warp == 9) {
-    wait_bounded(done, 0, p.timeout_ns);  // no MMA may still write
+  if (warp == 17) {
+    wait_bounded(&sm.done, 0, p.timeout_ns);  // no MMA may still write
     tmem_fence_after();
     tmem_free(tmem, 512);
   }
@@ -1102,7 +1154,7 @@ template <int DT, int HD>
 bool launch_typed(bool chunk, const CUtensorMap& tk, const CUtensorMap& tv, const AttendParams& p, int device,
                   cudaStream_t stream) {
   static bool rows_sized[MAX_DEVICES] = {}, chunk_sized[MAX_DEVICES] = {};
-  return chunk ? launch(chunk_kernel<DT, HD>, chunk_sized, CHUNK_THREADS, ChunkShape<HD>::SMEM, tk, tv, p, device, stream)
+  return chunk ? launch(chunk_kernel<DT, HD>, chunk_sized, CHUNK_THREADS, (int)sizeof(ChunkShared<HD>), tk, tv, p, device, stream)
                : launch(rows_kernel<DT, HD>, rows_sized, ROW_THREADS, RowShape<HD>::SMEM, tk, tv, p, device, stream);
 }
 

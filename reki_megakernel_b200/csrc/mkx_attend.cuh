@@ -92,12 +92,17 @@ __device__ __forceinline__ long long snapped(long long u, long long at, int unit
   return v <= snap ? u - v : units - v <= snap ? u + (units - v) : u;
 }
 
-// All threads of the block call this; false if the block has nothing to do.
+// All threads of the block call this; false if the block has nothing to do. The scratch is free again after the next
+// block barrier.
+struct LineScratch {
+  long long sums[2][32];
+  Line line;
+};
 template <int MT, int KT, int NTH>
-__device__ __forceinline__ bool find_line(const AttendParams& p, Line& out) {
+__device__ __forceinline__ bool find_line(const AttendParams& p, LineScratch& scratch, Line& out) {
   constexpr int W = NTH / 32;
-  __shared__ long long sums[2][W];
-  __shared__ Line line;
+  auto& sums = scratch.sums;
+  Line& line = scratch.line;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Episode e;
   long long all = 0, mine = 0;
@@ -235,30 +240,30 @@ __device__ __forceinline__ int part_place(const Segment& s, int k) { return 2 * 
 // Called by all NTH threads (named barrier 1); leaves the ticket at zero if so. The others' parts are then visible
 // through __ldcg.
 template <int NTH>
-__device__ __forceinline__ bool others_done(unsigned* ticket, int parts) {
-  __shared__ int done;
+__device__ __forceinline__ bool others_done(unsigned* ticket, int parts, int* done) {
   if (threadIdx.x == 0) {
-    done = ld_acquire_i32(reinterpret_cast<int*>(ticket)) == parts - 1;
-    if (done) *ticket = 0;
+    *done = ld_acquire_i32(reinterpret_cast<int*>(ticket)) == parts - 1;
+    if (*done) *ticket = 0;
   }
   asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");
-  return done;
+  const bool all = *done;
+  asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");  // the word is free again
+  return all;
 }
 // Called by all NTH threads (named barrier 1) after they wrote their part k of a split tile with __stcg: whether
 // this block is the last of the parts [k0, k0 + n) under ticket `ticket`, which is left at zero. The others' parts are
 // then visible through __ldcg.
 template <int NTH>
-__device__ __forceinline__ bool last_of(unsigned* ticket, int n) {
-  __shared__ int last;
+__device__ __forceinline__ bool last_of(unsigned* ticket, int n, int* last) {
   __threadfence();
   asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");
   if (threadIdx.x == 0) {
-    last = atomicAdd(ticket, 1u) == (unsigned)n - 1;
-    if (last) *ticket = 0;
+    *last = atomicAdd(ticket, 1u) == (unsigned)n - 1;
+    if (*last) *ticket = 0;
     __threadfence();
   }
   asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");
-  return last;
+  return *last;  // (the word is written again only behind the first barrier of the next call)
 }
 
 // The keys that the rows of a tile see: blocks of KT keys, first those of the sinks, then from the
