@@ -398,25 +398,24 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
 // ---- chunks ----------------------------------------------------------------------------------------
 // chunk_kernel: tiles of 256 rows as two tiles A, B of 128, one CTA per SM. Both products run on
 // tcgen05 (128-key blocks): S = Q K^T from shared memory into TMEM, O += P V with P read from TMEM and V
-// as TMA left it (dims contiguous). Eight warps per tile: two threads share a row, half of the keys of a
-// block each, so that what lies between S and P, which nothing else of the same tile can overlap, is
-// short. They exchange their maxima once a block. O is rescaled only when a maximum has grown by more
-// than 2^8 since the last time, which is rare after the first blocks: P stays below 2^8, far inside both
-// types. At head_dim 128 TMEM is full with two tiles of S and O, and P overwrites the scores it came
+// as TMA left it (dims contiguous). Four warps per tile, one thread per row: no shuffles, the row's
+// maximum and sum stay in registers. O is rescaled only when a maximum has grown by more than 2^8 since the
+// last time, which is rare after the first blocks: P stays below 2^8, far inside both types, and a block's
+// exponentials begin with the last block's maximum, without waiting for its own (they are taken again if it
+// grew). At head_dim 128 TMEM is full with two tiles of S and O, and P overwrites the scores it came
 // from: a tile's products wait for its softmax and the other way round, and the two tiles alternate. At
 // head_dim 64 P has columns of its own, and the next scores are there before the last ones are done.
 // Bound by the exponentials at head_dim 64 (16 a clock per SM: 2048 clocks for two 128 x 128 tiles, whose
 // products take 1024), by both alike at 128.
 constexpr int CT = 256;
 constexpr int CK = 128;
-constexpr int TILE_THREADS = 512;                   // warps 0-7 tile A, 8-15 tile B
-constexpr int CHUNK_THREADS = TILE_THREADS + 128;   // 16 TMA, 17 and 19 MMA, 18 walks the line
-// Registers per thread: 640 x 96 at launch; the warps of the tiles, half a row of scores each, take 104, the others 64
-// (512 x 104 + 128 x 64 = 640 x 96).
-constexpr int TILE_REGS = 104, OTHER_REGS = 64;
-constexpr bool POLY = true;
+constexpr int TILE_THREADS = 256;                   // warps 0-3 tile A, 4-7 tile B
+constexpr int CHUNK_THREADS = TILE_THREADS + 128;   // 8 TMA, 9 and 11 MMA, 10 walks the line
+// Registers per thread: 384 x 168 at launch; the warps of the tiles, a row of scores each, take 216, the others 72
+// (256 x 216 + 128 x 72 = 384 x 168).
+constexpr int TILE_REGS = 216, OTHER_REGS = 72;
 constexpr float LAZY = 8.f;  // log2 of the growth that is let pass
-constexpr int JOBS = 2;
+constexpr int JOBS = 4;
 
 template <int HD>
 struct ChunkShape {
@@ -424,6 +423,7 @@ struct ChunkShape {
   static constexpr int TILE = CK * HD * 2;              // one K or V block
   static constexpr int HALF = CK * 128;                 // its 64-dim half
   static constexpr int SLOTS = HD == 128 ? 5 : 8;
+  static constexpr int POLY_EACH = 4;                   // every so many pairs of exponentials is a polynomial
   static constexpr int QHALF = CT * 128;
   // TMEM columns of a tile: S, O, P
   static __device__ __forceinline__ uint32_t s_at(int x) { return 128 * x; }
@@ -501,14 +501,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
       "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
       "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
       "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -600,15 +592,12 @@ template <int HD>
 struct ChunkShared {
   char ring[ChunkShape<HD>::SLOTS * ChunkShape<HD>::TILE];  // K and V blocks
   char q[CT * HD * 2];                                      // [HD / 64][256 rows][128 bytes], 128-byte swizzle
-  union {
-    LineScratch line;
-    float row[2][2][128];  // [tile][half]: what the two threads of a row tell each other
-  } scratch;
+  LineScratch line;
   uint64_t full[ChunkShape<HD>::SLOTS], empty[ChunkShape<HD>::SLOTS], raw;
   uint64_t qfull[2];     // a tile's rows of Q are in shared memory
   uint64_t sfull[2];     // its scores are in TMEM
   uint64_t sfree[2];     // its scores are in registers (EARLY)
-  uint64_t pfull[2][2];  // the first, the second half of the probabilities of each thread are in TMEM
+  uint64_t pfull[2][2];  // the first, the second half of its probabilities are
   uint64_t ofull[2];     // its sums include them
   uint64_t done;
   uint64_t turns[2];     // the MMA warps' turns
@@ -640,31 +629,31 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     }
     mbar_init(&sm.raw, 1);
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&sm.qfull[x], 8);
+      mbar_init(&sm.qfull[x], 4);
       mbar_init(&sm.sfull[x], 1);
-      mbar_init(&sm.sfree[x], 8);
-      mbar_init(&sm.pfull[x][0], 8);
-      mbar_init(&sm.pfull[x][1], 8);
+      mbar_init(&sm.sfree[x], 4);
+      mbar_init(&sm.pfull[x][0], 4);
+      mbar_init(&sm.pfull[x][1], 4);
       mbar_init(&sm.ofull[x], 1);
       mbar_init(&sm.turns[x], 1);
     }
     mbar_init(&sm.done, 2);
     for (int j = 0; j < JOBS; ++j) {
       mbar_init(&sm.jfull[j], 1);
-      mbar_init(&sm.jempty[j], 19);  // the producer, the two MMA warps, the sixteen warps of the tiles
+      mbar_init(&sm.jempty[j], 11);  // the producer, the two MMA warps, the eight warps of the tiles
     }
     fence_mbar_init();
   }
   Line line;
-  if (!find_line<CT, CK, CHUNK_THREADS>(p, sm.scratch.line, line)) return;
-  if (warp == 17) tmem_alloc(&sm.tmem, 512);
+  if (!find_line<CT, CK, CHUNK_THREADS>(p, sm.line, line)) return;
+  if (warp == 9) tmem_alloc(&sm.tmem, 512);
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = sm.tmem;
 
-  if (warp >= 16) {
+  if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-    if (warp == 16) {
+    if (warp == 8) {
       // producer: slots hold K, V, K, V, ... of the blocks in order; lane j fetches the j-th page
       const int rows_box = min(1 << p.shift, CK), boxes = CK / rows_box;
       bool ok = true;
@@ -720,8 +709,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         atomicCAS(p.error, 0, 0x211);
         for (int k = max(0, n - SLOTS); k < n; ++k) wait_bounded(&sm.full[k % SLOTS], (k / SLOTS) & 1, p.timeout_ns);
       }
-    } else if (warp != 18) {
-      // the products of tile A (warp 17) and tile B (warp 19): two warps, because what one does around a block's
+    } else if (warp != 10) {
+      // the products of tile A (warp 9) and tile B (warp 11): two warps, because what one does around a block's
       // products, a few hundred clocks, then hides behind the other's. Without columns for P beside S they take turns,
       // so that one tile's products run under the other's softmax (otherwise both do the same at the same time: 281
       // instead of 239 us for 2011 rows after 6007, 32/8 heads x 128)
@@ -729,7 +718,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       constexpr uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(128 >> 4) << 24);
       constexpr uint32_t id_qk = base | ((uint32_t)(CK >> 3) << 17);
       constexpr uint32_t id_pv = base | ((uint32_t)(HD >> 3) << 17) | (1u << 16);  // V: dims contiguous
-      const int x = uniform(warp == 19);
+      const int x = uniform(warp == 11);
       const uint32_t lead = elect_one(), tm = (uint32_t)uniform((int)tmem);
       const uint32_t st = tm + S::s_at(x), ot = tm + S::o_at(x), pt = tm + S::p_at(x);
       const uint32_t q = desc_low(smem_u32(qs), 0) + x * (128 * 128 >> 4), k_low = desc_low(smem_u32(ring), 0),
@@ -774,7 +763,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             tmem_fence_after();
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const int kk = 4 * (k >> 1) + 2 * part + (k & 1);  // keys 0-31 and 64-95, then the others
+              const int kk = 4 * part + k;
               umma_ts(lead, ot, pt + 8 * kk, v + kk * (2048 >> 4), id_pv, (part > 0 || k > 0) ? 1u : (done > n0 ? 1u : 0u));
             }
           }
@@ -849,13 +838,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     __syncwarp();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TILE_REGS));
-    // two threads per row: keys 64 h .. of a block, dims HD / 2 * h .. of the sums
-    const int x = warp >> 3, h = (warp >> 2) & 1, row = 32 * (warp & 3) + lane;
+    const int x = warp >> 2, row = threadIdx.x;  // one row per thread
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t st = tmem + lanes + S::s_at(x) + 64 * h, ot = tmem + lanes + S::o_at(x) + HD / 2 * h,
-                   pt = tmem + lanes + S::p_at(x) + 32 * h;
-    const int pair = 2 + 4 * x + (warp & 3);  // named barrier of the two warps that share rows
-    auto pair_barrier = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory"); };
+    const uint32_t st = tmem + lanes + S::s_at(x), ot = tmem + lanes + S::o_at(x), pt = tmem + lanes + S::p_at(x);
     const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
     int n = 0;  // blocks of this tile since the start
     // After a wait that ran out the warp goes on without waiting: others of its barriers still count on it
@@ -879,12 +864,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         if (n == n0) {
           // the tile's Q into shared memory, coalesced: 16-byte chunks of a row by neighbouring threads. Only for a
           // tile with work in this segment: warps without any run ahead, by more phases than a barrier tells apart
-          const int first = job.r0 + 128 * x, last = job.r1, head = job.sg.kvh * p.group, th = threadIdx.x & 255;
+          const int first = job.r0 + 128 * x, last = job.r1, head = job.sg.kvh * p.group, th = threadIdx.x & 127;
           const char* rows = (const char*)p.q + 2 * (long long)job.sg.first_row * p.q_row;
-          uint4 v[HD / 16];
+          uint4 v[HD / 8];
 #pragma unroll
-          for (int k = 0; k < HD / 16; ++k) {  // all loads in flight at once
-            const int e = th + 256 * k, r = first + e / (HD / 8), ch = e % (HD / 8);
+          for (int k = 0; k < HD / 8; ++k) {  // all loads in flight at once
+            const int e = th + 128 * k, r = first + e / (HD / 8), ch = e % (HD / 8);
             v[k] = make_uint4(0, 0, 0, 0);
             if (r <= last) {
               const int t = by_group(p, r);
@@ -893,8 +878,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             }
           }
 #pragma unroll
-          for (int k = 0; k < HD / 16; ++k) {
-            const int e = th + 256 * k, qr = 128 * x + e / (HD / 8), ch = e % (HD / 8);
+          for (int k = 0; k < HD / 8; ++k) {
+            const int e = th + 128 * k, qr = 128 * x + e / (HD / 8), ch = e % (HD / 8);
             *reinterpret_cast<uint4*>(qs + (ch >> 3) * S::QHALF + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4)) =
                 make_uint4(signed_q(p, v[k].x), signed_q(p, v[k].y), signed_q(p, v[k].z), signed_q(p, v[k].w));
           }
@@ -904,39 +889,56 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         }
         wait(&sm.sfull[x], n & 1);
         tmem_fence_after();
-        uint32_t s[64];
-        tmem_ld64(st, s);
-        if (i < tile.whole_from || i >= tile.whole_to) {
-          const int key0 = block_key<CK>(job.keys, i) + 64 * h;
-          const int position = job.sg.past + by_group(p, job.r0 + 128 * x + row);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t seen = seen_mask(p, job.keys, position, key0 + 32 * j);
-#pragma unroll
-            for (int d = 0; d < 32; ++d)
-              if (!((seen >> d) & 1u)) s[32 * j + d] = 0xff800000u;
-          }
-        }
-        float tops[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) tops[k] = fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 4]));
-#pragma unroll
-        for (int j = 8; j < 64; j += 8)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tops[k] = fmaxf(fmaxf(tops[k], __uint_as_float(s[j + k])), __uint_as_float(s[j + k + 4]));
-        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        // the other half's maximum. Its thread has read this word before it lets go of the scores below, so the next
-        // block's does not overtake
-        sm.scratch.row[x][h][row] = top;
-        tmem_fence_before();
-        pair_barrier();
-        tmem_fence_after();  // (the other half's scores are in registers: P may overwrite them)
-        top = p.scale_log2 * fmaxf(top, sm.scratch.row[x][1 - h][row]);  // > 0: -inf stays
-        if (S::EARLY) {
+        uint32_t s[2][64];
+        tmem_ld64(st, s[0]);
+        tmem_ld64(st + 64, s[1]);
+        if (S::EARLY) {  // the next scores may come
+          tmem_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.sfree[x]);
         }
+        if (i < tile.whole_from || i >= tile.whole_to) {
+          const int key0 = block_key<CK>(job.keys, i), position = job.sg.past + by_group(p, job.r0 + row);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t seen = seen_mask(p, job.keys, position, key0 + 32 * j);
+            if (__all_sync(0xffffffffu, seen == ~0u)) continue;
+#pragma unroll
+            for (int d = 0; d < 32; ++d)
+              if (!((seen >> d) & 1u)) s[j >> 1][32 * (j & 1) + d] = 0xff800000u;
+          }
+        }
+        float tops[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) tops[k] = fmaxf(__uint_as_float(s[0][k]), __uint_as_float(s[0][k + 8]));
+#pragma unroll
+        for (int j = 16; j < 128; j += 16)
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            tops[k] = fmaxf(fmaxf(tops[k], __uint_as_float(s[j >> 6][(j & 63) + k])), __uint_as_float(s[j >> 6][(j & 63) + k + 8]));
+        // half of a block's probabilities, as words of P; their sum is added to `sums`
+        auto half_of = [&](const uint32_t (&sh)[64], float base, uint32_t (&w)[32], uint64_t (&sums)[4]) {
+          const uint64_t base2 = f2(-base, -base);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const uint64_t y = fma2(f2(__uint_as_float(sh[2 * j]), __uint_as_float(sh[2 * j + 1])), scale2, base2);
+            float2 v;
+            if (j % S::POLY_EACH == S::POLY_EACH - 1) {
+              v = exp2_pair<DT>(y);
+            } else {
+              v = unf2(y);
+              v = make_float2(ex2(v.x), ex2(v.y));
+            }
+            sums[j & 3] = add2(sums[j & 3], f2(v.x, v.y));
+            w[j] = Half16<DT>::pack(v.x, v.y);
+          }
+        };
+        uint32_t w[32];
+        uint64_t sums[4] = {0, 0, 0, 0};
+        half_of(s[0], m == -INFINITY ? 0.f : m, w, sums);
+        const float top = p.scale_log2 *  // > 0: -inf stays
+                          fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
+                                fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
         const bool grow = top > m + LAZY || (m == -INFINITY && top > m);
         const bool any_grow = __any_sync(0xffffffffu, grow);
         if ((S::EARLY || any_grow) && n > n0) {  // the last V product: read P (EARLY) and wrote O
@@ -947,7 +949,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           const float now = grow ? top : m, fix = grow ? ex2(m - now) : 1.f;
           if (n > n0)
 #pragma unroll
-            for (int j = 0; j < HD / 64; ++j) {
+            for (int j = 0; j < HD / 32; ++j) {
               uint32_t o[32];
               tmem_ld32(ot + 32 * j, o);
 #pragma unroll
@@ -956,34 +958,19 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             }
           l *= fix;
           m = now;
+          sums[0] = sums[1] = sums[2] = sums[3] = 0;
+          half_of(s[0], m == -INFINITY ? 0.f : m, w, sums);
         }
-        const float base = m == -INFINITY ? 0.f : m;
-        const uint64_t base2 = f2(-base, -base);
-        uint64_t sums[2] = {0, 0};
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-          uint32_t w[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int e = 32 * part + 2 * j;
-            const uint64_t y = fma2(f2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, base2);
-            float2 v;
-            if ((j & 3) == 3 && POLY) {
-              v = exp2_pair<DT>(y);
-            } else {
-              v = unf2(y);
-              v = make_float2(ex2(v.x), ex2(v.y));
-            }
-            sums[j & 1] = add2(sums[j & 1], f2(v.x, v.y));
-            w[j] = Half16<DT>::pack(v.x, v.y);
-          }
-          tmem_st16(pt + 16 * part, w);
+          if (part == 1) half_of(s[1], m == -INFINITY ? 0.f : m, w, sums);
+          tmem_st32(pt + 32 * part, w);
           tmem_wait_st();
           tmem_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.pfull[x][part]);
         }
-        const float2 total = unf2(add2(sums[0], sums[1]));
+        const float2 total = unf2(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
         l += total.x + total.y;
         ++n;
       }
@@ -993,17 +980,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         wait(&sm.ofull[x], (n - 1) & 1);
         tmem_fence_after();
       }
-      pair_barrier();  // the last maxima have been read
-      sm.scratch.row[x][h][row] = l;
-      pair_barrier();
-      l = sm.scratch.row[x][0][row] + sm.scratch.row[x][1][row];
-      pair_barrier();
       const Segment sg = job.sg;
-      const int r1 = job.r1, trow = 128 * x + row, r = job.r0 + trow, t = by_group(p, r);
+      const int r1 = job.r1, r = job.r0 + row, t = by_group(p, r);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.jempty[jn % JOBS]);
       char* out = (char*)p.out + 2 * ((long long)(sg.first_row + t) * p.o_row +
-                                      (long long)(sg.kvh * p.group + r - t * p.group) * p.o_head + HD / 2 * h);
+                                      (long long)(sg.kvh * p.group + r - t * p.group) * p.o_head);
       auto scale_of = [](float ls) { return ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls); };  // nothing seen: zero; NaN stays
       auto write = [&](const float (&o)[32], int j, float inv) {
 #pragma unroll
@@ -1023,7 +1005,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       };
       if (sg.parts == 1) {
 #pragma unroll
-        for (int j = 0; j < HD / 64; ++j) {
+        for (int j = 0; j < HD / 32; ++j) {
           float o[32];
           sums_of(j, o);
           if (r <= r1) write(o, j, scale_of(l));
@@ -1031,19 +1013,19 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         tmem_fence_before();
         continue;
       }
-      const int own = blockIdx.x - sg.lead, at_row = (HD / 8 * h) * CT + trow;
+      const int own = blockIdx.x - sg.lead;
       if (!others_done<TILE_THREADS>(p.tickets + sg.lead, sg.parts, &sm.flag)) {
         float* part = p.parts + (size_t)part_place(sg, own) * PART;
 #pragma unroll
-        for (int j = 0; j < HD / 64; ++j) {
+        for (int j = 0; j < HD / 32; ++j) {
           float o[32];
           sums_of(j, o);
 #pragma unroll
           for (int d = 0; d < 32; d += 4)
-            __stcg(reinterpret_cast<float4*>(part) + at_row + (8 * j + d / 4) * CT,
+            __stcg(reinterpret_cast<float4*>(part) + row + (8 * j + d / 4) * CT,
                    make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]));
         }
-        if (h == 0) __stcg(reinterpret_cast<float2*>(part + (size_t)CT * HD) + trow, make_float2(m, l));
+        __stcg(reinterpret_cast<float2*>(part + (size_t)CT * HD) + row, make_float2(m, l));
         if (!last_of<TILE_THREADS>(p.tickets + sg.lead, sg.parts, &sm.flag)) {
           tmem_fence_before();
           continue;
@@ -1052,7 +1034,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       // the parts in their order, whoever is last: the same sums every time
       auto ml_of = [&](int k) {
         return k == own ? make_float2(m, l)
-                        : __ldcg(reinterpret_cast<const float2*>(p.parts + (size_t)part_place(sg, k) * PART + CT * HD) + trow);
+                        : __ldcg(reinterpret_cast<const float2*>(p.parts + (size_t)part_place(sg, k) * PART + CT * HD) + row);
       };
       float top = -INFINITY, ls = 0.f;
 #pragma unroll 4
@@ -1064,7 +1046,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         ls += ex2(ml.x - base) * ml.y;
       }
 #pragma unroll 1
-      for (int j = 0; j < HD / 64; ++j) {
+      for (int j = 0; j < HD / 32; ++j) {
         float acc[32];
 #pragma unroll
         for (int d = 0; d < 32; ++d) acc[d] = 0.f;
@@ -1073,7 +1055,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           if (k == own) {
             sums_of(j, o);
           } else {
-            const float4* at = reinterpret_cast<const float4*>(p.parts + (size_t)part_place(sg, k) * PART) + at_row + 8 * j * CT;
+            const float4* at = reinterpret_cast<const float4*>(p.parts + (size_t)part_place(sg, k) * PART) + row + 8 * j * CT;
 #pragma unroll
             for (int d = 0; d < 32; d += 4) {
               const float4 v = __ldcg(at + (d / 4) * CT);
@@ -1095,7 +1077,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     tmem_fence_before();
   }
   __syncthreads();
-  if (warp == 17) {
+  if (warp == 9) {
     wait_bounded(&sm.done, 0, p.timeout_ns);  // no MMA may still write
     tmem_fence_after();
     tmem_free(tmem, 512);
