@@ -399,10 +399,8 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
 // chunk_kernel: tiles of 256 rows as two tiles A, B of 128, one CTA per SM. Both products run on
 // tcgen05 (128-key blocks): S = Q K^T from shared memory into TMEM, O += P V with P read from TMEM and V
 // as TMA left it (dims contiguous). Four warps per tile, one thread per row: no shuffles, the row's
-// maximum and sum stay in registers. The maximum is only a reference that keeps exponentials in range, so
-// it is left as it was while the sum of a row's next 64 exponentials is at most 2^14 (which both types of P
-// hold); only beyond that, and where a row has seen nothing yet, the new one is formed and O rescaled. At
-// head_dim 128 TMEM is full with two tiles of S and O, and P overwrites the scores it came
+// maximum and sum stay in registers. O is rescaled only when a maximum has grown by more than 2^8 since the
+// last time, which is rare after the first blocks: P stays below 2^8, far inside both types. At head_dim 128 TMEM is full with two tiles of S and O, and P overwrites the scores it came
 // from: a tile's products wait for its softmax and the other way round, and the two tiles alternate. At
 // head_dim 64 P has columns of its own, and the next scores are there before the last ones are done.
 // Bound by the exponentials at head_dim 64 (16 a clock per SM: 2048 clocks for two 128 x 128 tiles, whose
@@ -411,10 +409,10 @@ constexpr int CT = 256;
 constexpr int CK = 128;
 constexpr int TILE_THREADS = 256;                   // warps 0-3 tile A, 4-7 tile B
 constexpr int CHUNK_THREADS = TILE_THREADS + 128;   // 8 TMA, 9 and 11 MMA, 10 walks the line
-// Registers per thread: 384 x 168 at launch; the warps of the tiles, a row of scores each, take 200, the others 104
-// (256 x 200 + 128 x 104 = 384 x 168).
-constexpr int TILE_REGS = 200, OTHER_REGS = 104;
-constexpr float MOST = 16384.f;  // the sum of a row's 64 probabilities up to which its maximum is left as it was
+// Registers per thread: 384 x 168 at launch; the warps of the tiles, a row of scores each, take 216, the others 72
+// (256 x 216 + 128 x 72 = 384 x 168).
+constexpr int TILE_REGS = 216, OTHER_REGS = 72;
+constexpr float LAZY = 8.f;  // log2 of the growth that is let pass
 constexpr int JOBS = 4;
 
 template <int HD>
@@ -598,7 +596,7 @@ struct ChunkShared {
   uint64_t sfull[2];     // its scores are in TMEM
   uint64_t sfree[2];     // its scores are in registers (EARLY)
   uint64_t pfull[2][2];  // the first, the second half of its probabilities are
-  uint64_t ofull[2][2];  // its sums include them
+  uint64_t ofull[2];     // its sums include them
   uint64_t done;
   uint64_t turns[2];     // the MMA warps' turns
   uint64_t jfull[JOBS], jempty[JOBS];
@@ -634,8 +632,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       mbar_init(&sm.sfree[x], 4);
       mbar_init(&sm.pfull[x][0], 4);
       mbar_init(&sm.pfull[x][1], 4);
-      mbar_init(&sm.ofull[x][0], 1);
-      mbar_init(&sm.ofull[x][1], 1);
+      mbar_init(&sm.ofull[x], 1);
       mbar_init(&sm.turns[x], 1);
     }
     mbar_init(&sm.done, 2);
@@ -767,8 +764,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
               const int kk = 4 * part + k;
               umma_ts(lead, ot, pt + 8 * kk, v + kk * (2048 >> 4), id_pv, (part > 0 || k > 0) ? 1u : (done > n0 ? 1u : 0u));
             }
-            commit_by(lead, &sm.ofull[x][part]);
           }
+          commit_by(lead, &sm.ofull[x]);
           commit_by(lead, &sm.empty[v_slot]);
           ++done;
           return true;
@@ -890,88 +887,93 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         }
         wait(&sm.sfull[x], n & 1);
         tmem_fence_after();
-        const bool masked = i < tile.whole_from || i >= tile.whole_to;
-        // half a block at a time, 64 keys: exponentials with the maximum as it was; their sum shows whether one has
-        // outgrown it
+        uint32_t s[2][64];
+        tmem_ld64(st, s[0]);
+        tmem_ld64(st + 64, s[1]);
+        if (S::EARLY) {  // the next scores may come
+          tmem_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.sfree[x]);
+        }
+        if (i < tile.whole_from || i >= tile.whole_to) {
+          const int key0 = block_key<CK>(job.keys, i), position = job.sg.past + by_group(p, job.r0 + row);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t seen = seen_mask(p, job.keys, position, key0 + 32 * j);
+            if (__all_sync(0xffffffffu, seen == ~0u)) continue;
+#pragma unroll
+            for (int d = 0; d < 32; ++d)
+              if (!((seen >> d) & 1u)) s[j >> 1][32 * (j & 1) + d] = 0xff800000u;
+          }
+        }
+        float tops[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) tops[k] = fmaxf(__uint_as_float(s[0][k]), __uint_as_float(s[0][k + 8]));
+#pragma unroll
+        for (int j = 16; j < 128; j += 16)
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            tops[k] = fmaxf(fmaxf(tops[k], __uint_as_float(s[j >> 6][(j & 63) + k])), __uint_as_float(s[j >> 6][(j & 63) + k + 8]));
+        // half of a block's probabilities, as words of P; their sum is added to `sums`
+        auto half_of = [&](const uint32_t (&sh)[64], float base, uint32_t (&w)[32], uint64_t (&sums)[4]) {
+          const uint64_t base2 = f2(-base, -base);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const uint64_t y = fma2(f2(__uint_as_float(sh[2 * j]), __uint_as_float(sh[2 * j + 1])), scale2, base2);
+            float2 v;
+            if (j % S::POLY_EACH == S::POLY_EACH - 1) {
+              v = exp2_pair<DT>(y);
+            } else {
+              v = unf2(y);
+              v = make_float2(ex2(v.x), ex2(v.y));
+            }
+            sums[j & 3] = add2(sums[j & 3], f2(v.x, v.y));
+            w[j] = Half16<DT>::pack(v.x, v.y);
+          }
+        };
+        uint32_t w[32];
+        uint64_t sums[4] = {0, 0, 0, 0};
+        const float top = p.scale_log2 *  // > 0: -inf stays
+                          fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
+                                fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
+        const bool grow = top > m + LAZY || (m == -INFINITY && top > m);
+        const bool any_grow = __any_sync(0xffffffffu, grow);
+        if ((S::EARLY || any_grow) && n > n0) {  // the last V product: read P (EARLY) and wrote O
+          wait(&sm.ofull[x], (n - 1) & 1);
+          tmem_fence_after();
+        }
+        if (any_grow) {
+          const float now = grow ? top : m, fix = grow ? ex2(m - now) : 1.f;
+          if (n > n0)
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) {
+              uint32_t o[32];
+              tmem_ld32(ot + 32 * j, o);
+#pragma unroll
+              for (int d = 0; d < 32; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * fix);
+              tmem_st32(ot + 32 * j, o);
+            }
+          l *= fix;
+          m = now;
+        }
+        half_of(s[0], m == -INFINITY ? 0.f : m, w, sums);
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-          uint32_t s[64], w[32];
-          tmem_ld64(st + 64 * part, s);
-          if (S::EARLY && part == 1) {  // the next scores may come
-            tmem_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.sfree[x]);
-          }
-          if (masked) {
-            const int key0 = block_key<CK>(job.keys, i) + 64 * part, position = job.sg.past + by_group(p, job.r0 + row);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint32_t seen = seen_mask(p, job.keys, position, key0 + 32 * j);
-              if (__all_sync(0xffffffffu, seen == ~0u)) continue;
-#pragma unroll
-              for (int d = 0; d < 32; ++d)
-                if (!((seen >> d) & 1u)) s[32 * j + d] = 0xff800000u;
-            }
-          }
-          auto exponentials = [&](float base) {
-            const uint64_t base2 = f2(-base, -base);
-            uint64_t sums[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const uint64_t y = fma2(f2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), scale2, base2);
-              float2 v;
-              if (j % S::POLY_EACH == S::POLY_EACH - 1) {
-                v = exp2_pair<DT>(y);
-              } else {
-                v = unf2(y);
-                v = make_float2(ex2(v.x), ex2(v.y));
-              }
-              sums[j & 3] = add2(sums[j & 3], f2(v.x, v.y));
-              w[j] = Half16<DT>::pack(v.x, v.y);
-            }
-            const float2 both = unf2(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
-            return both.x + both.y;
-          };
-          float sum = exponentials(m == -INFINITY ? 0.f : m);
-          const bool written = n > n0 || part == 1;  // O holds something
-          if (__any_sync(0xffffffffu, !(sum <= MOST) || m == -INFINITY)) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < 64; j += 2) top = fmaxf(fmaxf(top, __uint_as_float(s[j])), __uint_as_float(s[j + 1]));
-            const float now = fmaxf(m, p.scale_log2 * top), fix = m == now ? 1.f : ex2(m - now);  // scale > 0: -inf stays
-            if (written) {  // the last V product, which wrote O
-              wait(&sm.ofull[x][1 - part], (part ? n : n - 1) & 1);
-              tmem_fence_after();
-#pragma unroll
-              for (int j = 0; j < HD / 32; ++j) {
-                uint32_t o[32];
-                tmem_ld32(ot + 32 * j, o);
-#pragma unroll
-                for (int d = 0; d < 32; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * fix);
-                tmem_st32(ot + 32 * j, o);
-              }
-            }
-            l *= fix;
-            m = now;
-            sum = exponentials(m == -INFINITY ? 0.f : m);
-          }
-          l += sum;
-          if (S::EARLY && n > n0) {  // the last block's product of this half has read P
-            wait(&sm.ofull[x][part], (n - 1) & 1);
-            tmem_fence_after();
-          }
+          if (part == 1) half_of(s[1], m == -INFINITY ? 0.f : m, w, sums);
           tmem_st32(pt + 32 * part, w);
           tmem_wait_st();
           tmem_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.pfull[x][part]);
         }
+        const float2 total = unf2(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+        l += total.x + total.y;
         ++n;
       }
       // the tile's sums: out, or into this block's part
       const bool any = n > n0;
       if (any) {
-        wait(&sm.ofull[x][1], (n - 1) & 1);
+        wait(&sm.ofull[x], (n - 1) & 1);
         tmem_fence_after();
       }
       const Segment sg = job.sg;
