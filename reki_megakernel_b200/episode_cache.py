@@ -20,6 +20,7 @@ graph. There is no CPU fallback: the CUDA library must load.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 import threading
 from typing import NamedTuple
@@ -46,8 +47,13 @@ class RowPlan(NamedTuple):
     marks: torch.Tensor
 
 
-# A call on a few rows is over on the GPU in a few microseconds: the checks below build their messages only when they
-# refuse, and read each property of a tensor once.
+# A call on a few rows is over on the GPU in a few microseconds, and a property of a tensor costs a tenth of one: the
+# checks read each once, and build their messages only when they refuse.
+_pack_plan = _lib.packer(_lib.PlanInputs)
+_pack_rotary = _lib.packer(_lib.Rotary)
+_pack_store = _lib.packer(_lib.StoreInputs)
+_NO_ROTARY = (0.0,) + (0,) * 6
+_pack_attend = _lib.packer(_lib.AttendInputs)
 
 def _vector(t, name: str, n: int, dtype, device) -> None:
     if t.dtype != dtype or t.shape != (n,) or t.device != device or not t.is_contiguous():
@@ -74,15 +80,23 @@ def _stream(device) -> int:
 
 
 def _strides(t: torch.Tensor, name: str):
-    """Strides of the leading dims, in elements; dims must be contiguous, the others multiples of 8 elements (16 bytes)
-    and the start 16-byte aligned. A dim of size one has no stride of its own."""
-    st, shape = t.stride(), t.shape
-    if shape[-1] > 1 and st[-1] != 1:
-        raise ValueError(f"{name}: the last dim must be contiguous")
-    out = [s if n > 1 else shape[-1] for s, n in zip(st[:-1], shape[:-1])]
-    if t.data_ptr() % 16 or any(s % 8 or s < 0 for s in out):
+    """Address and strides of the leading dims, in elements; dims must be contiguous, the others multiples of 8 elements
+    (16 bytes) and the start 16-byte aligned. A dim of size one has no stride of its own."""
+    at, shape = t.data_ptr(), t.shape
+    if t.is_contiguous():  # (then the last dim alone decides: the callers see to its size)
+        out, step = [], 1
+        for n in shape[:0:-1]:
+            step *= n
+            out.append(step)
+        out.reverse()
+    else:
+        st = t.stride()
+        if shape[-1] > 1 and st[-1] != 1:
+            raise ValueError(f"{name}: the last dim must be contiguous")
+        out = [s if n > 1 else shape[-1] for s, n in zip(st[:-1], shape[:-1])]
+    if at & 15 or any(s & 7 for s in out):
         raise ValueError(f"{name}: rows, heads and pages must start on 16-byte boundaries")
-    return out
+    return at, out
 
 
 # ---- placing ----------------------------------------------------------------------------------------
@@ -128,30 +142,36 @@ def plan_rows(length: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free
                             ("position", rows, torch.int32), ("length", B, torch.int32), ("marks", 3, torch.int64)):
             _vector(getattr(out, name), f"out.{name}", n, dt, dev)
     if ticket is None:
-        in_place = out.length.data_ptr() == length.data_ptr() or out.marks.data_ptr() == marks.data_ptr()
-        if in_place:
+        if out.length.data_ptr() == length.data_ptr() or out.marks.data_ptr() == marks.data_ptr():
             raise ValueError("advancing length or marks in place needs a ticket")
     else:
         _vector(ticket, "ticket", 1, torch.int32, dev)
-    a = _lib.PlanInputs(length.data_ptr(), new.data_ptr(), table.data_ptr(), free.data_ptr(), marks.data_ptr(),
-                        out.start.data_ptr(), out.slot.data_ptr(), out.episode.data_ptr(), out.position.data_ptr(),
-                        out.length.data_ptr(), out.marks.data_ptr(), ticket.data_ptr() if ticket is not None else None, B,
-                        table.shape[1],
-                        free.shape[0], page_rows, rows)
-    _lib.check(_lib.load().mkx_cache_plan(C.byref(a), dev.index, _stream(dev)), "mkx_cache_plan")
+    st = _lib.load().mkx_cache_plan(
+        _pack_plan(length.data_ptr(), new.data_ptr(), table.data_ptr(), free.data_ptr(), marks.data_ptr(),
+                   out.start.data_ptr(), out.slot.data_ptr(), out.episode.data_ptr(), out.position.data_ptr(),
+                   out.length.data_ptr(), out.marks.data_ptr(), ticket.data_ptr() if ticket is not None else 0, B,
+                   table.shape[1], free.shape[0], page_rows, rows), dev.index, _stream(dev))
+    if st:
+        _lib.check(st, "mkx_cache_plan")
     return out
 
 
 # ---- rotary positions and storing -------------------------------------------------------------------
 
-def _rotary(head_dim: int, sections, base: float, interleaved: bool) -> _lib.Rotary:
-    sections = tuple(sections) if sections is not None else (head_dim // 2,)
+@functools.lru_cache(maxsize=64)
+def _rotary(head_dim: int, sections, base: float, interleaved: bool) -> tuple:
+    """The fields of ``mkx_rotary``."""
+    sections = sections if sections is not None else (head_dim // 2,)
     half = sum(sections)
     if not 1 <= len(sections) <= 4 or min(sections) < 0 or half < 8 or half % 8 or 2 * half > head_dim:
         raise ValueError(f"sections must be 1 to 4 counts whose sum is a multiple of 8 up to {head_dim // 2}")
     if not (base > 0 and math.isfinite(base)):
         raise ValueError("base must be positive")
-    return _lib.Rotary(base, len(sections), (C.c_int * 4)(*sections), int(interleaved))
+    return (float(base), len(sections), *sections, *(0,) * (4 - len(sections)), int(interleaved))
+
+
+def _sections(sections):
+    return sections if sections is None or type(sections) is tuple else tuple(sections)
 
 
 def _positions(positions: torch.Tensor, axes: int, rows: int, device) -> torch.Tensor:
@@ -171,12 +191,12 @@ def rope_tables(positions: torch.Tensor, head_dim: int, *, sections=None, base: 
     dev = _cuda(positions, "positions")
     if not 16 <= head_dim <= 256 or head_dim % 16:
         raise ValueError("head_dim must be a multiple of 16 up to 256")
-    rot = _rotary(head_dim, sections, base, interleaved)
+    rot = _rotary(head_dim, _sections(sections), base, interleaved)
     rows = positions.shape[-1]
-    positions = _positions(positions, rot.axes, rows, dev)
+    positions = _positions(positions, rot[1], rows, dev)
     cos = torch.empty((rows, head_dim), dtype=torch.float32, device=dev)
     sin = torch.empty_like(cos)
-    _lib.check(_lib.load().mkx_rope_tables(C.byref(rot), positions.data_ptr(), positions.stride(0), rows, head_dim,
+    _lib.check(_lib.load().mkx_rope_tables(_pack_rotary(*rot), positions.data_ptr(), positions.stride(0), rows, head_dim,
                                            cos.data_ptr(), sin.data_ptr(), dev.index, _stream(dev)), "mkx_rope_tables")
     return cos, sin
 
@@ -227,26 +247,29 @@ def write_rows(k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, k_pages: to
     dev = _cuda(k, "k")
     check_write_args(k, v, slot, k_pages, v_pages, q, positions, out)
     rows, kv_heads, hd = k.shape
-    a = _lib.StoreInputs()
+    rot, at, axis = _NO_ROTARY, 0, 0
     if positions is not None:
-        a.rot = rot = _rotary(hd, sections, base, interleaved)
-        positions = _positions(positions, rot.axes, rows, dev)
-        a.positions, a.pos_stride = positions.data_ptr(), positions.stride(0)
+        rot = _rotary(hd, _sections(sections), base, interleaved)
+        positions = _positions(positions, rot[1], rows, dev)
+        at, axis = positions.data_ptr(), positions.stride(0)
+    heads = qp = op = 0
+    qs = os = (0, 0)
     if q is not None:
         if out is None:
             out = torch.empty_like(q)
-        a.q, a.q_out, a.heads = q.data_ptr(), out.data_ptr(), q.shape[1]
-        a.q_row, a.q_head = _strides(q, "q")
-        a.qo_row, a.qo_head = _strides(out, "out")
-    a.k, a.v, a.slot = k.data_ptr(), v.data_ptr(), slot.data_ptr()
-    a.k_pages, a.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
-    a.k_row, a.k_head = _strides(k, "k")
-    a.v_row, a.v_head = _strides(v, "v")
-    a.kp_page, a.kp_row, a.kp_head = _strides(k_pages, "k_pages")
-    a.vp_page, a.vp_row, a.vp_head = _strides(v_pages, "v_pages")
-    a.rows, a.kv_heads, a.head_dim, a.dtype = rows, kv_heads, hd, DTYPES[k.dtype]
-    a.pages, a.page_rows = k_pages.shape[0], k_pages.shape[1]
-    _lib.check(_lib.load().mkx_cache_store(C.byref(a), dev.index, _stream(dev)), "mkx_cache_store")
+        heads = q.shape[1]
+        qp, qs = _strides(q, "q")
+        op, os = _strides(out, "out")
+    kp, ks = _strides(k, "k")
+    vp, vs = _strides(v, "v")
+    kpp, kps = _strides(k_pages, "k_pages")
+    vpp, vps = _strides(v_pages, "v_pages")
+    pages, page_rows = k_pages.shape[:2]
+    st = _lib.load().mkx_cache_store(
+        _pack_store(qp, kp, vp, op, kpp, vpp, slot.data_ptr(), at, axis, *qs, *ks, *vs, *os, *kps, *vps, rows, heads,
+                    kv_heads, hd, DTYPES[k.dtype], pages, page_rows, *rot), dev.index, _stream(dev))
+    if st:
+        _lib.check(st, "mkx_cache_store")
     return out
 
 
@@ -254,20 +277,8 @@ def write_rows(k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, k_pages: to
 
 _TICKET_BYTES = 4096 * 4
 _lock = threading.Lock()
-_spaces: dict = {}   # (device index, stream) -> workspace of eager calls, which that stream keeps in order
-_errors: dict = {}   # device index -> error word, shared by all calls (it is only ever set)
-
-
-def _error_word(device) -> torch.Tensor:
-    with _lock:
-        t = _errors.get(device.index)
-        if t is None:
-            # not from a graph's pool, and zero before any stream can use it
-            if _capturing(device):
-                raise RuntimeError("call attend once before its first capture")
-            t = _errors[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
-            torch.cuda.synchronize(device)
-    return t
+_spaces: dict = {}   # (device index, stream) -> (workspace of eager calls, which that stream keeps in order; address)
+_errors: dict = {}   # device index -> (error word, shared by all calls: it is only ever set; address)
 
 
 def _capturing(device) -> bool:
@@ -277,21 +288,52 @@ def _capturing(device) -> bool:
         return torch._C._cuda_isCurrentStreamCapturing()
 
 
-def _workspace(device, stream: int, size: int) -> torch.Tensor:
-    """``size`` bytes whose first words are zero between calls. Eager calls of one stream share one (the stream keeps
-    them in order); a captured call gets its own out of the graph's pool, zeroed by the graph, so that two graphs may
-    be replayed at once."""
-    if _capturing(device):
-        t = torch.empty(size, dtype=torch.uint8, device=device)
-        t[:_TICKET_BYTES].zero_()
-        return t
-    with _lock:
-        t = _spaces.get((device.index, stream))
-        if t is None or t.numel() < size:
-            t = torch.empty(size, dtype=torch.uint8, device=device)
-            t[:_TICKET_BYTES].zero_()
-            _spaces[device.index, stream] = t
+def _error_word(device) -> int:
+    e = _errors.get(device.index)
+    if e is None:
+        with _lock:
+            e = _errors.get(device.index)
+            if e is None:
+                # not from a graph's pool, and zero before any stream can use it
+                if _capturing(device):
+                    raise RuntimeError("call attend once before its first capture")
+                t = torch.zeros(1, dtype=torch.int32, device=device)
+                torch.cuda.synchronize(device)
+                e = _errors[device.index] = (t, t.data_ptr())
+    return e[1]
+
+
+def _new_space(device, size: int) -> torch.Tensor:
+    t = torch.empty(size, dtype=torch.uint8, device=device)
+    t[:_TICKET_BYTES].zero_()
     return t
+
+
+@functools.lru_cache(maxsize=None)
+def _largest_space(index: int) -> int:
+    """Bytes of workspace that no call on this device exceeds: the tiles of the largest heads in either kernel."""
+    lib = _lib.load()
+    sizes = [lib.mkx_attend_workspace(_pack_attend(*(0,) * 19, n, 1, 1, 1, hd, 0, 1, 16, 1, n, 1, 0, 0, 1.0), index)
+             for hd in HEAD_DIMS for n in (1, 1024)]
+    return max(sizes + [_TICKET_BYTES])
+
+
+def _workspace(device, stream: int):
+    """(address, bytes, owner) of a workspace whose first words are zero between calls. Eager calls of one stream share
+    one, which the stream keeps in order; a captured call gets its own out of the graph's pool, zeroed by the graph, so that
+    two graphs may be replayed at once."""
+    size = _largest_space(device.index)
+    if _capturing(device):
+        t = _new_space(device, size)
+        return t.data_ptr(), size, t
+    s = _spaces.get((device.index, stream))
+    if s is None:
+        with _lock:
+            s = _spaces.get((device.index, stream))
+            if s is None:
+                t = _new_space(device, size)
+                s = _spaces[device.index, stream] = (t.data_ptr(), size, t)
+    return s
 
 
 def check_attend_args(q, k_pages, v_pages, table, length, start, max_rows, causal, window, sinks, scale, out) -> None:
@@ -349,25 +391,30 @@ def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table:
         out = torch.empty_like(q)
     if rows == 0:
         return out
-    lib, stream = _lib.load(), _stream(dev)
-    big = (1 << 31) - 1
-    a = _lib.AttendInputs(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), table.data_ptr(), length.data_ptr(),
-        start.data_ptr(), 0, _error_word(dev).data_ptr(), *_strides(q, "q"), *_strides(out, "out"),
-        *_strides(k_pages, "k_pages"), *_strides(v_pages, "v_pages"), rows, length.shape[0], heads, k_pages.shape[2], hd,
-        DTYPES[q.dtype], k_pages.shape[0], k_pages.shape[1], table.shape[1], rows if max_rows is None else min(max_rows, rows),
-        int(causal), min(window, big), min(sinks, big), 1.0 / math.sqrt(hd) if scale is None else scale)
-    space = _workspace(dev, stream, max(lib.mkx_attend_workspace(C.byref(a), dev.index), _TICKET_BYTES))
-    a.workspace = space.data_ptr()
-    _lib.check(lib.mkx_cache_attend(C.byref(a), space.numel(), dev.index, stream), "mkx_cache_attend")
+    stream = _stream(dev)
+    qp, qs = _strides(q, "q")
+    op, os = _strides(out, "out")
+    kp, ks = _strides(k_pages, "k_pages")
+    vp, vs = _strides(v_pages, "v_pages")
+    pages, page_rows, kv_heads = k_pages.shape[:3]
+    error = _error_word(dev)
+    space, size, owner = _workspace(dev, stream)
+    st = _lib.load().mkx_cache_attend(
+        _pack_attend(qp, kp, vp, op, table.data_ptr(), length.data_ptr(), start.data_ptr(), space, error, *qs, *os, *ks, *vs,
+                     rows, length.shape[0], heads, kv_heads, hd, DTYPES[q.dtype], pages, page_rows, table.shape[1],
+                     rows if max_rows is None or max_rows > rows else max_rows, 1 if causal else 0,
+                     window if window < MAX_ROWS else MAX_ROWS, sinks if sinks < MAX_ROWS else MAX_ROWS,
+                     1.0 / math.sqrt(hd) if scale is None else scale), size, dev.index, stream)
+    if st:
+        _lib.check(st, "mkx_cache_attend")
     return out
 
 
 def check_device_error(device=None) -> None:
     """Raises if a bounded wait of an ``attend`` on ``device`` ran out since the last check (synchronises)."""
     index = torch.device("cuda", torch.cuda.current_device()).index if device is None else torch.device(device).index or 0
-    word = _errors.get(index)
-    if word is not None:
+    if index in _errors:
+        word = _errors[index][0]
         code = int(word.item())
         if code:
             word.zero_()

@@ -39,6 +39,31 @@ def test_struct_layout_matches_c(struct, cls, tmp_path):
     assert C.sizeof(ct) == int(c["sizeof"])
 
 
+def test_packed_structs_match_ctypes():
+    from reki_megakernel_b200 import _lib
+    for cls in (_lib.Rotary, _lib.PlanInputs, _lib.StoreInputs, _lib.AttendInputs):
+        flat, want = [], cls()
+        n = 1
+
+        def fill(obj, n):
+            for name, kind in obj._fields_:
+                if issubclass(kind, C.Structure):
+                    n = fill(getattr(obj, name), n)
+                elif kind is C.c_int * 4:
+                    for i in range(4):
+                        getattr(obj, name)[i] = n
+                        flat.append(n)
+                        n += 1
+                else:
+                    setattr(obj, name, n)
+                    flat.append(n)
+                    n += 1
+            return n
+
+        fill(want, n)
+        assert _lib.packer(cls)(*flat) == bytes(want), cls
+
+
 def test_ticket_bytes_match_the_header():
     from reki_megakernel_b200 import episode_cache as E
     text = (ROOT / "include" / "mkx_cache.h").read_text()
@@ -181,8 +206,10 @@ def test_wrappers_refuse_the_cpu_and_odd_strides():
     with pytest.raises(ValueError):
         E.rope_tables(torch.zeros(4, dtype=I32), 64)
     x = torch.zeros(4, 2, 64, dtype=BF)
-    assert E._strides(x, "x") == [128, 64]
-    assert E._strides(torch.zeros(1, 2, 64, dtype=BF), "x") == [64, 64]
+    assert E._strides(x, "x") == (x.data_ptr(), [128, 64])
+    assert E._strides(x[:, 1:], "x")[1] == [128, 64]
+    assert E._strides(torch.zeros(8, 2, 72, dtype=BF)[::2, :1, :64], "x")[1] == [288, 64]
+    assert E._strides(torch.zeros(2, 3, 4, 64, dtype=BF).transpose(1, 2), "x")[1] == [768, 64, 256]
     for bad in (torch.zeros(4, 2, 65, dtype=BF)[:, :, :64], torch.zeros(4, 2, 72, dtype=BF)[:, :, 1:65], torch.zeros(4, 64, 2, dtype=BF).transpose(1, 2)):
         with pytest.raises(ValueError):
             E._strides(bad, "x")
