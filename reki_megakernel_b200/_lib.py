@@ -7,6 +7,7 @@ library is missing or does not load, importing this module raises.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import struct
 from pathlib import Path
 
@@ -99,16 +100,9 @@ class AttendInputs(C.Structure):
                                "table_width", "max_rows", "causal", "window", "sinks")] + [("scale", C.c_float)]
 
 
-def packer(cls):
-    """The struct ``cls`` as bytes from its fields' values, in order: a tenth of a microsecond per field less than a
-    ctypes object. Nested structs and arrays are spelled out."""
-    codes = {C.c_void_p: "P", C.c_longlong: "q", C.c_int: "i", C.c_float: "f", C.c_double: "d", C.c_int * 4: "4i"}
-
-    def of(c):
-        return "".join(of(f[1]) if issubclass(f[1], C.Structure) else codes[f[1]] for f in c._fields_)
-
-    tail = "0d" if any(f[1] is C.c_double for f in cls._fields_) else "0P"  # padded like the C struct
-    return struct.Struct("@" + of(cls) + tail).pack
+def pack_rotary(base: float, axes: int, s0: int, s1: int, s2: int, s3: int, interleaved: int) -> bytes:
+    """``mkx_rotary`` as bytes."""
+    return struct.pack("@d6i0d", base, axes, s0, s1, s2, s3, interleaved)
 
 
 SIGNATURES = {
@@ -144,7 +138,7 @@ SIGNATURES = {
     "mkx_mods_input": (C.c_int, [P, P, P]),
     "mkx_mods_last_error": (C.c_int, [P, C.POINTER(C.c_int)]),
     "mkx_mods_destroy": (None, [P]),
-    # the inputs of the cache's entry points come as the bytes of the struct (packer) or by reference
+    # structs of the cache's entry points come by reference or as bytes
     "mkx_cache_plan": (C.c_int, [P, C.c_int, P]),
     "mkx_cache_release": (C.c_int, [P, C.c_int, P]),
     "mkx_rope_tables": (C.c_int, [P, P, C.c_longlong, C.c_int, C.c_int, P, P, C.c_int, P]),
@@ -195,6 +189,30 @@ def load(build_if_missing: bool = True) -> C.CDLL:
         fn.argtypes = args
     _LIB = lib
     return lib
+
+
+_TORCH = None
+
+
+def load_torch():
+    """The torch binding of the episode cache (``_mkx_torch.so``, built first if missing or stale), bound to the library
+    that ``load`` loads. There is no fallback."""
+    global _TORCH
+    if _TORCH is None:
+        path = _build.TORCH_LIB
+        try:
+            _build.build_torch()
+        except RuntimeError:
+            if not path.exists():
+                raise
+        spec = importlib.util.spec_from_file_location("_mkx_torch", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        lib = load()
+        module.bind(*(C.cast(getattr(lib, n), C.c_void_p).value
+                      for n in ("mkx_cache_plan", "mkx_cache_store", "mkx_cache_attend", "mkx_attend_workspace")))
+        _TORCH = module
+    return _TORCH
 
 
 class MkxError(RuntimeError):

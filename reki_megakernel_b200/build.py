@@ -1,4 +1,4 @@
-"""Build recipe for the in-tree CUDA library ``libmkx.so`` (sm_100a only).
+"""Build recipe for the in-tree CUDA library ``libmkx.so`` (sm_100a only) and its torch binding ``_mkx_torch.so``.
 
     python -m reki_megakernel_b200.build             # libmkx.so
     python -m reki_megakernel_b200.build --traced    # libmkx_trace.so (profiling variant)
@@ -8,10 +8,12 @@ source tree and is the one ``reki_megakernel_b200._lib`` loads.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -27,6 +29,9 @@ HEADERS = [PKG / "csrc" / "mkx_device.cuh", PKG / "csrc" / "mkx_tma.cuh", PKG / 
            PKG / "csrc" / "mkx_attend.cuh", PKG / "csrc" / "mkx_cache_host.h", ROOT / "include" / "mkx.h",
            ROOT / "include" / "mkx_prepare.h", ROOT / "include" / "mkx_mods.h", ROOT / "include" / "mkx_batch.h",
            ROOT / "include" / "mkx_cache.h"]
+# The episode cache's entry points for torch tensors (host code; reaches libmkx.so by address).
+TORCH_LIB = PKG / "_mkx_torch.so"
+TORCH_SOURCES = [PKG / "csrc" / "mk_torch.cpp", ROOT / "include" / "mkx.h", ROOT / "include" / "mkx_cache.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -42,7 +47,7 @@ def stale(lib: Path | None = None) -> bool:
     if not lib.exists():
         return True
     t = lib.stat().st_mtime
-    return any(p.stat().st_mtime > t for p in SOURCES + HEADERS)
+    return any(p.stat().st_mtime > t for p in (TORCH_SOURCES if lib == TORCH_LIB else SOURCES + HEADERS))
 
 
 def build(force: bool = False, verbose: bool = False, traced: bool = False) -> Path:
@@ -64,5 +69,27 @@ def build(force: bool = False, verbose: bool = False, traced: bool = False) -> P
     return lib
 
 
+def build_torch(force: bool = False) -> Path:
+    """Compiles the torch binding with the host compiler against the headers of the installed torch."""
+    if not force and not stale(TORCH_LIB):
+        return TORCH_LIB
+    gxx = shutil.which("g++")
+    spec = importlib.util.find_spec("torch")
+    if gxx is None or spec is None:
+        raise RuntimeError("g++ and torch are required to build _mkx_torch.so")
+    torch = Path(spec.submodule_search_locations[0])
+    cuda = Path(nvcc()).resolve().parents[1]
+    tmp = TORCH_LIB.with_suffix(f".so.tmp{os.getpid()}")
+    cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-I", str(torch / "include"), "-I", sysconfig.get_paths()["include"],
+           "-I", str(cuda / "include"), "-I", str(ROOT / "include"), "-o", str(tmp), str(TORCH_SOURCES[0]),
+           "-L", str(torch / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_LIB)
+    return TORCH_LIB
+
+
 if __name__ == "__main__":
+    print(build_torch(force="--force" in sys.argv))
     print(build(force="--force" in sys.argv, verbose="-v" in sys.argv, traced="--traced" in sys.argv))

@@ -22,7 +22,6 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
-import threading
 from typing import NamedTuple
 
 import torch
@@ -47,13 +46,8 @@ class RowPlan(NamedTuple):
     marks: torch.Tensor
 
 
-# A call on a few rows is over on the GPU in a few microseconds, and a property of a tensor costs a tenth of one: the
-# checks read each once, and build their messages only when they refuse.
-_pack_plan = _lib.packer(_lib.PlanInputs)
-_pack_rotary = _lib.packer(_lib.Rotary)
-_pack_store = _lib.packer(_lib.StoreInputs)
-_NO_ROTARY = (0.0,) + (0,) * 6
-_pack_attend = _lib.packer(_lib.AttendInputs)
+# Calls go through ``_mkx_torch`` (csrc/mk_torch.cpp), which checks, allocates and launches in one step and answers None
+# to arguments it does not accept; the checks below then say what is wrong.
 
 def _vector(t, name: str, n: int, dtype, device) -> None:
     if t.dtype != dtype or t.shape != (n,) or t.device != device or not t.is_contiguous():
@@ -76,27 +70,19 @@ def _cuda(t: torch.Tensor, name: str) -> torch.device:
 
 
 def _stream(device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)  # torch.cuda.current_stream builds an object: 2 us
+    return torch.cuda.current_stream(device).cuda_stream
 
 
-def _strides(t: torch.Tensor, name: str):
-    """Address and strides of the leading dims, in elements; dims must be contiguous, the others multiples of 8 elements
-    (16 bytes) and the start 16-byte aligned. A dim of size one has no stride of its own."""
-    at, shape = t.data_ptr(), t.shape
-    if t.is_contiguous():  # (then the last dim alone decides: the callers see to its size)
-        out, step = [], 1
-        for n in shape[:0:-1]:
-            step *= n
-            out.append(step)
-        out.reverse()
-    else:
-        st = t.stride()
-        if shape[-1] > 1 and st[-1] != 1:
-            raise ValueError(f"{name}: the last dim must be contiguous")
-        out = [s if n > 1 else shape[-1] for s, n in zip(st[:-1], shape[:-1])]
-    if at & 15 or any(s & 7 for s in out):
+def _check_strides(t: torch.Tensor, name: str) -> None:
+    """Dims must be contiguous, rows, heads and pages 16 bytes apart or a multiple, and the start 16-byte aligned."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last dim must be contiguous")
+    if t.data_ptr() % 16 or any(s % 8 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
         raise ValueError(f"{name}: rows, heads and pages must start on 16-byte boundaries")
-    return at, out
+
+
+def _refused(what: str):
+    return ValueError(f"{what}: these arguments are not supported")
 
 
 # ---- placing ----------------------------------------------------------------------------------------
@@ -118,56 +104,39 @@ def check_plan_args(length, new, table, free, marks, page_rows: int, rows: int) 
 
 
 def plan_rows(length: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free: torch.Tensor, marks: torch.Tensor, *,
-              page_rows: int, rows: int, out: RowPlan | None = None, ticket: torch.Tensor | None = None) -> RowPlan:
+              page_rows: int, rows: int, ticket: torch.Tensor | None = None) -> RowPlan:
     """Places ``new[b]`` rows behind the ``length[b]`` rows that episode b holds: pages off the ring ``free``, their
     table entries (``table`` [B, pages] int32, written in place), and the new rows' start, slot, episode and position.
 
     ``marks`` [3] int64: pages ever taken, pages ever returned (their difference is free, the next at
     ``free[taken % len(free)]``), and, in the returned marks, the new rows that got no slot. ``rows``: how many rows
     the step has room for; rows behind the last new one get slot -1. The returned length and marks are the state after
-    the step; ``out`` may name the arguments themselves (``out.length is length``) to advance them in place, then
-    ``ticket`` ([1] int32, zero) has to be a word that only plans of this state use."""
-    dev = _cuda(length, "length")
-    check_plan_args(length, new, table, free, marks, page_rows, rows)
-    B = length.shape[0]
-    if out is None:
-        # one allocation: slot, marks, position, episode, each on a 16-byte boundary, then length and start
-        pad = -rows % 4
-        slot, _, m, _, position, _, episode, _, after, start = torch.empty(
-            4 * (rows + pad) + 8 + 2 * B + 1, dtype=torch.int32, device=dev).split_with_sizes(
-                [2 * rows, 2 * pad, 6, 2, rows, pad, rows, pad, B, B + 1])
-        out = RowPlan(start, slot.view(torch.int64), episode, position, after, m.view(torch.int64))
-    else:
-        for name, n, dt in (("start", B + 1, torch.int32), ("slot", rows, torch.int64), ("episode", rows, torch.int32),
-                            ("position", rows, torch.int32), ("length", B, torch.int32), ("marks", 3, torch.int64)):
-            _vector(getattr(out, name), f"out.{name}", n, dt, dev)
-    if ticket is None:
-        if out.length.data_ptr() == length.data_ptr() or out.marks.data_ptr() == marks.data_ptr():
-            raise ValueError("advancing length or marks in place needs a ticket")
-    else:
-        _vector(ticket, "ticket", 1, torch.int32, dev)
-    st = _lib.load().mkx_cache_plan(
-        _pack_plan(length.data_ptr(), new.data_ptr(), table.data_ptr(), free.data_ptr(), marks.data_ptr(),
-                   out.start.data_ptr(), out.slot.data_ptr(), out.episode.data_ptr(), out.position.data_ptr(),
-                   out.length.data_ptr(), out.marks.data_ptr(), ticket.data_ptr() if ticket is not None else 0, B,
-                   table.shape[1], free.shape[0], page_rows, rows), dev.index, _stream(dev))
-    if st:
-        _lib.check(st, "mkx_cache_plan")
-    return out
+    the step: new tensors, or, with a ``ticket`` ([1] int32, zero, a word that only plans of this state use), the
+    arguments themselves, advanced in place."""
+    r = _lib.load_torch().plan(length, new, table, free, marks, page_rows, rows, ticket)
+    if type(r) is tuple:
+        return RowPlan(*r)
+    if r is None:
+        _cuda(length, "length")
+        check_plan_args(length, new, table, free, marks, page_rows, rows)
+        if ticket is not None:
+            _vector(ticket, "ticket", 1, torch.int32, length.device)
+        raise _refused("plan_rows")
+    _lib.check(r, "mkx_cache_plan")
 
 
 # ---- rotary positions and storing -------------------------------------------------------------------
 
 @functools.lru_cache(maxsize=64)
-def _rotary(head_dim: int, sections, base: float, interleaved: bool) -> tuple:
-    """The fields of ``mkx_rotary``."""
+def _rotary(head_dim: int, sections, base: float, interleaved: bool):
+    """(the struct ``mkx_rotary`` as bytes, number of axes)."""
     sections = sections if sections is not None else (head_dim // 2,)
     half = sum(sections)
     if not 1 <= len(sections) <= 4 or min(sections) < 0 or half < 8 or half % 8 or 2 * half > head_dim:
         raise ValueError(f"sections must be 1 to 4 counts whose sum is a multiple of 8 up to {head_dim // 2}")
     if not (base > 0 and math.isfinite(base)):
         raise ValueError("base must be positive")
-    return (float(base), len(sections), *sections, *(0,) * (4 - len(sections)), int(interleaved))
+    return _lib.pack_rotary(base, len(sections), *sections, *(0,) * (4 - len(sections)), int(interleaved)), len(sections)
 
 
 def _sections(sections):
@@ -191,12 +160,12 @@ def rope_tables(positions: torch.Tensor, head_dim: int, *, sections=None, base: 
     dev = _cuda(positions, "positions")
     if not 16 <= head_dim <= 256 or head_dim % 16:
         raise ValueError("head_dim must be a multiple of 16 up to 256")
-    rot = _rotary(head_dim, _sections(sections), base, interleaved)
+    rot, axes = _rotary(head_dim, _sections(sections), base, interleaved)
     rows = positions.shape[-1]
-    positions = _positions(positions, rot[1], rows, dev)
+    positions = _positions(positions, axes, rows, dev)
     cos = torch.empty((rows, head_dim), dtype=torch.float32, device=dev)
     sin = torch.empty_like(cos)
-    _lib.check(_lib.load().mkx_rope_tables(_pack_rotary(*rot), positions.data_ptr(), positions.stride(0), rows, head_dim,
+    _lib.check(_lib.load().mkx_rope_tables(rot, positions.data_ptr(), positions.stride(0), rows, head_dim,
                                            cos.data_ptr(), sin.data_ptr(), dev.index, _stream(dev)), "mkx_rope_tables")
     return cos, sin
 
@@ -244,97 +213,25 @@ def write_rows(k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, k_pages: to
     ``sections``: frequencies per axis (default: one axis with head_dim / 2); axis(i) goes through them one axis after
     the other, or, ``interleaved``, over the axes in turn while each has some left. Tensors may be slices: dims
     contiguous, rows, heads and pages on 16-byte boundaries."""
-    dev = _cuda(k, "k")
-    check_write_args(k, v, slot, k_pages, v_pages, q, positions, out)
-    rows, kv_heads, hd = k.shape
-    rot, at, axis = _NO_ROTARY, 0, 0
+    rot = None
     if positions is not None:
-        rot = _rotary(hd, _sections(sections), base, interleaved)
-        positions = _positions(positions, rot[1], rows, dev)
-        at, axis = positions.data_ptr(), positions.stride(0)
-    heads = qp = op = 0
-    qs = os = (0, 0)
-    if q is not None:
-        if out is None:
-            out = torch.empty_like(q)
-        heads = q.shape[1]
-        qp, qs = _strides(q, "q")
-        op, os = _strides(out, "out")
-    kp, ks = _strides(k, "k")
-    vp, vs = _strides(v, "v")
-    kpp, kps = _strides(k_pages, "k_pages")
-    vpp, vps = _strides(v_pages, "v_pages")
-    pages, page_rows = k_pages.shape[:2]
-    st = _lib.load().mkx_cache_store(
-        _pack_store(qp, kp, vp, op, kpp, vpp, slot.data_ptr(), at, axis, *qs, *ks, *vs, *os, *kps, *vps, rows, heads,
-                    kv_heads, hd, DTYPES[k.dtype], pages, page_rows, *rot), dev.index, _stream(dev))
-    if st:
-        _lib.check(st, "mkx_cache_store")
-    return out
+        rot, axes = _rotary(k.shape[-1], _sections(sections), base, interleaved)
+    r = _lib.load_torch().store(k, v, slot, k_pages, v_pages, q, positions, rot, out)
+    if r is None:
+        _cuda(k, "k")
+        check_write_args(k, v, slot, k_pages, v_pages, q, positions, out)
+        if positions is not None:
+            _positions(positions, axes, k.shape[0], k.device)
+        for name, t in (("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages), ("q", q), ("out", out)):
+            if t is not None:
+                _check_strides(t, name)
+        raise _refused("write_rows")
+    if type(r) is int:
+        _lib.check(r, "mkx_cache_store")
+    return None if r is True else r
 
 
 # ---- attention ----------------------------------------------------------------------------------------
-
-_TICKET_BYTES = 4096 * 4
-_lock = threading.Lock()
-_spaces: dict = {}   # (device index, stream) -> (workspace of eager calls, which that stream keeps in order; address)
-_errors: dict = {}   # device index -> (error word, shared by all calls: it is only ever set; address)
-
-
-def _capturing(device) -> bool:
-    if torch._C._cuda_getDevice() == device.index:
-        return torch._C._cuda_isCurrentStreamCapturing()
-    with torch.cuda.device(device):
-        return torch._C._cuda_isCurrentStreamCapturing()
-
-
-def _error_word(device) -> int:
-    e = _errors.get(device.index)
-    if e is None:
-        with _lock:
-            e = _errors.get(device.index)
-            if e is None:
-                # not from a graph's pool, and zero before any stream can use it
-                if _capturing(device):
-                    raise RuntimeError("call attend once before its first capture")
-                t = torch.zeros(1, dtype=torch.int32, device=device)
-                torch.cuda.synchronize(device)
-                e = _errors[device.index] = (t, t.data_ptr())
-    return e[1]
-
-
-def _new_space(device, size: int) -> torch.Tensor:
-    t = torch.empty(size, dtype=torch.uint8, device=device)
-    t[:_TICKET_BYTES].zero_()
-    return t
-
-
-@functools.lru_cache(maxsize=None)
-def _largest_space(index: int) -> int:
-    """Bytes of workspace that no call on this device exceeds: the tiles of the largest heads in either kernel."""
-    lib = _lib.load()
-    sizes = [lib.mkx_attend_workspace(_pack_attend(*(0,) * 19, n, 1, 1, 1, hd, 0, 1, 16, 1, n, 1, 0, 0, 1.0), index)
-             for hd in HEAD_DIMS for n in (1, 1024)]
-    return max(sizes + [_TICKET_BYTES])
-
-
-def _workspace(device, stream: int):
-    """(address, bytes, owner) of a workspace whose first words are zero between calls. Eager calls of one stream share
-    one, which the stream keeps in order; a captured call gets its own out of the graph's pool, zeroed by the graph, so that
-    two graphs may be replayed at once."""
-    size = _largest_space(device.index)
-    if _capturing(device):
-        t = _new_space(device, size)
-        return t.data_ptr(), size, t
-    s = _spaces.get((device.index, stream))
-    if s is None:
-        with _lock:
-            s = _spaces.get((device.index, stream))
-            if s is None:
-                t = _new_space(device, size)
-                s = _spaces[device.index, stream] = (t.data_ptr(), size, t)
-    return s
-
 
 def check_attend_args(q, k_pages, v_pages, table, length, start, max_rows, causal, window, sinks, scale, out) -> None:
     """What ``attend`` checks of shapes, types, devices and values. Raises ValueError."""
@@ -384,41 +281,28 @@ def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table:
     episode's length does not matter; the K and V rows below it are finite. ``max_rows``: no episode has more new rows
     (default: q's rows); a tight value picks the kernel that fits. A wait that ran out on the device surfaces in
     ``check_device_error()``."""
-    dev = _cuda(q, "q")
-    check_attend_args(q, k_pages, v_pages, table, length, start, max_rows, causal, window, sinks, scale, out)
-    rows, heads, hd = q.shape
-    if out is None:
-        out = torch.empty_like(q)
-    if rows == 0:
-        return out
-    stream = _stream(dev)
-    qp, qs = _strides(q, "q")
-    op, os = _strides(out, "out")
-    kp, ks = _strides(k_pages, "k_pages")
-    vp, vs = _strides(v_pages, "v_pages")
-    pages, page_rows, kv_heads = k_pages.shape[:3]
-    error = _error_word(dev)
-    space, size, owner = _workspace(dev, stream)
-    st = _lib.load().mkx_cache_attend(
-        _pack_attend(qp, kp, vp, op, table.data_ptr(), length.data_ptr(), start.data_ptr(), space, error, *qs, *os, *ks, *vs,
-                     rows, length.shape[0], heads, kv_heads, hd, DTYPES[q.dtype], pages, page_rows, table.shape[1],
-                     rows if max_rows is None or max_rows > rows else max_rows, 1 if causal else 0,
-                     window if window < MAX_ROWS else MAX_ROWS, sinks if sinks < MAX_ROWS else MAX_ROWS,
-                     1.0 / math.sqrt(hd) if scale is None else scale), size, dev.index, stream)
-    if st:
-        _lib.check(st, "mkx_cache_attend")
-    return out
+    most = -1 if max_rows is None else max_rows if max_rows >= 0 else -2  # -1: q's rows; below: refused
+    r = _lib.load_torch().attend(q, k_pages, v_pages, table, length, start, most, causal, window, sinks, scale, out)
+    if r is None:
+        _cuda(q, "q")
+        check_attend_args(q, k_pages, v_pages, table, length, start, max_rows, causal, window, sinks, scale, out)
+        for name, t in (("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("out", out)):
+            if t is not None:
+                _check_strides(t, name)
+        raise _refused("attend")
+    if r is False:
+        raise RuntimeError("call attend once on this device before its first capture")
+    if type(r) is int:
+        _lib.check(r, "mkx_cache_attend")
+    return r
 
 
 def check_device_error(device=None) -> None:
     """Raises if a bounded wait of an ``attend`` on ``device`` ran out since the last check (synchronises)."""
-    index = torch.device("cuda", torch.cuda.current_device()).index if device is None else torch.device(device).index or 0
-    if index in _errors:
-        word = _errors[index][0]
-        code = int(word.item())
-        if code:
-            word.zero_()
-            raise _lib.MkxError("attend", _lib.MKX_ERR_DEVICE, f"error word {code:#x}")
+    index = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    code = _lib.load_torch().error_code(index, False)
+    if code:
+        raise _lib.MkxError("attend", _lib.MKX_ERR_DEVICE, f"error word {code:#x}")
 
 
 # ---- the cache ------------------------------------------------------------------------------------------
@@ -454,8 +338,7 @@ class EpisodeCache:
         wide = pages if pages_per_episode is None else pages_per_episode
         if wide < 1 or wide * page_rows > MAX_ROWS:
             raise ValueError(f"an episode may hold up to {MAX_ROWS} rows")
-        _lib.load()
-        _error_word(dev)
+        _lib.load_torch().error_code(dev.index, True)  # allocates the device's error word, which a capture could not
         self.device, self.page_rows, self.episodes = dev, page_rows, episodes
         self.k = torch.zeros((layers, pages, page_rows, kv_heads, head_dim), dtype=dtype, device=dev)
         self.v = torch.zeros_like(self.k)
@@ -468,10 +351,7 @@ class EpisodeCache:
     def plan(self, new: torch.Tensor, rows: int) -> RowPlan:
         """Places ``new`` [episodes] int32 rows (device); ``rows`` is the room of the step's row tensors. The plan's
         length and marks are the cache's own. Rows without a slot are counted in ``marks[2]``."""
-        dev, e = self.device, torch.empty
-        out = RowPlan(e(self.episodes + 1, dtype=torch.int32, device=dev), e(rows, dtype=torch.int64, device=dev),
-                      e(rows, dtype=torch.int32, device=dev), e(rows, dtype=torch.int32, device=dev), self.length, self.marks)
-        return plan_rows(self.length, new, self.table, self.free, self.marks, page_rows=self.page_rows, rows=rows, out=out,
+        return plan_rows(self.length, new, self.table, self.free, self.marks, page_rows=self.page_rows, rows=rows,
                          ticket=self._ticket)
 
     def release(self, ended: torch.Tensor) -> None:

@@ -39,36 +39,24 @@ def test_struct_layout_matches_c(struct, cls, tmp_path):
     assert C.sizeof(ct) == int(c["sizeof"])
 
 
-def test_packed_structs_match_ctypes():
+def test_constants_match_the_header():
     from reki_megakernel_b200 import _lib
-    for cls in (_lib.Rotary, _lib.PlanInputs, _lib.StoreInputs, _lib.AttendInputs):
-        flat, want = [], cls()
-        n = 1
-
-        def fill(obj, n):
-            for name, kind in obj._fields_:
-                if issubclass(kind, C.Structure):
-                    n = fill(getattr(obj, name), n)
-                elif kind is C.c_int * 4:
-                    for i in range(4):
-                        getattr(obj, name)[i] = n
-                        flat.append(n)
-                        n += 1
-                else:
-                    setattr(obj, name, n)
-                    flat.append(n)
-                    n += 1
-            return n
-
-        fill(want, n)
-        assert _lib.packer(cls)(*flat) == bytes(want), cls
-
-
-def test_ticket_bytes_match_the_header():
     from reki_megakernel_b200 import episode_cache as E
     text = (ROOT / "include" / "mkx_cache.h").read_text()
-    assert E._TICKET_BYTES == 4 * int(re.search(r"MKX_ATTEND_TICKETS (\d+)", text)[1])
     assert E.MAX_EPISODES == int(re.search(r"MKX_MAX_EPISODES (\d+)", text)[1])
+    want = _lib.Rotary(1e6, 3, (C.c_int * 4)(8, 12, 16, 0), 1)
+    assert _lib.pack_rotary(1e6, 3, 8, 12, 16, 0, 1) == bytes(want)
+
+
+def test_torch_binding_refuses_what_it_does_not_know():
+    """It answers None (the wrappers then say what is wrong), whatever it is given."""
+    from reki_megakernel_b200 import _lib
+    m = _lib.load_torch()
+    x = torch.zeros(3)
+    for f in (m.plan, m.store, m.attend):
+        assert f() is None and f(1, 2, 3) is None
+        for n in (8, 9, 12):
+            assert f(*[x] * n) is None and f(*[None] * n) is None and f(*["a"] * n) is None
 
 
 def test_null_arguments_are_rejected_without_a_device():
@@ -146,73 +134,65 @@ def test_c_attend_refuses(kw):
 
 # ---- the wrappers ---------------------------------------------------------------------------------------
 
-def _plan_args():
-    return dict(length=_t(3, I32), new=_t(3, I32), table=_t((3, 5), I32), free=_t(9, I32), marks=_t(3, I64), page_rows=16, rows=7)
+def plan_args(dev=META):
+    t = lambda shape, dtype, d=dev: torch.zeros(shape, dtype=dtype, device=d)  # noqa: E731
+    good = dict(length=t(3, I32), new=t(3, I32), table=t((3, 5), I32), free=t(9, I32), marks=t(3, I64), page_rows=16, rows=7)
+    bad = [dict(length=t(0, I32)), dict(length=t(5000, I32)), dict(new=t(4, I32)), dict(new=t(3, I64)), dict(table=t((2, 5), I32)),
+           dict(table=t((3, 0), I32)), dict(table=t((5, 3), I32).t()), dict(table=t((3, 5), I64)), dict(free=t(0, I32)), dict(free=t((3, 3), I32)),
+           dict(marks=t(2, I64)), dict(marks=t(3, I32)), dict(page_rows=48), dict(rows=-1), dict(rows=1 << 31), dict(new=t(3, I32, "cpu")),
+           dict(table=t((1, 1), I32).expand(3, (1 << 26) + 1)), dict(length=t((3, 1), I32)), dict(new=t(6, I32)[::2])]
+    return good, bad
 
 
-def test_plan_args():
-    from reki_megakernel_b200.episode_cache import check_plan_args
-    check_plan_args(**_plan_args())
-    bad = [dict(length=_t(0, I32)), dict(length=_t(5000, I32)), dict(new=_t(4, I32)), dict(new=_t(3, I64)), dict(table=_t((2, 5), I32)),
-           dict(table=_t((3, 0), I32)), dict(table=_t((5, 3), I32).t()), dict(table=_t((3, 5), I64)), dict(free=_t(0, I32)), dict(free=_t((3, 3), I32)),
-           dict(marks=_t(2, I64)), dict(marks=_t(3, I32)), dict(page_rows=48), dict(rows=-1), dict(rows=1 << 31),
-           dict(new=_t(3, I32, "cpu")), dict(table=_t((3, (1 << 26) + 1), I32))]
+def write_args(dev=META):
+    t = lambda shape, dtype=BF, d=dev: torch.zeros(shape, dtype=dtype, device=d)  # noqa: E731
+    good = dict(k=t((7, 2, 64)), v=t((7, 2, 64)), slot=t(7, I64), k_pages=t((4, 32, 2, 64)), v_pages=t((4, 32, 2, 64)), q=t((7, 6, 64)),
+                positions=t((1, 7), I32), out=None)
+    bad = [dict(v=t((7, 1, 64))), dict(k=t((7, 2, 72)), v=t((7, 2, 72))), dict(k=t((7, 2, 64), torch.float32)), dict(slot=t(6, I64)),
+           dict(slot=t(7, I32)), dict(k_pages=t((4, 20, 2, 64)), v_pages=t((4, 20, 2, 64))), dict(v_pages=t((4, 32, 3, 64))),
+           dict(k_pages=t((4, 32, 2, 64), torch.float16)), dict(k_pages=t((4, 32, 2, 64), BF, "cpu")), dict(q=t((6, 6, 64))),
+           dict(q=t((7, 6, 32))), dict(q=t((7, 6, 64), torch.float16)), dict(positions=None), dict(out=t((7, 6, 32))),
+           dict(q=None, out=t((7, 6, 64))), dict(k=t((7, 128))), dict(out=t((7, 6, 64), BF, "cpu"))]
+    return good, bad
+
+
+def attend_args(dev=META):
+    t = lambda shape, dtype=BF, d=dev: torch.zeros(shape, dtype=dtype, device=d)  # noqa: E731
+    good = dict(q=t((7, 6, 64)), k_pages=t((4, 32, 2, 64)), v_pages=t((4, 32, 2, 64)), table=t((3, 5), I32), length=t(3, I32), start=t(4, I32),
+                max_rows=None, causal=True, window=8, sinks=2, scale=None, out=None)
+    bad = [dict(q=t((7, 6, 80))), dict(q=t((7, 6, 64), torch.float32)), dict(q=t((7, 5, 64))), dict(k_pages=t((4, 32, 2, 128))),
+           dict(v_pages=t((4, 16, 2, 64))), dict(v_pages=t((4, 32, 2, 64), torch.float16)), dict(table=t((2, 5), I32)),
+           dict(table=t((3, 5), I64)), dict(length=t(3, I64)), dict(start=t(3, I32)), dict(max_rows=-1), dict(max_rows=-2), dict(causal=False),
+           dict(window=-1), dict(window=0), dict(sinks=-2), dict(scale=float("nan")), dict(out=t((7, 6, 128))), dict(out=t((7, 6, 64), BF, "cpu")),
+           dict(k_pages=t((4, 24, 2, 64)), v_pages=t((4, 24, 2, 64))), dict(length=t(0, I32), start=t(1, I32), table=t((0, 5), I32))]
+    return good, bad
+
+
+@pytest.mark.parametrize("name", ["plan", "write", "attend"])
+def test_arguments(name):
+    from reki_megakernel_b200 import episode_cache as E
+    check = getattr(E, f"check_{name}_args")
+    good, bad = globals()[f"{name}_args"]()
+    check(**good)
+    if name == "write":
+        check(**{**good, "q": None, "positions": None})
     for kw in bad:
         with pytest.raises(ValueError):
-            check_plan_args(**{**_plan_args(), **kw})
-
-
-def _write_args():
-    return dict(k=_t((7, 2, 64)), v=_t((7, 2, 64)), slot=_t(7, I64), k_pages=_t((4, 32, 2, 64)), v_pages=_t((4, 32, 2, 64)),
-                q=_t((7, 6, 64)), positions=_t((1, 7), I32), out=None)
-
-
-def test_write_args():
-    from reki_megakernel_b200.episode_cache import check_write_args
-    check_write_args(**_write_args())
-    check_write_args(**{**_write_args(), "q": None, "positions": None})
-    bad = [dict(v=_t((7, 1, 64))), dict(k=_t((7, 2, 72)), v=_t((7, 2, 72))), dict(k=_t((7, 2, 64), torch.float32)), dict(slot=_t(6, I64)),
-           dict(slot=_t(7, I32)), dict(k_pages=_t((4, 20, 2, 64)), v_pages=_t((4, 20, 2, 64))), dict(v_pages=_t((4, 32, 3, 64))),
-           dict(k_pages=_t((4, 32, 2, 64), torch.float16)), dict(k_pages=_t((4, 32, 2, 64), BF, "cpu")), dict(q=_t((6, 6, 64))),
-           dict(q=_t((7, 6, 32))), dict(q=_t((7, 6, 64), torch.float16)), dict(positions=None), dict(out=_t((7, 6, 32))),
-           dict(q=None, out=_t((7, 6, 64)))]
-    for kw in bad:
-        with pytest.raises(ValueError):
-            check_write_args(**{**_write_args(), **kw})
-
-
-def _attend_args():
-    return dict(q=_t((7, 6, 64)), k_pages=_t((4, 32, 2, 64)), v_pages=_t((4, 32, 2, 64)), table=_t((3, 5), I32), length=_t(3, I32),
-                start=_t(4, I32), max_rows=None, causal=True, window=8, sinks=2, scale=None, out=None)
-
-
-def test_attend_args():
-    from reki_megakernel_b200.episode_cache import check_attend_args
-    check_attend_args(**_attend_args())
-    bad = [dict(q=_t((7, 6, 80))), dict(q=_t((7, 6, 64), torch.float32)), dict(q=_t((7, 5, 64))), dict(k_pages=_t((4, 32, 2, 128))),
-           dict(v_pages=_t((4, 16, 2, 64))), dict(v_pages=_t((4, 32, 2, 64), torch.float16)), dict(table=_t((2, 5), I32)),
-           dict(table=_t((3, 5), I64)), dict(length=_t(3, I64)), dict(start=_t(3, I32)), dict(max_rows=-1), dict(causal=False),
-           dict(window=-1), dict(window=0), dict(sinks=-2), dict(scale=float("nan")), dict(out=_t((7, 6, 128))), dict(out=_t((7, 6, 64), BF, "cpu"))]
-    for kw in bad:
-        with pytest.raises(ValueError):
-            check_attend_args(**{**_attend_args(), **kw})
+            check(**{**good, **kw})
 
 
 def test_wrappers_refuse_the_cpu_and_odd_strides():
     from reki_megakernel_b200 import episode_cache as E
-    a = {k: (torch.zeros(v.shape, dtype=v.dtype) if isinstance(v, torch.Tensor) else v) for k, v in _attend_args().items()}
-    with pytest.raises(ValueError):
-        E.attend(**a)
+    for name, f in (("plan", E.plan_rows), ("write", E.write_rows), ("attend", E.attend)):
+        with pytest.raises(ValueError, match="CUDA"):
+            f(**globals()[f"{name}_args"]("cpu")[0])
     with pytest.raises(ValueError):
         E.rope_tables(torch.zeros(4, dtype=I32), 64)
-    x = torch.zeros(4, 2, 64, dtype=BF)
-    assert E._strides(x, "x") == (x.data_ptr(), [128, 64])
-    assert E._strides(x[:, 1:], "x")[1] == [128, 64]
-    assert E._strides(torch.zeros(8, 2, 72, dtype=BF)[::2, :1, :64], "x")[1] == [288, 64]
-    assert E._strides(torch.zeros(2, 3, 4, 64, dtype=BF).transpose(1, 2), "x")[1] == [768, 64, 256]
+    for good in (torch.zeros(4, 2, 64, dtype=BF), torch.zeros(8, 2, 72, dtype=BF)[::2, :1, :64], torch.zeros(2, 3, 4, 64, dtype=BF).transpose(1, 2)):
+        E._check_strides(good, "x")
     for bad in (torch.zeros(4, 2, 65, dtype=BF)[:, :, :64], torch.zeros(4, 2, 72, dtype=BF)[:, :, 1:65], torch.zeros(4, 64, 2, dtype=BF).transpose(1, 2)):
         with pytest.raises(ValueError):
-            E._strides(bad, "x")
+            E._check_strides(bad, "x")
 
 
 # ---- the restatement ------------------------------------------------------------------------------------

@@ -15,6 +15,34 @@ def ec():
     return episode_cache
 
 
+@pytest.mark.parametrize("name", ["plan", "write", "attend"])
+def test_refusals(name):
+    """What the checks refuse is refused by the calls themselves, before anything is launched; the good arguments run."""
+    import test_episode_cache_host as host
+    E = ec()
+    f = {"plan": E.plan_rows, "write": E.write_rows, "attend": E.attend}[name]
+    good, bad = getattr(host, f"{name}_args")(DEV)
+    if name != "plan":
+        wide = torch.zeros(7, 6, 72, dtype=BF, device=DEV)
+        bad += [dict(q=wide[:, :, 4:68]), dict(q=torch.zeros(7, 6, 65, dtype=BF, device=DEV)[:, :, :64]),
+                dict(q=torch.zeros(7, 64, 6, dtype=BF, device=DEV).transpose(1, 2)), dict(out=wide[:, :, 1:65])]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            f(**{**good, **kw})
+    f(**good)
+    if name == "plan":
+        ticket = torch.zeros(1, dtype=torch.int32, device=DEV)
+        with pytest.raises(ValueError):
+            f(**good, ticket=ticket.long())
+        assert f(**good, ticket=ticket).length is good["length"] and int(ticket) == 0
+    if name == "write":
+        for kw in (dict(sections=(20, 20)), dict(sections=(8, 8, 8)), dict(base=-1.0), dict(positions=torch.zeros(2, 7, dtype=torch.int32, device=DEV)),
+                   dict(positions=torch.zeros(1, 7, dtype=torch.int64, device=DEV)), dict(positions=torch.zeros(7, 2, dtype=torch.int32, device=DEV).t(), sections=(16, 16))):
+            with pytest.raises(ValueError):
+                f(**{**good, **kw})
+    torch.cuda.synchronize()
+
+
 # ---- placing -------------------------------------------------------------------------------------------
 
 def _plan_case(B, page, wide, pages, seed, rows=None, slack=0, most=70):
