@@ -73,6 +73,15 @@ PyObject* none() { Py_RETURN_NONE; }
 cudaStream_t stream_of(at::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 at::TensorOptions on(at::Device dev, at::ScalarType type) { return at::TensorOptions().device(dev).dtype(type); }
 
+// A vector of n values at word `at` of a block of 32-bit words (`at` even for 64-bit values).
+Tensor view(const Tensor& block, int64_t at, int64_t n, at::ScalarType type) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(block.storage()), block.key_set(),
+                                                      c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(type == at::kLong ? at / 2 : at);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 // ---- placing: (length, new, table, free, marks, page_rows, rows, ticket) -> (start, slot, episode, position, length, marks)
 PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -90,10 +99,14 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !table_fits(table, b, page_rows, dev))
     return none();
   if (in_place && (!tensor(a[7], ticket) || !vector(ticket, 1, at::kInt, dev))) return none();
-  const auto words = on(dev, at::kInt), longs = on(dev, at::kLong);
-  Tensor start = at::empty({b + 1}, words), slot = at::empty({rows}, longs), episode = at::empty({rows}, words),
-         position = at::empty({rows}, words), after = in_place ? length : at::empty({b}, words),
-         marks_after = in_place ? marks : at::empty({3}, longs);
+  // one allocation: slot, episode, position, marks, each on a 16-byte boundary, then length and start
+  const int64_t padded = (rows + 3) / 4 * 4;
+  const Tensor block = at::empty({4 * padded + 8 + 2 * b + 1}, on(dev, at::kInt));
+  Tensor slot = view(block, 0, rows, at::kLong), episode = view(block, 2 * padded, rows, at::kInt),
+         position = view(block, 3 * padded, rows, at::kInt),
+         marks_after = in_place ? marks : view(block, 4 * padded, 3, at::kLong),
+         after = in_place ? length : view(block, 4 * padded + 8, b, at::kInt),
+         start = view(block, 4 * padded + 8 + b, b + 1, at::kInt);
   mkx_plan_inputs p;
   std::memset(&p, 0, sizeof(p));
   p.length = static_cast<const int*>(length.data_ptr());
