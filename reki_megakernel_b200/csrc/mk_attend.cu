@@ -16,6 +16,7 @@
 
 #include "mkx_attend.cuh"
 #include "mkx_cache_host.h"
+#include "mkx_pdl.cuh"
 
 namespace mkxa {
 namespace {
@@ -96,6 +97,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
   __shared__ LineScratch scratch;
   __shared__ int flag;
   Line line;
+  pdl_begin();
   if (!find_line<MT, KT, ROW_THREADS>(p, scratch, line)) return;  // its barriers publish the mbarriers too
   Walk<MT, KT> walk(p, line);
   Segment sg;
@@ -643,6 +645,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     fence_mbar_init();
   }
   Line line;
+  pdl_begin();
   if (!find_line<CT, CK, CHUNK_THREADS>(p, sm.line, line)) return;
   if (warp == 9) tmem_alloc(&sm.tmem, 512);
   __syncthreads();
@@ -1125,8 +1128,7 @@ bool launch(Kernel kernel, bool (&sized)[MAX_DEVICES], int threads, int smem, co
     if (!mkxc::cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))) return false;
     sized[device] = true;
   }
-  kernel<<<(unsigned)p.slots, threads, smem, stream>>>(tk, tv, p);
-  return mkxc::cuda_ok(cudaGetLastError());
+  return pdl_launch(kernel, p.slots, threads, smem, stream, tk, tv, p);
 }
 template <int DT, int HD>
 bool launch_typed(bool chunk, const CUtensorMap& tk, const CUtensorMap& tv, const AttendParams& p, int device,

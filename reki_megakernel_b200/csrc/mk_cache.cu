@@ -9,6 +9,7 @@
 #include "mkx_cache_host.h"
 #include "mkx_device.cuh"
 #include "mkx_half.cuh"
+#include "mkx_pdl.cuh"
 
 namespace mkxc {
 using namespace mkx;
@@ -68,6 +69,7 @@ __global__ void __launch_bounds__(NT) plan_kernel(const __grid_constant__ mkx_pl
   long long* ring_at = warp_sums + 8;                       // [B] ring place of the episode's first page, mod ring
   PlanShared* ep = reinterpret_cast<PlanShared*>(ring_at + p.B);  // [B]
   __shared__ int is_last;
+  pdl_begin();
   const long long taken = p.marks[0], returned = p.marks[1];
   const long long avail = returned > taken ? returned - taken : 0;
   long long rows = 0, pages = 0, lost = 0;
@@ -185,6 +187,7 @@ __global__ void __launch_bounds__(NT) release_kernel(const __grid_constant__ mkx
   int* first = reinterpret_cast<int*>(warp_sums + 8);  // [B] place among the returned pages
   int* count = first + p.B;                            // [B]
   __shared__ int is_last;
+  pdl_begin();
   const long long returned = p.marks[1];
   long long pages = 0;
   for (int b0 = 0; b0 < p.B; b0 += NT) {
@@ -250,6 +253,7 @@ __device__ __forceinline__ float2 cos_sin(int position, float hi, float lo) {
 __global__ void __launch_bounds__(256) tables_kernel(const __grid_constant__ Rates rates, const int* positions,
                                                      long long pos_stride, int rows, int head_dim, float* cos, float* sin) {
   // one (row, frequency or passing pair) per thread: two entries of each table
+  pdl_begin();
   const int pairs = head_dim / 2;
   const long long n = (long long)rows * pairs;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
@@ -283,6 +287,7 @@ __global__ void __launch_bounds__(256) store_kernel(const __grid_constant__ mkx_
   const int per_row = (groups_q + 2 * groups_k) * lanes;
   const long long n = (long long)p.rows * per_row;
   const long long cells = (long long)p.pages << shift;
+  pdl_begin();
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
     const long long row = i / per_row;
     const int u = (int)(i - row * per_row);
@@ -448,8 +453,7 @@ extern "C" mkx_status mkx_cache_plan(const mkx_plan_inputs* in, int device, cuda
     return MKX_ERR_CUDA;
   long long grid = ((long long)p.rows + NT * ROWS_PER_THREAD - 1) / (NT * ROWS_PER_THREAD);
   grid = grid < 1 ? 1 : grid > sms ? sms : grid;
-  plan_kernel<<<(int)grid, NT, smem, stream>>>(p, shift);
-  return cuda_ok(cudaGetLastError()) ? MKX_OK : MKX_ERR_CUDA;
+  return pdl_launch(plan_kernel, (int)grid, NT, smem, stream, p, shift) ? MKX_OK : MKX_ERR_CUDA;
 }
 
 extern "C" mkx_status mkx_cache_release(const mkx_release_inputs* in, int device, cudaStream_t stream) {
@@ -462,8 +466,7 @@ extern "C" mkx_status mkx_cache_release(const mkx_release_inputs* in, int device
   if (!cuda_ok(scope.err)) return MKX_ERR_CUDA;
   const int sms = sm_count(device);
   if (sms == 0) return MKX_ERR_CUDA;
-  release_kernel<<<p.B < sms ? p.B : sms, NT, 64 + p.B * 8, stream>>>(p, shift);
-  return cuda_ok(cudaGetLastError()) ? MKX_OK : MKX_ERR_CUDA;
+  return pdl_launch(release_kernel, p.B < sms ? p.B : sms, NT, 64 + p.B * 8, stream, p, shift) ? MKX_OK : MKX_ERR_CUDA;
 }
 
 extern "C" mkx_status mkx_rope_tables(const mkx_rotary* rot, const int* positions, long long pos_stride, int rows,
@@ -477,8 +480,9 @@ extern "C" mkx_status mkx_rope_tables(const mkx_rotary* rot, const int* position
   if (sms == 0) return MKX_ERR_CUDA;
   long long grid = ((long long)rows * (head_dim / 2) + 255) / 256;
   if (grid > 8ll * sms) grid = 8ll * sms;
-  tables_kernel<<<(int)grid, 256, 0, stream>>>(rates_of(*rot), positions, pos_stride, rows, head_dim, cos, sin);
-  return cuda_ok(cudaGetLastError()) ? MKX_OK : MKX_ERR_CUDA;
+  return pdl_launch(tables_kernel, (int)grid, 256, 0, stream, rates_of(*rot), positions, pos_stride, rows, head_dim, cos, sin)
+             ? MKX_OK
+             : MKX_ERR_CUDA;
 }
 
 extern "C" mkx_status mkx_cache_store(const mkx_store_inputs* in, int device, cudaStream_t stream) {
@@ -510,9 +514,7 @@ extern "C" mkx_status mkx_cache_store(const mkx_store_inputs* in, int device, cu
   const int gq = with_q ? (p.heads + HG - 1) / HG : 0, gk = (p.kv_heads + HG - 1) / HG;
   long long grid = ((long long)p.rows * (gq + 2 * gk) * (p.head_dim / 16) + 255) / 256;
   if (grid > 64ll * sms) grid = 64ll * sms;
-  if (p.dtype == MKX_BF16)
-    store_kernel<MKX_BF16><<<(int)grid, 256, 0, stream>>>(p, rates, shift, gq, gk);
-  else
-    store_kernel<MKX_FP16><<<(int)grid, 256, 0, stream>>>(p, rates, shift, gq, gk);
-  return cuda_ok(cudaGetLastError()) ? MKX_OK : MKX_ERR_CUDA;
+  const bool ok = pdl_launch(p.dtype == MKX_BF16 ? store_kernel<MKX_BF16> : store_kernel<MKX_FP16>, (int)grid, 256, 0, stream, p,
+                             rates, shift, gq, gk);
+  return ok ? MKX_OK : MKX_ERR_CUDA;
 }
