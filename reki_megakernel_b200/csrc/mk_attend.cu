@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
     while (ok && walk.next(sg)) {
       const int r0 = sg.tile * MT, r1 = min(r0 + MT, sg.fresh * p.group) - 1;
       const Keys ks = keys_of<KT>(p, sg, r0, r1);
-      const int i0 = (int)((long long)ks.blocks * sg.v0 / sg.units), i1 = (int)((long long)ks.blocks * sg.v1 / sg.units);
+      const int i0 = first_block(sg, ks.blocks), i1 = end_block(sg, ks.blocks);
       auto page_at = [&](int i) {
         return lane < boxes ? page_of(p, ks, sg.b, (block_key<KT>(ks, i) >> p.shift) + lane) : -1;
       };
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
   while (walk.next(sg)) {
     const int r0 = sg.tile * MT, r1 = min(r0 + MT, sg.fresh * p.group) - 1;
     const Keys ks = keys_of<KT>(p, sg, r0, r1);
-    const int i0 = (int)((long long)ks.blocks * sg.v0 / sg.units), i1 = (int)((long long)ks.blocks * sg.v1 / sg.units);
+    const int i0 = first_block(sg, ks.blocks), i1 = end_block(sg, ks.blocks);
     // queries: A fragments of the 16 rows (rows that are not there hold anything: no row touches another)
     uint32_t qf[HD / 16][4];
     int pos[2];
@@ -569,8 +569,8 @@ __device__ __forceinline__ void fill(const AttendParams& p, Job& job, const Segm
   job.sg = sg;
   job.r0 = r0;
   job.r1 = r1;
-  job.i0 = (int)((long long)all.blocks * sg.v0 / sg.units);
-  job.i1 = (int)((long long)all.blocks * sg.v1 / sg.units);
+  job.i0 = first_block(sg, all.blocks);
+  job.i1 = end_block(sg, all.blocks);
   job.keys = all;
   for (int x = 0; x < 2; ++x) {
     Tile t{0, 0, 0, 0, 0};
@@ -1214,7 +1214,7 @@ extern "C" mkx_status mkx_cache_attend(const mkx_attend_inputs* in, size_t works
   p.q_and = a.scale == 0.f ? 0u : ~0u;
   p.q_xor = a.scale < 0.f ? 0x80008000u : 0u;
   p.slots = pl.slots;
-  p.min_units = 2;
+  p.min_shift = 1;
   p.snap = 2;
   p.timeout_ns = 2000000000ull;
   const bool ok =

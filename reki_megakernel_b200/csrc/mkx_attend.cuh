@@ -25,7 +25,7 @@ struct AttendParams {
   float scale_log2;       // |scale| * log2(e): scores are kept in powers of two
   uint32_t q_and, q_xor;  // q's words as they enter: the sign of a negative scale, nothing for scale 0
   int slots;      // blocks of the grid
-  int min_units;  // key blocks that one block takes at least
+  int min_shift;  // log2 of the key blocks that one block takes at least
   int snap;       // units by which a cut may move to a tile's end
   unsigned long long timeout_ns;
 };
@@ -98,12 +98,55 @@ struct LineScratch {
   long long sums[2][32];
   Line line;
 };
+
+// What the thread of episode b (units at .. at + mine - 1) knows of the block's stretch.
+__device__ __forceinline__ void cut_line(const AttendParams& p, Line& line, const Episode& e, int b, long long at,
+                                         long long mine, long long all, int blocks) {
+  const long long u0 = quotient(all * blockIdx.x, blocks), u1 = quotient(all * (blockIdx.x + 1), blocks);
+  if (u0 >= at && u0 < at + mine) {
+    line.total = all;
+    line.at = at;
+    line.begin = snapped(u0, at, e.units, p.snap);
+    line.blocks = blocks;
+    line.b = b;
+    line.e = e;
+  }
+  if (u1 >= at && u1 < at + mine) line.end = snapped(u1, at, e.units, p.snap);
+}
+
 template <int MT, int KT, int NTH>
 __device__ __forceinline__ bool find_line(const AttendParams& p, LineScratch& scratch, Line& out) {
   constexpr int W = NTH / 32;
   auto& sums = scratch.sums;
   Line& line = scratch.line;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto prefix = [&](long long mine) {  // inclusive, over the warp
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, mine, d);
+      if (lane >= d) mine += o;
+    }
+    return mine;
+  };
+  auto blocks_of = [&](long long all) { return (int)min((long long)p.slots, (all >> p.min_shift) + 1); };
+  if (p.B <= 32) {  // one warp does it, between one pair of barriers less
+    if (warp == 0) {
+      Episode e;
+      long long mine = 0;
+      if (lane < p.B) {
+        e = episode_of<MT, KT>(p, lane);
+        mine = (long long)e.tiles * p.kv_heads * e.units;
+      }
+      const long long inc = prefix(mine), all = __shfl_sync(0xffffffffu, inc, 31);
+      const int blocks = blocks_of(all);
+      if (lane == 0) line.begin = line.end = (int)blockIdx.x < blocks ? all : 0;
+      __syncwarp();
+      if ((int)blockIdx.x < blocks) cut_line(p, line, e, lane, inc - mine, mine, all, blocks);
+    }
+    __syncthreads();
+    out = line;
+    return out.begin < out.end;
+  }
   Episode e;
   long long all = 0, mine = 0;
   for (int b = threadIdx.x; b < p.B; b += NTH) {
@@ -122,12 +165,12 @@ __device__ __forceinline__ bool find_line(const AttendParams& p, LineScratch& sc
   all = 0;
 #pragma unroll
   for (int w = 0; w < W; ++w) all += sums[0][w];
-  const int blocks = (int)min((long long)p.slots, quotient(all, p.min_units) + 1);
+  const int blocks = blocks_of(all);
   if (all == 0 || (int)blockIdx.x >= blocks) return false;
-  const long long u0 = quotient(all * blockIdx.x, blocks), u1 = quotient(all * (blockIdx.x + 1), blocks);
+  const long long u1 = quotient(all * (blockIdx.x + 1), blocks);
   if (threadIdx.x == 0) line.end = all;
   long long before = 0;
-  for (int b0 = 0;; b0 += NTH) {  // ends: u0 < all
+  for (int b0 = 0;; b0 += NTH) {
     const int b = b0 + threadIdx.x;
     if (b0 > 0) {
       mine = 0;
@@ -136,12 +179,7 @@ __device__ __forceinline__ bool find_line(const AttendParams& p, LineScratch& sc
         mine = (long long)e.tiles * p.kv_heads * e.units;
       }
     }
-    long long inc = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, inc, d);
-      if (lane >= d) inc += o;
-    }
+    const long long inc = prefix(mine);
     if (b0 > 0) __syncthreads();  // the sums have been read
     if (lane == 31) sums[1][warp] = inc;
     __syncthreads();
@@ -151,15 +189,7 @@ __device__ __forceinline__ bool find_line(const AttendParams& p, LineScratch& sc
       if (w < warp) at += sums[1][w];
       before += sums[1][w];
     }
-    if (u0 >= at && u0 < at + mine) {
-      line.total = all;
-      line.at = at;
-      line.begin = snapped(u0, at, e.units, p.snap);
-      line.blocks = blocks;
-      line.b = b;
-      line.e = e;
-    }
-    if (u1 >= at && u1 < at + mine) line.end = snapped(u1, at, e.units, p.snap);
+    cut_line(p, line, e, b, at, mine, all, blocks);
     if (before > u1 || before >= all) break;
   }
   __syncthreads();
@@ -264,6 +294,14 @@ __device__ __forceinline__ bool last_of(unsigned* ticket, int n, int* last) {
   }
   asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");
   return *last;  // (the word is written again only behind the first barrier of the next call)
+}
+
+// The key blocks of a segment, of `blocks` that its tile really has (its units are those of the episode's longest tile).
+__device__ __forceinline__ int first_block(const Segment& s, int blocks) {
+  return s.v0 == 0 ? 0 : (int)quotient((long long)blocks * s.v0, s.units);
+}
+__device__ __forceinline__ int end_block(const Segment& s, int blocks) {
+  return s.v1 == s.units ? blocks : (int)quotient((long long)blocks * s.v1, s.units);
 }
 
 // The keys that the rows of a tile see: blocks of KT keys, first those of the sinks, then from the
