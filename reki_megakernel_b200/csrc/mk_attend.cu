@@ -27,7 +27,7 @@ constexpr int MAX_KEYS = 1 << 30;  // rows of an episode: keys and positions are
 constexpr int ROW_WARPS = 4;
 constexpr int ROW_THREADS = 32 * (ROW_WARPS + 1);
 constexpr int ROW_STAGES = 3;
-constexpr int JOIN_AT_ONCE = 12;  // parts that one block joins
+constexpr int JOIN_AT_ONCE = 12;  // parts that one block joins; more in two levels
 
 template <int HD>
 struct RowShape {
@@ -1013,62 +1013,96 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         continue;
       }
       const int own = blockIdx.x - sg.lead;
-      if (!others_done<TILE_THREADS>(p.tickets + sg.lead, sg.parts, &sm.flag)) {
-        float* part = p.parts + (size_t)part_place(sg, own) * PART;
+      auto ml_at = [&](int k) { return reinterpret_cast<float2*>(p.parts + (size_t)part_place(sg, k) * PART + CT * HD) + row; };
+      auto sums_at = [&](int k, int j) {
+        return reinterpret_cast<float4*>(p.parts + (size_t)part_place(sg, k) * PART) + row + 8 * j * CT;
+      };
+      // Adds up the parts first, first + step, ..., `count` of them, in their order, whoever is last: the same sums every
+      // time. Part `mine` is still in TMEM (-1: none). emit(32 sums, j) for each 32 dims.
+      auto join = [&](int first, int step, int count, int mine, float& top, float& ls, auto emit) {
+        auto ml_of = [&](int k) { return k == mine ? make_float2(m, l) : __ldcg(ml_at(k)); };
+        top = -INFINITY;
+        ls = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < count; ++i) top = fmaxf(top, ml_of(first + i * step).x);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+        for (int i = 0; i < count; ++i) {
+          const float2 ml = ml_of(first + i * step);
+          ls += ex2(ml.x - base) * ml.y;
+        }
+#pragma unroll 1
+        for (int j = 0; j < HD / 32; ++j) {
+          float acc[32];
+#pragma unroll
+          for (int d = 0; d < 32; ++d) acc[d] = 0.f;
+#pragma unroll 2
+          for (int i = 0; i < count; ++i) {
+            const int k = first + i * step;
+            float o[32];
+            if (k == mine) {
+              sums_of(j, o);
+            } else {
+#pragma unroll
+              for (int d = 0; d < 32; d += 4) {
+                const float4 v = __ldcg(sums_at(k, j) + (d / 4) * CT);
+                o[d] = v.x;
+                o[d + 1] = v.y;
+                o[d + 2] = v.z;
+                o[d + 3] = v.w;
+              }
+            }
+            const float f = ex2(ml_of(k).x - base);
+#pragma unroll
+            for (int d = 0; d < 32; ++d) acc[d] += f * o[d];
+          }
+          emit(acc, j);
+        }
+      };
+      auto keep = [&](int k, const float (&o)[32], int j) {
+        if (r <= r1)
+#pragma unroll
+          for (int d = 0; d < 32; d += 4)
+            __stcg(sums_at(k, j) + (d / 4) * CT, make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]));
+      };
+      // many parts are joined in two levels, so that no block reads more than a few
+      int step = 1, groups = sg.parts, mine = -1;
+      if (sg.parts > JOIN_AT_ONCE)
+        while (step * step < sg.parts) ++step;
+      if (step == 1 && others_done<TILE_THREADS>(p.tickets + sg.lead, sg.parts, &sm.flag)) {
+        mine = own;
+      } else {
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j) {
           float o[32];
           sums_of(j, o);
-#pragma unroll
-          for (int d = 0; d < 32; d += 4)
-            __stcg(reinterpret_cast<float4*>(part) + row + (8 * j + d / 4) * CT,
-                   make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]));
+          keep(own, o, j);
         }
-        __stcg(reinterpret_cast<float2*>(part + (size_t)CT * HD) + row, make_float2(m, l));
-        if (!last_of<TILE_THREADS>(p.tickets + sg.lead, sg.parts, &sm.flag)) {
+        if (r <= r1) __stcg(ml_at(own), make_float2(m, l));
+        if (step > 1) {
+          const int first = own / step * step, count = min(step, sg.parts - first);
+          if (!last_of<TILE_THREADS>(p.tickets + p.slots + part_place(sg, first), count, &sm.flag)) {
+            tmem_fence_before();
+            continue;
+          }
+          if (__any_sync(0xffffffffu, r <= r1)) {
+            // the sums take the place of the group's first part, each thread's behind its own reads of it
+            float top, ls;
+            join(first, 1, count, -1, top, ls, [&](const float (&o)[32], int j) { keep(first, o, j); });
+            if (r <= r1) __stcg(ml_at(first), make_float2(top, ls));
+          }
+          groups = ceil_div(sg.parts, step);
+        }
+        if (!last_of<TILE_THREADS>(p.tickets + sg.lead, groups, &sm.flag)) {
           tmem_fence_before();
           continue;
         }
       }
-      // the parts in their order, whoever is last: the same sums every time
-      auto ml_of = [&](int k) {
-        return k == own ? make_float2(m, l)
-                        : __ldcg(reinterpret_cast<const float2*>(p.parts + (size_t)part_place(sg, k) * PART + CT * HD) + row);
-      };
-      float top = -INFINITY, ls = 0.f;
-#pragma unroll 4
-      for (int k = 0; k < sg.parts; ++k) top = fmaxf(top, ml_of(k).x);
-      const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll 4
-      for (int k = 0; k < sg.parts; ++k) {
-        const float2 ml = ml_of(k);
-        ls += ex2(ml.x - base) * ml.y;
-      }
-#pragma unroll 1
-      for (int j = 0; j < HD / 32; ++j) {
-        float acc[32];
-#pragma unroll
-        for (int d = 0; d < 32; ++d) acc[d] = 0.f;
-        for (int k = 0; k < sg.parts; ++k) {
-          float o[32];
-          if (k == own) {
-            sums_of(j, o);
-          } else {
-            const float4* at = reinterpret_cast<const float4*>(p.parts + (size_t)part_place(sg, k) * PART) + row + 8 * j * CT;
-#pragma unroll
-            for (int d = 0; d < 32; d += 4) {
-              const float4 v = __ldcg(at + (d / 4) * CT);
-              o[d] = v.x;
-              o[d + 1] = v.y;
-              o[d + 2] = v.z;
-              o[d + 3] = v.w;
-            }
-          }
-          const float f = ex2(ml_of(k).x - base);
-#pragma unroll
-          for (int d = 0; d < 32; ++d) acc[d] += f * o[d];
-        }
-        if (r <= r1) write(acc, j, scale_of(ls));
+      if (__any_sync(0xffffffffu, r <= r1)) {
+        float top, ls;
+        join(0, step, groups, mine, top, ls, [&](const float (&o)[32], int j) {
+          if (r <= r1) write(o, j, scale_of(ls));
+        });
       }
       tmem_fence_before();
     }
@@ -1104,6 +1138,22 @@ struct Plan {
   size_t bytes;
 };
 
+// rows_kernel's time goes with the (16 rows) x keys of all tiles, chunk_kernel's with the (256 rows) x (128 keys), and it
+// has more to do around a tile; measured in us (head_dim 64 / 128): a block 1.43 / 1.7 on one of the SMs and 4.5 around a
+// tile against 59 / 79 a million keys of a 16-row tile on the whole GPU, 25 against 8 for the launch, and 20 more where so
+// few tiles share the SMs that parts are joined twice. How long the caches are is not known here: what the tables can hold
+// stands for it. Beyond one 16-row tile, rows_kernel against chunk_kernel (us; episodes x rows per K/V head after keys, K/V
+// heads, head_dim): 1 x 32 after 4000, 12, 64: 14.9, 25.5; 1 x 64 after 4000: 16.0, 25.9; after 40000: 68.7, 55.5; 128 x 20
+// after 500: 79.7, 124.9; 64 x 32 after 4000: 360, 237; 8 x 32 after 8000, 8, 128: 91, 71; 1 x 32 after 100000, 1: 33, 62.
+bool chunk_is_faster(const mkx_attend_inputs& a, long long rows) {
+  double keys = (double)a.table_width * a.page_rows;
+  if (a.window > 0 && (double)a.window + a.sinks + a.max_rows < keys) keys = (double)a.window + a.sinks + a.max_rows;
+  const double heads = (double)a.B * a.kv_heads, tiles = heads * ((rows + CT - 1) / CT), sms = 148;
+  const double by_rows = 8 + heads * ((rows + MT - 1) / MT) * keys * (a.head_dim == 64 ? 59e-6 : 79e-6);
+  const double by_chunk = 25 + tiles / sms * (keys / CK * (a.head_dim == 64 ? 1.43 : 1.7) + 4.5) + (tiles * JOIN_AT_ONCE < sms ? 20 : 0);
+  return by_chunk < by_rows;
+}
+
 // The launch of a call, from sizes alone; false for sizes that are refused.
 bool plan_of(const mkx_attend_inputs& a, int sms, Plan& pl) {
   if (a.rows < 0 || a.B < 1 || a.B > MKX_MAX_EPISODES || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads != 0 ||
@@ -1113,8 +1163,7 @@ bool plan_of(const mkx_attend_inputs& a, int sms, Plan& pl) {
   if (a.head_dim != 64 && a.head_dim != 128) return false;
   const long long group = a.heads / a.kv_heads;
   const long long most = a.max_rows < a.rows ? a.max_rows : a.rows;
-  // rows of one K/V head and episode beyond one 16-row tile would read the pages again: chunk_kernel
-  pl.chunk = most * group > MT;
+  pl.chunk = most * group > MT && chunk_is_faster(a, most * group);
   pl.kt = pl.chunk ? CK : 8192 / a.head_dim;
   pl.slots = pl.chunk ? sms : 2 * sms;
   pl.bytes = MKX_ATTEND_TICKETS * 4 + (size_t)2 * pl.slots * (pl.chunk ? CT : MT) * (a.head_dim + 2) * 4;

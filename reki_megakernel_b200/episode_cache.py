@@ -279,7 +279,8 @@ def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table:
     with a ``window`` > 0, with j > p - window or j < ``sinks``. out = softmax(scale q k^T) v (scale: 1 / sqrt(head_dim)),
     zero for a row that sees nothing; rows behind start[B] are left as they were. What pages hold beyond an
     episode's length does not matter; the K and V rows below it are finite. ``max_rows``: no episode has more new rows
-    (default: q's rows); a tight value picks the kernel that fits. A wait that ran out on the device surfaces in
+    (default: q's rows). The kernel is chosen by ``max_rows`` and by what a table row can hold, so tight values of both
+    pick the one that fits. A wait that ran out on the device surfaces in
     ``check_device_error()``."""
     most = -1 if max_rows is None else max_rows if max_rows >= 0 else -2  # -1: q's rows; below: refused
     r = _lib.load_torch().attend(q, k_pages, v_pages, table, length, start, most, causal, window, sinks, scale, out)

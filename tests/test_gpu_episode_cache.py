@@ -261,6 +261,10 @@ def _check_attend(c, max_rows=None, tail=0, out=None, **kw):
     return got
 
 
+# Beyond 16 rows of a K/V head the kernel goes by what the tables can hold (how long the caches are is not known when a
+# call is launched): a tight table brings these small caches to the kernel of 16-row tiles, a wide one to that of chunks.
+WIDTHS = pytest.mark.parametrize("extra_width", [2, 300000])
+
 SHAPES = [(12, 12, 64), (32, 8, 128), (7, 1, 64), (16, 2, 128), (40, 2, 64), (5, 5, 128)]
 LENGTHS = [  # new, past
     ([1], [0]), ([1, 1, 1], [0, 16, 700]), ([10] * 5, [31, 0, 64, 1000, 129]), ([0, 3, 0, 17, 1], [40, 0, 0, 260, 513]),
@@ -269,16 +273,18 @@ LENGTHS = [  # new, past
 
 @pytest.mark.parametrize("heads,kv,hd", SHAPES)
 @pytest.mark.parametrize("new,past", LENGTHS)
-def test_attend_causal(heads, kv, hd, new, past):
+@WIDTHS
+def test_attend_causal(heads, kv, hd, new, past, extra_width):
     dtype, page = (BF, 32) if (heads + len(new)) % 2 else (FP, 16)
-    c = pages_for(new, past, heads, kv, hd, page=page, dtype=dtype, seed=heads + sum(new))
+    c = pages_for(new, past, heads, kv, hd, page=page, dtype=dtype, seed=heads + sum(new), extra_width=extra_width)
     _check_attend(c, max_rows=max(new))
 
 
 @pytest.mark.parametrize("heads,kv,hd", SHAPES)
 @pytest.mark.parametrize("new,past", LENGTHS[1:5])
-def test_attend_all(heads, kv, hd, new, past):
-    c = pages_for(new, past, heads, kv, hd, page=64, dtype=FP if heads % 2 else BF, seed=sum(past))
+@WIDTHS
+def test_attend_all(heads, kv, hd, new, past, extra_width):
+    c = pages_for(new, past, heads, kv, hd, page=64, dtype=FP if heads % 2 else BF, seed=sum(past), extra_width=extra_width)
     _check_attend(c, causal=False)
 
 
@@ -286,9 +292,10 @@ def test_attend_all(heads, kv, hd, new, past):
 @pytest.mark.parametrize("new,past,heads,kv,hd,page", [
     ([1, 1], [900, 3], 12, 12, 64, 32), ([9, 1, 0, 40], [400, 0, 12, 1000], 16, 4, 128, 16),
     ([260, 35], [700, 0], 6, 2, 64, 128), ([150], [2000], 4, 1, 128, 256)])
-def test_attend_window(window, sinks, new, past, heads, kv, hd, page):
+@WIDTHS
+def test_attend_window(window, sinks, new, past, heads, kv, hd, page, extra_width):
     """Pages that no row sees any more hold NaN: they may have gone to somebody else."""
-    c = pages_for(new, past, heads, kv, hd, page=page, seed=window)
+    c = pages_for(new, past, heads, kv, hd, page=page, seed=window, extra_width=extra_width)
     for b in range(len(new)):
         for j in range(-(-(new[b] + past[b]) // page)):
             if new[b] and (j + 1) * page <= past[b] - window + 1 and j * page >= sinks:
@@ -302,19 +309,21 @@ def test_attend_window(window, sinks, new, past, heads, kv, hd, page):
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("new", [1, 200])
-def test_attend_page_sizes(page, hd, new):
+@WIDTHS
+def test_attend_page_sizes(page, hd, new, extra_width):
     for n in (page - 1, page, page + 1, 3 * page + 5):
-        c = pages_for([new, new], [n, 2 * n], 4, 2, hd, page=page, seed=n)
+        c = pages_for([new, new], [n, 2 * n], 4, 2, hd, page=page, seed=n, extra_width=extra_width)
         _check_attend(c)
 
 
-def test_attend_rows_that_see_nothing():
+@WIDTHS
+def test_attend_rows_that_see_nothing(extra_width):
     """An episode without any row (length 0) and new rows that were never stored (length below the new rows)."""
-    c = pages_for([4, 6, 2], [0, 20, 50], 4, 2, 64)
+    c = pages_for([4, 6, 2], [0, 20, 50], 4, 2, 64, extra_width=extra_width)
     c["length"][0] = 0
     got = _check_attend(c)
     assert (got[:4] == 0).all()
-    c = pages_for([4, 150, 2], [0, 20, 50], 4, 2, 64)
+    c = pages_for([4, 150, 2], [0, 20, 50], 4, 2, 64, extra_width=extra_width)
     c["length"][1] = 60      # 90 rows lie before position 0
     got = ec().attend(**c)
     assert (got[4:94] == 0).all() and torch.isfinite(got.float()).all()
@@ -323,8 +332,9 @@ def test_attend_rows_that_see_nothing():
 
 
 @pytest.mark.parametrize("new", [[3, 1], [150, 40]])
-def test_attend_leaves_rows_behind_the_last(new):
-    c = pages_for(new, [70, 9], 4, 4, 64, tail_rows=13)
+@WIDTHS
+def test_attend_leaves_rows_behind_the_last(new, extra_width):
+    c = pages_for(new, [70, 9], 4, 4, 64, tail_rows=13, extra_width=extra_width)
     out = torch.full_like(c["q"], 7.0)
     got = _check_attend(c, tail=13, out=out)
     assert got is out and (out[sum(new):] == 7.0).all()
@@ -338,10 +348,11 @@ def test_attend_leaves_rows_behind_the_last(new):
 
 
 @pytest.mark.parametrize("new", [[2, 1, 9], [140, 300]])
-def test_attend_strides(new):
+@WIDTHS
+def test_attend_strides(new, extra_width):
     """q and out as slices of wider rows, pages laid out head by head and as a slice of a pool of layers."""
     past = [300] * len(new)
-    c = pages_for(new, past, 6, 2, 64, head_major=True, seed=4)
+    c = pages_for(new, past, 6, 2, 64, head_major=True, seed=4, extra_width=extra_width)
     n = sum(new)
     wide = torch.zeros(n, 10 * 64, dtype=BF, device=DEV)
     wide[:, 128:512] = c["q"].reshape(n, -1)
@@ -354,15 +365,16 @@ def test_attend_strides(new):
     _check_attend(c, out=out)
 
 
-def test_attend_scale_and_large_scores():
+@WIDTHS
+def test_attend_scale_and_large_scores(extra_width):
     """Scores of thousands: one key takes all; a scale of zero: the mean."""
-    c = pages_for([3, 200], [90, 50], 4, 2, 64, q_scale=400.0, seed=8)
+    c = pages_for([3, 200], [90, 50], 4, 2, 64, q_scale=400.0, seed=8, extra_width=extra_width)
     ref, _ = attend_oracle(**c)
     got = ec().attend(**c)
     # scores up to 2^13 have fp32 error 2^-10: a tie within that may go either way, elsewhere the row is a copy
     near = (got.double() - ref).abs() <= 2.0 ** -7 * ref.abs() + 2.0 ** -6
     assert near.double().mean() >= 0.995 and torch.isfinite(got.float()).all()
-    c = pages_for([3, 200], [90, 50], 4, 2, 64, seed=8)
+    c = pages_for([3, 200], [90, 50], 4, 2, 64, seed=8, extra_width=extra_width)
     _check_attend(c, scale=0.0)
     _check_attend(c, scale=-0.2)
 
