@@ -276,11 +276,15 @@ __global__ void __launch_bounds__(256) tables_kernel(const __grid_constant__ Rat
 // ---- storing -------------------------------------------------------------------------------------
 // A thread takes 8 dims and their 8 partners (16-byte accesses) of a row for up to HG heads of one of
 // q, k, v, and forms the 8 angles once for those heads. Bound by HBM: every row is read and written
-// once; the angles are about 25 instructions each, spread over HG heads.
+// once; the angles are about 25 instructions each, spread over HG heads. 30,011 rows of 32 + 8 + 8
+// heads x 128 (738 MB): 123 to 127 us, 5.8 to 6.0 TB/s; 4096 rows of 3 x 12 heads x 64: 8.8 us.
+// The bound of 64 registers (four blocks an SM): 128 and 10.0 us without it, 179 and 13.5 us with 48
+// registers, 500 to 16,000 rows level. HG, measured without the bound: 2 heads 174 us, 4 heads 128,
+// 8 heads 123, but then 16,000 rows of 3 x 12 heads take 38.6 us where 4 heads take 31 to 32.
 constexpr int HG = 4;
 
 template <int DT>
-__global__ void __launch_bounds__(256) store_kernel(const __grid_constant__ mkx_store_inputs p,
+__global__ void __launch_bounds__(256, 4) store_kernel(const __grid_constant__ mkx_store_inputs p,
                                                     const __grid_constant__ Rates rates, int shift, int groups_q,
                                                     int groups_k) {
   const int lanes = p.head_dim / 16;
