@@ -370,7 +370,15 @@ PyObject* error_code(PyObject*, PyObject* const* a, Py_ssize_t n) {
     t = it->second;
   }
   const int code = t.item<int>();
-  if (code) t.zero_();
+  if (code) {  // the calls that gave up may have left tickets behind
+    c10::cuda::CUDAGuard guard(dev);
+    c10::cuda::device_synchronize();
+    t.zero_();
+    std::lock_guard<std::mutex> hold(lock);
+    for (auto& s : spaces)
+      if (s.first.first == (int)index) s.second.narrow(0, 0, MKX_ATTEND_TICKETS * 4).zero_();
+    c10::cuda::device_synchronize();
+  }
   return PyLong_FromLong(code);
   END_HANDLE_TH_ERRORS
 }
