@@ -227,6 +227,16 @@ def test_write_rows(rows, heads, kv, hd, page, dtype, sections, interleaved):
     assert (flat[rest.to(DEV)] == 3.0).all() and (vp.view(-1, kv, hd)[rest.to(DEV)] == -5.0).all()
 
 
+def test_write_rotates_k_alone():
+    g = torch.Generator().manual_seed(9)
+    k, v = (torch.randn(37, 2, 128, generator=g).to(FP).to(DEV) for _ in range(2))
+    slot, pos = torch.randperm(64, generator=g)[:37].to(DEV), torch.randint(0, 900, (2, 37), generator=g).to(torch.int32)
+    kp, vp = (torch.zeros(4, 16, 2, 128, dtype=FP, device=DEV) for _ in range(2))
+    assert ec().write_rows(k, v, slot, kp, vp, positions=pos.to(DEV), sections=(40, 24), base=500.0) is None
+    _check_turned(kp.view(64, 2, 128)[slot], k, angles_oracle(pos, (40, 24), base=500.0))
+    assert torch.equal(vp.view(64, 2, 128)[slot], v)
+
+
 def test_write_without_positions_and_in_place():
     """K as it is where there are no positions; q may be rotated in place; pages may be laid out head by head."""
     g = torch.Generator().manual_seed(0)
@@ -304,6 +314,18 @@ def test_attend_window(window, sinks, new, past, heads, kv, hd, page, extra_widt
                 if j % 2:
                     c["table"][b, j] = -1
     _check_attend(c, max_rows=max(new), window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("most", [1, 5, 40])
+@WIDTHS
+def test_attend_many_episodes(most, extra_width):
+    """More episodes than a block has threads, many without new rows or without any."""
+    g = torch.Generator().manual_seed(most)
+    new = [int(x) for x in torch.randint(0, most + 1, (700,), generator=g)]
+    past = [int(x) if x % 3 else 0 for x in torch.randint(0, 200, (700,), generator=g)]
+    c = pages_for(new, past, 4, 2, 64, page=16, seed=most, extra_width=min(extra_width, 20000))
+    _check_attend(c, max_rows=most)
+    _check_attend(c, max_rows=most, window=30, sinks=2)
 
 
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
