@@ -369,10 +369,10 @@ PyObject* error_code(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (it == errors.end() || !it->second.defined()) return PyLong_FromLong(0);
     t = it->second;
   }
+  c10::cuda::CUDAGuard guard(dev);
+  c10::cuda::device_synchronize();  // the calls of all streams
   const int code = t.item<int>();
   if (code) {  // the calls that gave up may have left tickets behind
-    c10::cuda::CUDAGuard guard(dev);
-    c10::cuda::device_synchronize();
     t.zero_();
     std::lock_guard<std::mutex> hold(lock);
     for (auto& s : spaces)
