@@ -37,7 +37,7 @@ extern "C" {
  * and position in the episode; rows behind the last one get -1, -1, 0. table entries of granted pages
  * are written, all others stay. length_out and marks_out may be length and marks: then `ticket` (else it
  * may be null), a word that is zero before the first call and after each, orders reads before writes. Negative lengths
- * count as 0. */
+ * and marks count as 0, lengths above 2^30 as 2^30, more free pages than the ring has places as those. */
 typedef struct {
   const int* length;         /* [B] */
   const int* new_rows;       /* [B] */

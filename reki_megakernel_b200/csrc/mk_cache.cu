@@ -54,8 +54,10 @@ __device__ __forceinline__ long long block_exclusive(long long v, long long* war
 // Every block forms the two prefixes over the episodes (new rows, new pages) by itself from the B
 // lengths -- a few KB out of L2 -- and then maps its own share of the rows, so one launch without any
 // exchange between blocks does it all; a row's episode comes from a binary search in shared memory. The
-// state (lengths, marks) is written by the last block that has read it. Latency bound: at 16 episodes
-// and 160 rows the launch is all there is; 100,003 rows of 700 episodes are 1.6 MB of output.
+// state (lengths, marks) is written by the last block that has read it. Latency bound: 160 rows of 16
+// episodes take 6.4 us, 100,003 rows of 700 episodes (1.6 MB of output) 7.1 us, both what a call costs
+// (host and launch).
+constexpr int MOST_ROWS = 1 << 30;  // that a table row can stand for
 struct PlanShared {
   int start;  // first row
   int past;   // rows held before
@@ -70,14 +72,15 @@ __global__ void __launch_bounds__(NT) plan_kernel(const __grid_constant__ mkx_pl
   PlanShared* ep = reinterpret_cast<PlanShared*>(ring_at + p.B);  // [B]
   __shared__ int is_last;
   pdl_begin();
-  const long long taken = p.marks[0], returned = p.marks[1];
-  const long long avail = returned > taken ? returned - taken : 0;
+  // whatever the state holds, no index leaves the ring or a table row
+  const long long taken = max(p.marks[0], 0ll), returned = p.marks[1];
+  const long long avail = returned > taken ? min(returned - taken, (long long)p.ring_pages) : 0;
   long long rows = 0, pages = 0, lost = 0;
   for (int b0 = 0; b0 < p.B; b0 += NT) {
     const int b = b0 + threadIdx.x;
     int past = 0, fresh = 0;
     if (b < p.B) {
-      past = max(p.length[b], 0);
+      past = min(max(p.length[b], 0), MOST_ROWS);
       fresh = max(p.new_rows[b], 0);
     }
     long long total;
@@ -150,7 +153,8 @@ __global__ void __launch_bounds__(NT) plan_kernel(const __grid_constant__ mkx_pl
       if (r >= total_rows) continue;
       while (b + 1 < p.B && ep[b + 1].start <= r) ++b;
       const PlanShared e = ep[b];
-      const int at = e.past + (int)(r - e.start), page = at >> shift;
+      const unsigned at = (unsigned)e.past + (unsigned)(r - e.start);  // below 2^30 + 2^31
+      const int page = (int)(at >> shift);
       int id = -1;
       if (page < e.page0) {
         if (page < p.table_width) id = p.table[(size_t)b * p.table_width + page];
@@ -162,7 +166,7 @@ __global__ void __launch_bounds__(NT) plan_kernel(const __grid_constant__ mkx_pl
       }
       slot[i] = id < 0 ? -1 : ((long long)id << shift) + (at & ((1 << shift) - 1));
       epi[i] = b;
-      pos[i] = at;
+      pos[i] = (int)at;
     }
     if (r0 + ROWS_PER_THREAD <= p.rows) {
       *reinterpret_cast<longlong2*>(p.slot + r0) = make_longlong2(slot[0], slot[1]);
@@ -188,7 +192,7 @@ __global__ void __launch_bounds__(NT) release_kernel(const __grid_constant__ mkx
   int* count = first + p.B;                            // [B]
   __shared__ int is_last;
   pdl_begin();
-  const long long returned = p.marks[1];
+  const long long returned = max(p.marks[1], 0ll);
   long long pages = 0;
   for (int b0 = 0; b0 < p.B; b0 += NT) {
     const int b = b0 + threadIdx.x;
@@ -285,8 +289,8 @@ constexpr int HG = 4;
 
 template <int DT>
 __global__ void __launch_bounds__(256, 4) store_kernel(const __grid_constant__ mkx_store_inputs p,
-                                                    const __grid_constant__ Rates rates, int shift, int groups_q,
-                                                    int groups_k) {
+                                                       const __grid_constant__ Rates rates, int shift, int groups_q,
+                                                       int groups_k) {
   const int lanes = p.head_dim / 16;
   const int per_row = (groups_q + 2 * groups_k) * lanes;
   const long long n = (long long)p.rows * per_row;
@@ -322,7 +326,7 @@ __global__ void __launch_bounds__(256, 4) store_kernel(const __grid_constant__ m
     const bool turns = what != 2 && p.positions && 8 * c < rates.half;
     // dims of this lane: 8 c and their partners, or 16 dims side by side where nothing turns
     int d0 = 16 * c, d1 = 16 * c + 8;
-    if (what != 2 && p.positions && 8 * c < rates.half) {
+    if (turns) {
       d0 = 8 * c;
       d1 = 8 * c + rates.half;
     }

@@ -15,7 +15,7 @@ share one pool of pages. One step of serving is
 ``EpisodeCache`` keeps the pools, tables and counters of such a cache. ``rope_tables`` makes the
 cos / sin tables of the same positions for ``RegisterPrepare.run`` and ``ExpertMegakernel.run``. All
 calls are asynchronous on the current stream of the tensors' device and can be captured in a CUDA
-graph. There is no CPU fallback: the CUDA library must load.
+graph. There is no CPU fallback: the CUDA library must load. Inference only: nothing records gradients.
 """
 from __future__ import annotations
 
@@ -277,7 +277,7 @@ def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table:
 
     A row at position p sees the rows j < length[b] of its episode with j <= p (all of them if not ``causal``) and,
     with a ``window`` > 0, with j > p - window or j < ``sinks``. out = softmax(scale q k^T) v (scale: 1 / sqrt(head_dim)),
-    zero for a row that sees nothing; rows behind start[B] are left as they were. What pages hold beyond an
+    zero for a row that sees nothing; rows behind start[B] are left as they were. ``out`` may be q. What pages hold beyond an
     episode's length does not matter; the K and V rows below it are finite. ``max_rows``: no episode has more new rows
     (default: q's rows). The kernel is chosen by ``max_rows`` and by what a table row can hold, so tight values of both
     pick the one that fits. A wait that ran out on the device surfaces in
@@ -300,7 +300,9 @@ def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table:
 
 def check_device_error(device=None) -> None:
     """Raises if a bounded wait of an ``attend`` on ``device`` ran out since the last check (synchronises)."""
-    index = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    index = None if device is None else torch.device(device).index
+    if index is None:
+        index = torch.cuda.current_device()
     code = _lib.load_torch().error_code(index, False)
     if code:
         raise _lib.MkxError("attend", _lib.MKX_ERR_DEVICE, f"error word {code:#x}")
@@ -351,7 +353,8 @@ class EpisodeCache:
 
     def plan(self, new: torch.Tensor, rows: int) -> RowPlan:
         """Places ``new`` [episodes] int32 rows (device); ``rows`` is the room of the step's row tensors. The plan's
-        length and marks are the cache's own. Rows without a slot are counted in ``marks[2]``."""
+        length and marks are the cache's own. Rows without a slot are counted in ``marks[2]``: their episodes grew by
+        the stored rows alone, fewer than the plan's ``start`` says, so that step is not one to ``attend`` with."""
         return plan_rows(self.length, new, self.table, self.free, self.marks, page_rows=self.page_rows, rows=rows,
                          ticket=self._ticket)
 

@@ -110,6 +110,23 @@ def test_plan_runs_out(kind):
     _same_plan(r, t[2], ref)
 
 
+def test_plan_of_an_impossible_state():
+    """Lengths and marks that no plan leaves behind: rows without a slot, and nothing outside of the arrays."""
+    most = 2 ** 31 - 1
+    for marks, length in (([-5, 3, 0], [0, 0]), ([2 ** 40 + 1, 2 ** 50, 0], [5, 0]), ([0, 4, 0], [most, -3]),
+                          ([9, 2, 0], [most, most]), ([-2 ** 62, 2 ** 62, 0], [17, most])):
+        table = torch.full((2, 3), -1, dtype=torch.int32, device=DEV)
+        ring = torch.arange(4, dtype=torch.int32, device=DEV)
+        as_int = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+        plan = ec().plan_rows(as_int(length), as_int([40, 60]), table, ring,
+                              torch.tensor(marks, dtype=torch.int64, device=DEV), page_rows=16, rows=100)
+        assert int(plan.slot.min()) >= -1 and int(plan.slot.max()) < 4 * 16
+        got = plan.slot[plan.slot >= 0]
+        assert got.unique().numel() == got.numel()
+        assert plan.start.tolist() == [0, 40, 100] and plan.episode.tolist() == [0] * 40 + [1] * 60
+        assert int(plan.length.min()) >= 0 and int(table.min()) >= -1 and int(table.max()) < 4
+
+
 def test_plan_nothing_new():
     length, new, table, ring, marks, _ = _plan_case(5, 32, 8, 90, seed=1)
     t = _tensors(length, [0] * 5, table, ring, marks)
@@ -399,6 +416,15 @@ def test_attend_scale_and_large_scores(extra_width):
     c = pages_for([3, 200], [90, 50], 4, 2, 64, seed=8, extra_width=extra_width)
     _check_attend(c, scale=0.0)
     _check_attend(c, scale=-0.2)
+
+
+@WIDTHS
+def test_attend_into_its_queries(extra_width):
+    c = pages_for([40, 3, 150], [700, 2000, 90], 8, 2, 128, page=32, seed=21, extra_width=min(extra_width, 100000))
+    apart = ec().attend(**c, max_rows=150, window=500, sinks=3)
+    q = c.pop("q").clone()
+    assert ec().attend(q, **c, max_rows=150, window=500, sinks=3, out=q) is q
+    assert torch.equal(q, apart)
 
 
 def test_attend_long_cache_and_far_pages():
