@@ -1,13 +1,21 @@
-// Attention of new rows over the paged episode cache (include/mkx_cache.h).
+// Attention of new rows over the paged episode cache (include/mkx_cache.h), in one pass over the keys:
+// with m the running maximum of a row's scores (in powers of two), l the sum of 2^(s - m) and o the sum
+// of 2^(s - m) v, a larger maximum m' scales l and o by 2^(m - m'), and the row is o / l at the end; the
+// same rule joins the parts of a row that different warps or blocks took. m, l, o are fp32 throughout.
+// Two kernels, chosen by chunk_is_faster; the work of a call is one line of key blocks that the blocks of
+// the grid share evenly, however many episodes of whatever lengths there are (find_line, Walk).
 //
 // rows_kernel: tiles of 16 rows (new row x head of the group that shares a K/V head). With few rows a
 // call is bound by reading the pages: one producer warp keeps a ring of K/V blocks in flight by TMA (one
 // box per page, 128-byte swizzle, pages that no row sees read as zero without touching memory), four
-// warps each take a quarter of a block's keys with mma.sync m16n8k16 and keep their own running
-// maximum and sum, joined once at the end; long caches are split over blocks (find_share), the last
-// part to finish joins the tile in the order of the parts. The probabilities enter the second product
-// as the sum of two 16-bit words, so that it is as exact as fp32 weights; the tensor pipe is idle
-// enough for that here.
+// warps each take a quarter of a block's keys with mma.sync m16n8k16 (tcgen05 needs 128 rows to a tile,
+// of which a single row of 4 heads would fill 4) and keep their own running maximum and sum, joined once
+// at the end; long caches are split over blocks, the last part to finish joins the tile in the order of
+// the parts. The probabilities enter the second product as the sum of two 16-bit words, so that it is
+// as exact as fp32 weights; the tensor pipe is idle enough for that here.
+// Two blocks per SM with three stages each. 96 single rows after 4,170 rows each, 32/8 heads x 128
+// (1641 MB): 268 us, 6.1 TB/s; 10 rows of 128 episodes of 470, 12 heads x 64, not causal (192 MB): 43 us, 4.5 TB/s
+// -- 3 us to the first bytes, and stretches end up to 10 % apart, since the SMs get unequal shares of HBM.
 #include <cmath>
 #include <cstdint>
 #include <cstring>
@@ -27,7 +35,9 @@ constexpr int MAX_KEYS = 1 << 30;  // rows of an episode: keys and positions are
 constexpr int ROW_WARPS = 4;
 constexpr int ROW_THREADS = 32 * (ROW_WARPS + 1);
 constexpr int ROW_STAGES = 3;
-constexpr int JOIN_AT_ONCE = 12;  // parts that one block joins; more in two levels
+constexpr int JOIN_AT_ONCE = 12;      // parts that one block joins; more in two levels
+constexpr int ROWS_JOIN_AT_ONCE = 26;  // the same where a part has 16 rows: below it the second level costs more than it saves
+                                      // (17 to 26 parts: 13.3 against 14.5 us; 37: 20.8 against 18.4 us)
 
 template <int HD>
 struct RowShape {
@@ -342,10 +352,6 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
       auto add_up = [&](int first, int step, int count) {
         if (r > r1) return;
         mx = -INFINITY;
-        for (int k = 0; k < count; ++k)
-          mx = fmaxf(mx, __ldcg(reinterpret_cast<const float2*>(
-                             p.parts + (size_t)part_place(sg, first + k * step) * PART + MT * HD) + row).x);
-        const float safe = mx == -INFINITY ? 0.f : mx;
         ls = 0.f;
 #pragma unroll
         for (int quarter = 0; quarter < 4; ++quarter)
@@ -355,21 +361,22 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
         for (int k = 0; k < count; ++k) {
           const float* at = p.parts + (size_t)part_place(sg, first + k * step) * PART;
           const float2 t = __ldcg(reinterpret_cast<const float2*>(at + MT * HD) + row);
-          const float w = ex2(t.x - safe);
-          ls += w * t.y;
+          const float top = fmaxf(mx, t.x), safe = top == -INFINITY ? 0.f : top, fix = ex2(mx - safe), w = ex2(t.x - safe);
+          mx = top;
+          ls = ls * fix + w * t.y;
 #pragma unroll
           for (int quarter = 0; quarter < 4; ++quarter)
 #pragma unroll
             for (int d = 0; d < D; d += 2) {
               const float2 v = __ldcg(reinterpret_cast<const float2*>(at + row * HD + quarter * (HD / 4) + q * D + d));
-              acc[quarter][d] += w * v.x;
-              acc[quarter][d + 1] += w * v.y;
+              acc[quarter][d] = acc[quarter][d] * fix + w * v.x;
+              acc[quarter][d + 1] = acc[quarter][d + 1] * fix + w * v.y;
             }
         }
       };
       // many parts are joined in two levels, so that no block reads more than a few
       int step = 1, groups = sg.parts;
-      if (sg.parts > JOIN_AT_ONCE) {
+      if (sg.parts > ROWS_JOIN_AT_ONCE) {
         step = JOIN_AT_ONCE;
         groups = ceil_div(sg.parts, step);
         const int first = (int)(blockIdx.x - sg.lead) / step * step, count = min(step, sg.parts - first);
@@ -402,11 +409,18 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
 // tcgen05 (128-key blocks): S = Q K^T from shared memory into TMEM, O += P V with P read from TMEM and V
 // as TMA left it (dims contiguous). Four warps per tile, one thread per row: no shuffles, the row's
 // maximum and sum stay in registers. O is rescaled only when a maximum has grown by more than 2^8 since the
-// last time, which is rare after the first blocks: P stays below 2^8, far inside both types. At head_dim 128 TMEM is full with two tiles of S and O, and P overwrites the scores it came
-// from: a tile's products wait for its softmax and the other way round, and the two tiles alternate. At
-// head_dim 64 P has columns of its own, and the next scores are there before the last ones are done.
+// last time, which is rare after the first blocks: P stays below 2^8, far inside both types. P is rounded
+// to 16 bits once, as the second product takes no wider weights on tcgen05; the sum l is of the unrounded.
+// At head_dim 128 TMEM is full with two tiles of S and O, and P overwrites the scores it came from: a
+// tile's products wait for its softmax and the other way round, and the two tiles alternate. At head_dim
+// 64 P has columns of its own, and the next scores are there before the last ones are done.
 // Bound by the exponentials at head_dim 64 (16 a clock per SM: 2048 clocks for two 128 x 128 tiles, whose
-// products take 1024), by both alike at 128.
+// products take 1024), by both alike at 128; a quarter of them is taken off that unit (exp2_pair). What is
+// reached is 2950 to 3030 clocks for the two tiles at 128, where the softmax between two products of a
+// tile (load, maximum, exponentials, store) is a chain that the other tile's covers in part.
+// 2011 rows after 6007, 32/8 heads x 128 (231 GFLOP): 222 us by itself, 246 to 253 us in a long run under
+// the power cap (0.92 PFLOP/s); six chunks of 1,000 rows, window 1024 and 70 sinks, 12 heads x 64 (20
+// GFLOP): 64 us.
 constexpr int CT = 256;
 constexpr int CK = 128;
 constexpr int TILE_THREADS = 256;                   // warps 0-3 tile A, 4-7 tile B
@@ -916,7 +930,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         for (int j = 16; j < 128; j += 16)
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            tops[k] = fmaxf(fmaxf(tops[k], __uint_as_float(s[j >> 6][(j & 63) + k])), __uint_as_float(s[j >> 6][(j & 63) + k + 8]));
+            tops[k] = fmaxf(fmaxf(tops[k], __uint_as_float(s[j >> 6][(j & 63) + k])),
+                            __uint_as_float(s[j >> 6][(j & 63) + k + 8]));
         // half of a block's probabilities, as words of P; their sum is added to `sums`
         auto half_of = [&](const uint32_t (&sh)[64], float base, uint32_t (&w)[32], uint64_t (&sums)[4]) {
           const uint64_t base2 = f2(-base, -base);
@@ -1118,6 +1133,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 }
 
 // ---- host ----------------------------------------------------------------------------------------
+// L2 takes in the bytes that a row of one head has, no more: at head_dim 64 with 256 bytes the neighbouring head's
+// row comes along, and may be gone before its block gets there (10 rows of 128 episodes 45.5 instead of 42.8 us, 32
+// single rows after 2000 44.4 instead of 42.3); at 128 with 128 bytes the two halves come apart (16 single rows after
+// 12,500 140.2 instead of 134.7 us).
 bool encode_pages(CUtensorMap* m, const void* base, int dtype, int head_dim, int page_rows, int kv_heads, int pages,
                   long long row, long long head, long long page, int box_rows) {
   EncodeTiledFn fn = tensor_map_encoder();
@@ -1128,7 +1147,8 @@ bool encode_pages(CUtensorMap* m, const void* base, int dtype, int head_dim, int
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   return fn(m, dtype == MKX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
             const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            head_dim == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 struct Plan {
@@ -1150,7 +1170,8 @@ bool chunk_is_faster(const mkx_attend_inputs& a, long long rows) {
   if (a.window > 0 && (double)a.window + a.sinks + a.max_rows < keys) keys = (double)a.window + a.sinks + a.max_rows;
   const double heads = (double)a.B * a.kv_heads, tiles = heads * ((rows + CT - 1) / CT), sms = 148;
   const double by_rows = 8 + heads * ((rows + MT - 1) / MT) * keys * (a.head_dim == 64 ? 59e-6 : 79e-6);
-  const double by_chunk = 25 + tiles / sms * (keys / CK * (a.head_dim == 64 ? 1.43 : 1.7) + 4.5) + (tiles * JOIN_AT_ONCE < sms ? 20 : 0);
+  const double by_chunk = 25 + tiles / sms * (keys / CK * (a.head_dim == 64 ? 1.43 : 1.7) + 4.5) +
+                          (tiles * JOIN_AT_ONCE < sms ? 20 : 0);
   return by_chunk < by_rows;
 }
 

@@ -281,16 +281,16 @@ __device__ __forceinline__ bool others_done(unsigned* ticket, int parts, int* do
   return all;
 }
 // Called by all NTH threads (named barrier 1) after they wrote their part k of a split tile with __stcg: whether
-// this block is the last of the parts [k0, k0 + n) under ticket `ticket`, which is left at zero. The others' parts are
-// then visible through __ldcg.
+// this block is the last of n parts under ticket `ticket`, which is left at zero. The others' parts are then visible
+// through __ldcg: what a block wrote before its barrier is released by the one thread that takes the ticket.
 template <int NTH>
 __device__ __forceinline__ bool last_of(unsigned* ticket, int n, int* last) {
-  __threadfence();
   asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");
   if (threadIdx.x == 0) {
-    *last = atomicAdd(ticket, 1u) == (unsigned)n - 1;
+    unsigned before;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(ticket) : "memory");
+    *last = before == (unsigned)n - 1;
     if (*last) *ticket = 0;
-    __threadfence();
   }
   asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");
   return *last;  // (the word is written again only behind the first barrier of the next call)
