@@ -242,16 +242,13 @@ struct Rates {
   int half;
 };
 
-__device__ __forceinline__ float2 cos_sin(int position, float hi, float lo) {
+__device__ __forceinline__ float turns_of(int position, float hi, float lo) {
   // a position beyond 2^24 is not a float: its low byte is turned apart
   const float a = (float)(position & ~0xff), b = (float)(position & 0xff);
   const float t = a * hi, u = b * hi;
   float r = (t - rintf(t)) + fmaf(a, hi, -t) + a * lo;
   r += (u - rintf(u)) + fmaf(b, hi, -u) + b * lo;
-  r -= rintf(r);
-  float s, c;
-  sincospif(2.f * r, &s, &c);
-  return make_float2(c, s);
+  return r - rintf(r);
 }
 
 __global__ void __launch_bounds__(256) tables_kernel(const __grid_constant__ Rates rates, const int* positions,
@@ -266,7 +263,7 @@ __global__ void __launch_bounds__(256) tables_kernel(const __grid_constant__ Rat
     float2 cs = make_float2(1.f, 0.f);
     int d0 = 2 * f, d1 = 2 * f + 1;  // passing dims 2 half ..
     if (f < rates.half) {
-      cs = cos_sin(positions[rates.axis[f] * pos_stride + row], rates.hi[f], rates.lo[f]);
+      sincospif(2.f * turns_of(positions[rates.axis[f] * pos_stride + row], rates.hi[f], rates.lo[f]), &cs.y, &cs.x);
       d0 = f;
       d1 = f + rates.half;
     }
@@ -280,17 +277,17 @@ __global__ void __launch_bounds__(256) tables_kernel(const __grid_constant__ Rat
 // ---- storing -------------------------------------------------------------------------------------
 // A thread takes 8 dims and their 8 partners (16-byte accesses) of a row for up to HG heads of one of
 // q, k, v, and forms the 8 angles once for those heads. Bound by HBM: every row is read and written
-// once; the angles are about 25 instructions each, spread over HG heads. 30,011 rows of 32 + 8 + 8
-// heads x 128 (738 MB): 123 to 127 us, 5.8 to 6.0 TB/s; 4096 rows of 3 x 12 heads x 64: 8.8 us.
-// The bound of 64 registers (four blocks an SM): 128 and 10.0 us without it, 179 and 13.5 us with 48
-// registers, 500 to 16,000 rows level. HG, measured without the bound: 2 heads 174 us, 4 heads 128,
-// 8 heads 123, but then 16,000 rows of 3 x 12 heads take 38.6 us where 4 heads take 31 to 32.
+// once. The angles are reduced as above, and within half a turn __cosf and __sinf are off by 2^-21 at
+// most, 2^9 times finer than half a step of fp16; with sincospif, 20 more instructions an angle and 74
+// registers, the same calls take 128 instead of 118 us (30,011 rows of 32 + 8 + 8 heads x 128, 738 MB: 6.2
+// TB/s) and 10.0 instead of 8.2 (4096 rows of 3 x 12 heads x 64). With 8 heads (132 registers) they take 162 and
+// 14.1 us; 2 heads and sincospif, 174 and 11.3.
 constexpr int HG = 4;
 
 template <int DT>
-__global__ void __launch_bounds__(256, 4) store_kernel(const __grid_constant__ mkx_store_inputs p,
-                                                       const __grid_constant__ Rates rates, int shift, int groups_q,
-                                                       int groups_k) {
+__global__ void __launch_bounds__(256) store_kernel(const __grid_constant__ mkx_store_inputs p,
+                                                    const __grid_constant__ Rates rates, int shift, int groups_q,
+                                                    int groups_k) {
   const int lanes = p.head_dim / 16;
   const int per_row = (groups_q + 2 * groups_k) * lanes;
   const long long n = (long long)p.rows * per_row;
@@ -325,7 +322,7 @@ __global__ void __launch_bounds__(256, 4) store_kernel(const __grid_constant__ m
     const int h0 = group * HG, nh = min(HG, heads - h0);
     const bool turns = what != 2 && p.positions && 8 * c < rates.half;
     // dims of this lane: 8 c and their partners, or 16 dims side by side where nothing turns
-    // (the condition is that of `turns`; by that name 76 instead of 40 bytes of registers spill: 145 us for 125)
+    // (the condition of `turns` in full: by that name it costs 13 registers, 125 instead of 118 us)
     int d0 = 16 * c, d1 = 16 * c + 8;
     if (what != 2 && p.positions && 8 * c < rates.half) {
       d0 = 8 * c;
@@ -344,9 +341,10 @@ __global__ void __launch_bounds__(256, 4) store_kernel(const __grid_constant__ m
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int f = 8 * c + j;
-        const float2 t = cos_sin(p.positions[rates.axis[f] * p.pos_stride + row], rates.hi[f], rates.lo[f]);
-        cs[j] = t.x;
-        sn[j] = t.y;
+        const float angle =
+            6.283185307f * turns_of(p.positions[rates.axis[f] * p.pos_stride + row], rates.hi[f], rates.lo[f]);
+        cs[j] = __cosf(angle);
+        sn[j] = __sinf(angle);
       }
 #pragma unroll
       for (int h = 0; h < HG; ++h)
