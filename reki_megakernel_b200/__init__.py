@@ -7,7 +7,8 @@ CPU fallback.
 from .synthetic import ExpertDims, ExpertWeights, StepInputs, make_inputs, make_model, make_past, make_weights
 
 __all__ = ["ExpertDims", "ExpertWeights", "StepInputs", "make_inputs", "make_model", "make_past", "make_weights",
-           "ExpertMegakernel", "install", "RegisterPrepare", "register_prepare"]
+           "ExpertMegakernel", "install", "RegisterPrepare", "register_prepare",
+           "EpisodeCache", "plan_rows", "write_rows", "rope_tables", "attend"]
 
 
 def __getattr__(name):
@@ -17,4 +18,7 @@ def __getattr__(name):
     if name in ("RegisterPrepare", "register_prepare"):
         from . import prepare
         return getattr(prepare, name)
+    if name in ("EpisodeCache", "plan_rows", "write_rows", "rope_tables", "attend"):
+        from . import episode_cache
+        return getattr(episode_cache, name)
     raise AttributeError(name)
