@@ -50,6 +50,15 @@ struct RowShape {
   static constexpr int SMEM = ROW_STAGES * STAGE + ROW_WARPS * MT * (JOIN * 4 + 8) + MT * QROW + 1024 + 128;
 };
 
+// log2 of what fp16 probabilities are multiplied by (sums and totals alike, so it drops out at the end): below 2^-24 fp16
+// ends, and many keys that far under one high one (a first row that everything looks at) weigh something together. 2^15,
+// the most that fits, where the largest is 1; in chunks it may be 2^8. What is lost of a key is then below 2^-32 of the
+// largest weight, without a cost. bf16 has the exponents of fp32.
+template <int DT>
+constexpr float ROWS_LIFT = DT == MKX_FP16 ? 15.f : 0.f;
+template <int DT>
+constexpr float CHUNK_LIFT = DT == MKX_FP16 ? 7.f : 0.f;
+
 template <int DT>
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (DT == MKX_BF16)
@@ -253,7 +262,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
         const float now = fmaxf(m[x], top[x]), safe = now == -INFINITY ? 0.f : now;
         fix[x] = ex2(m[x] - safe);
         m[x] = now;
-        top[x] = safe;
+        top[x] = safe - ROWS_LIFT<DT>;
         l[x] *= fix[x];
       }
 #pragma unroll
@@ -409,7 +418,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
 // tcgen05 (128-key blocks): S = Q K^T from shared memory into TMEM, O += P V with P read from TMEM and V
 // as TMA left it (dims contiguous). Four warps per tile, one thread per row: no shuffles, the row's
 // maximum and sum stay in registers. O is rescaled only when a maximum has grown by more than 2^8 since the
-// last time, which is rare after the first blocks: P stays below 2^8, far inside both types. P is rounded
+// last time, which is rare after the first blocks: P stays below 2^8 (2^15 as lifted), inside both types. P is rounded
 // to 16 bits once, as the second product takes no wider weights on tcgen05; the sum l is of the unrounded.
 // At head_dim 128 TMEM is full with two tiles of S and O, and P overwrites the scores it came from: a
 // tile's products wait for its softmax and the other way round, and the two tiles alternate. At head_dim
@@ -974,10 +983,11 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           l *= fix;
           m = now;
         }
-        half_of(s[0], m == -INFINITY ? 0.f : m, w, sums);
+        const float base = (m == -INFINITY ? 0.f : m) - CHUNK_LIFT<DT>;
+        half_of(s[0], base, w, sums);
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-          if (part == 1) half_of(s[1], m == -INFINITY ? 0.f : m, w, sums);
+          if (part == 1) half_of(s[1], base, w, sums);
           tmem_st32(pt + 32 * part, w);
           tmem_wait_st();
           tmem_fence_before();

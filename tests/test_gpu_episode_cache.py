@@ -418,6 +418,34 @@ def test_attend_scale_and_large_scores(extra_width):
     _check_attend(c, scale=-0.2)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("drop", [8, 13, 18])
+def test_attend_many_small_weights(drop, new, dtype):
+    """One key far above all others: weights of e^-drop (e^-18 < 2^-25, half the smallest fp16), which count together.
+    Half a step of the output and of each weight, 2^-12 for scores and exponentials, and 2^-32 of |v| < 6 for each key:
+    weights enter 2^7 times as large or more, so that fp16's 2^-25 is 2^-32 of the largest."""
+    c = pages_for([new], [20000], 4, 1, 64, page=64, dtype=dtype, seed=3)
+    here = c["table"][0][:-(-(20000 + new) // 64)].long()
+    k, v = (c[name][here].flatten(0, 1) for name in ("k_pages", "v_pages"))
+    k[:20000 + new] = 0.0
+    k[0, :, 0] = 1.0
+    v[:20000 + new] = v[:20000 + new].abs() + 0.5
+    v[0] = 0.0
+    c["k_pages"][here], c["v_pages"][here] = k.view(-1, 64, 1, 64), v.view(-1, 64, 1, 64)
+    c["q"].zero_()
+    c["q"][..., 0] = float(drop)
+    # 400 such episodes on the same pages: more tiles than blocks, so that stretches of keys stay long
+    ref, weight = (x.repeat(400, 1, 1) for x in attend_oracle(**c, scale=1.0))
+    c["q"], c["table"], c["length"] = c["q"].repeat(400, 1, 1), c["table"].repeat(400, 1), c["length"].repeat(400)
+    c["start"] = torch.arange(401, dtype=torch.int32, device=DEV) * new
+    got = ec().attend(**c, max_rows=new, scale=1.0)
+    u = torch.finfo(dtype).eps / 2
+    tol = u * ref.abs() + (u + 2.0 ** -12) * weight + 20041 * 2.0 ** -32 * 6
+    err = (got.double() - ref).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
 @WIDTHS
 def test_attend_into_its_queries(extra_width):
     c = pages_for([40, 3, 150], [700, 2000, 90], 8, 2, 128, page=32, seed=21, extra_width=min(extra_width, 100000))
