@@ -26,7 +26,7 @@ SOURCES = [PKG / "csrc" / "mk_expert.cu", PKG / "csrc" / "mk_prepare.cu", PKG / 
            PKG / "csrc" / "mk_batch.cu", PKG / "csrc" / "mk_copies.cu", PKG / "csrc" / "mk_cache.cu",
            PKG / "csrc" / "mk_attend.cu"]
 HEADERS = [PKG / "csrc" / "mkx_device.cuh", PKG / "csrc" / "mkx_tma.cuh", PKG / "csrc" / "mkx_half.cuh",
-           PKG / "csrc" / "mkx_attend.cuh", PKG / "csrc" / "mkx_pdl.cuh", PKG / "csrc" / "mkx_cache_host.h", ROOT / "include" / "mkx.h",
+           PKG / "csrc" / "mkx_attend.cuh", PKG / "csrc" / "mkx_join.h", PKG / "csrc" / "mkx_pdl.cuh", PKG / "csrc" / "mkx_cache_host.h", ROOT / "include" / "mkx.h",
            ROOT / "include" / "mkx_prepare.h", ROOT / "include" / "mkx_mods.h", ROOT / "include" / "mkx_batch.h",
            ROOT / "include" / "mkx_cache.h"]
 # The episode cache's entry points for torch tensors (host code; reaches libmkx.so by address).

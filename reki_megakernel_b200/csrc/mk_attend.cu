@@ -114,7 +114,8 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
     fence_mbar_init();
   }
   __shared__ LineScratch scratch;
-  __shared__ int flag;
+  __shared__ JoinWords words;
+  const BarrierTeam<32 * ROW_WARPS> team;
   Line line;
   pdl_begin();
   if (!find_line<MT, KT, ROW_THREADS>(p, scratch, line)) return;  // its barriers publish the mbarriers too
@@ -389,12 +390,12 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
         step = JOIN_AT_ONCE;
         groups = ceil_div(sg.parts, step);
         const int first = (int)(blockIdx.x - sg.lead) / step * step, count = min(step, sg.parts - first);
-        if (!last_of<32 * ROW_WARPS>(p.tickets + p.slots + part_place(sg, first), count, &flag)) continue;
+        if (!last_of(team, p.tickets + p.slots + part_place(sg, first), count, words)) continue;
         add_up(first, 1, count);
         row_barrier();  // the group's first part has been read: the group's sums take its place
         keep(first);
       }
-      if (!last_of<32 * ROW_WARPS>(p.tickets + sg.lead, groups, &flag)) continue;
+      if (!last_of(team, p.tickets + sg.lead, groups, words)) continue;
       add_up(0, step, groups);
     }
     if (r <= r1) {
@@ -626,7 +627,7 @@ struct ChunkShared {
   uint64_t turns[2];     // the MMA warps' turns
   uint64_t jfull[JOBS], jempty[JOBS];
   uint32_t tmem;
-  int flag;
+  JoinWords words;
   Job jobs[JOBS];
 };
 static_assert(sizeof(ChunkShared<128>) <= 227 * 1024, "one block's shared memory");
@@ -866,6 +867,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t st = tmem + lanes + S::s_at(x), ot = tmem + lanes + S::o_at(x), pt = tmem + lanes + S::p_at(x);
     const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
+    const BarrierTeam<TILE_THREADS> team;
     int n = 0;  // blocks of this tile since the start
     // After a wait that ran out the warp goes on without waiting: others of its barriers still count on it
     bool ok = true;
@@ -1094,7 +1096,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       int step = 1, groups = sg.parts, mine = -1;
       if (sg.parts > JOIN_AT_ONCE)
         while (step * step < sg.parts) ++step;
-      if (step == 1 && others_done<TILE_THREADS>(p.tickets + sg.lead, sg.parts, &sm.flag)) {
+      if (step == 1 && others_done(team, p.tickets + sg.lead, sg.parts, sm.words)) {
         mine = own;
       } else {
 #pragma unroll
@@ -1106,7 +1108,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         if (r <= r1) __stcg(ml_at(own), make_float2(m, l));
         if (step > 1) {
           const int first = own / step * step, count = min(step, sg.parts - first);
-          if (!last_of<TILE_THREADS>(p.tickets + p.slots + part_place(sg, first), count, &sm.flag)) {
+          if (!last_of(team, p.tickets + p.slots + part_place(sg, first), count, sm.words)) {
             tmem_fence_before();
             continue;
           }
@@ -1118,7 +1120,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           }
           groups = ceil_div(sg.parts, step);
         }
-        if (!last_of<TILE_THREADS>(p.tickets + sg.lead, groups, &sm.flag)) {
+        if (!last_of(team, p.tickets + sg.lead, groups, sm.words)) {
           tmem_fence_before();
           continue;
         }

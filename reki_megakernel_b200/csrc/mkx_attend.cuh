@@ -7,6 +7,7 @@
 #include "mkx_cache.h"
 #include "mkx_device.cuh"
 #include "mkx_half.cuh"
+#include "mkx_join.h"
 #include "mkx_tma.cuh"
 
 namespace mkxa {
@@ -266,35 +267,23 @@ struct Walk {
 // A block keeps at most two parts: of the tile its stretch begins inside of, and of the one it ends inside of.
 __device__ __forceinline__ int part_place(const Segment& s, int k) { return 2 * (s.lead + k) + (k == 0); }
 
-// Whether the other parts - 1 blocks of a tile have all delivered: then this one keeps its part to itself, and joins.
-// Called by all NTH threads (named barrier 1); leaves the ticket at zero if so. The others' parts are then visible
-// through __ldcg.
+// The threads of a block that join tiles, by named barrier 1 (see mkx_join.h).
 template <int NTH>
-__device__ __forceinline__ bool others_done(unsigned* ticket, int parts, int* done) {
-  if (threadIdx.x == 0) {
-    *done = ld_acquire_i32(reinterpret_cast<int*>(ticket)) == parts - 1;
-    if (*done) *ticket = 0;
+struct BarrierTeam {
+  __device__ __forceinline__ bool leads() const { return threadIdx.x == 0; }
+  __device__ __forceinline__ void meet() const { asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory"); }
+  __device__ __forceinline__ bool read(const int* word) const { return *word != 0; }
+  __device__ __forceinline__ void write(int* word, bool v) const { *word = v; }
+  __device__ __forceinline__ unsigned held(const unsigned* ticket) const {
+    return (unsigned)ld_acquire_i32(reinterpret_cast<const int*>(ticket));
   }
-  asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");
-  const bool all = *done;
-  asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");  // the word is free again
-  return all;
-}
-// Called by all NTH threads (named barrier 1) after they wrote their part k of a split tile with __stcg: whether
-// this block is the last of n parts under ticket `ticket`, which is left at zero. The others' parts are then visible
-// through __ldcg: what a block wrote before its barrier is released by the one thread that takes the ticket.
-template <int NTH>
-__device__ __forceinline__ bool last_of(unsigned* ticket, int n, int* last) {
-  asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");
-  if (threadIdx.x == 0) {
+  __device__ __forceinline__ unsigned take(unsigned* ticket) const {
     unsigned before;
     asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(ticket) : "memory");
-    *last = before == (unsigned)n - 1;
-    if (*last) *ticket = 0;
+    return before;
   }
-  asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");
-  return *last;  // (the word is written again only behind the first barrier of the next call)
-}
+  __device__ __forceinline__ void clear(unsigned* ticket) const { *ticket = 0; }
+};
 
 // The key blocks of a segment, of `blocks` that its tile really has (its units are those of the episode's longest tile).
 __device__ __forceinline__ int first_block(const Segment& s, int blocks) {
