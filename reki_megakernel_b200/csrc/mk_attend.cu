@@ -82,9 +82,6 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&v)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 __device__ __forceinline__ void row_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * ROW_WARPS) : "memory"); }
 
 extern __shared__ __align__(1024) char asmem[];
@@ -115,7 +112,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
   }
   __shared__ LineScratch scratch;
   __shared__ JoinWords words;
-  const BarrierTeam<32 * ROW_WARPS> team;
+  BarrierTeam<32 * ROW_WARPS> team;
   Line line;
   pdl_begin();
   if (!find_line<MT, KT, ROW_THREADS>(p, scratch, line)) return;  // its barriers publish the mbarriers too
@@ -625,6 +622,7 @@ struct ChunkShared {
   uint64_t ofull[2];     // its sums include them
   uint64_t done;
   uint64_t turns[2];     // the MMA warps' turns
+  uint64_t joins;        // the tiles' warps meet to join
   uint64_t jfull[JOBS], jempty[JOBS];
   uint32_t tmem;
   JoinWords words;
@@ -662,6 +660,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       mbar_init(&sm.turns[x], 1);
     }
     mbar_init(&sm.done, 2);
+    mbar_init(&sm.joins, TILE_THREADS / 32);
     for (int j = 0; j < JOBS; ++j) {
       mbar_init(&sm.jfull[j], 1);
       mbar_init(&sm.jempty[j], 11);  // the producer, the two MMA warps, the eight warps of the tiles
@@ -867,9 +866,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t st = tmem + lanes + S::s_at(x), ot = tmem + lanes + S::o_at(x), pt = tmem + lanes + S::p_at(x);
     const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
-    const BarrierTeam<TILE_THREADS> team;
+    BoundedTeam team(&sm.joins, p.timeout_ns);
     int n = 0;  // blocks of this tile since the start
-    // After a wait that ran out the warp goes on without waiting: others of its barriers still count on it
+    // After a wait that ran out the warp goes on without waiting: others of its barriers still count on it. Where it cannot
+    // go on (no job, nobody to join with), it leaves, and those who count on it run into their own limits.
     bool ok = true;
     auto wait = [&](uint64_t* bar, int parity) {
       ok = ok && __all_sync(0xffffffffu, wait_bounded(bar, (uint32_t)parity, p.timeout_ns)) != 0;
@@ -1099,6 +1099,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       if (step == 1 && others_done(team, p.tickets + sg.lead, sg.parts, sm.words)) {
         mine = own;
       } else {
+        if (!team.ok) break;
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j) {
           float o[32];
@@ -1110,6 +1111,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           const int first = own / step * step, count = min(step, sg.parts - first);
           if (!last_of(team, p.tickets + p.slots + part_place(sg, first), count, sm.words)) {
             tmem_fence_before();
+            if (!team.ok) break;
             continue;
           }
           if (__any_sync(0xffffffffu, r <= r1)) {
@@ -1122,6 +1124,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         }
         if (!last_of(team, p.tickets + sg.lead, groups, sm.words)) {
           tmem_fence_before();
+          if (!team.ok) break;
           continue;
         }
       }
@@ -1133,7 +1136,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       }
       tmem_fence_before();
     }
-    if (!ok && lane == 0) atomicCAS(p.error, 0, 0x214);
+    if (!(ok && team.ok) && lane == 0) atomicCAS(p.error, 0, 0x214);
     tmem_fence_before();
   }
   __syncthreads();

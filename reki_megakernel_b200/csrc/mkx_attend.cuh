@@ -267,11 +267,10 @@ struct Walk {
 // A block keeps at most two parts: of the tile its stretch begins inside of, and of the one it ends inside of.
 __device__ __forceinline__ int part_place(const Segment& s, int k) { return 2 * (s.lead + k) + (k == 0); }
 
-// The threads of a block that join tiles, by named barrier 1 (see mkx_join.h).
-template <int NTH>
-struct BarrierTeam {
+// What the teams of both kernels share (see mkx_join.h).
+struct TicketTeam {
+  bool ok = true;
   __device__ __forceinline__ bool leads() const { return threadIdx.x == 0; }
-  __device__ __forceinline__ void meet() const { asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory"); }
   __device__ __forceinline__ bool read(const int* word) const { return *word != 0; }
   __device__ __forceinline__ void write(int* word, bool v) const { *word = v; }
   __device__ __forceinline__ unsigned held(const unsigned* ticket) const {
@@ -283,6 +282,14 @@ struct BarrierTeam {
     return before;
   }
   __device__ __forceinline__ void clear(unsigned* ticket) const { *ticket = 0; }
+};
+// NTH threads that all walk the same line to its end, whatever runs out on the way: named barrier 1.
+template <int NTH>
+struct BarrierTeam : TicketTeam {
+  __device__ __forceinline__ bool meet() const {
+    asm volatile("bar.sync 1, %0;" ::"n"(NTH) : "memory");
+    return true;
+  }
 };
 
 // The key blocks of a segment, of `blocks` that its tile really has (its units are those of the episode's longest tile).
@@ -360,6 +367,9 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, unsigned long long limit) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer();
@@ -367,5 +377,21 @@ __device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, uns
     if (globaltimer() - t0 > limit) return false;
   return true;
 }
+
+// Warps of which one may leave early, after a wait that ran out: an mbarrier that counts them, waited for with a limit.
+// `met` says at which of its phases the warp is; none is ahead by more than one, since a phase needs them all.
+struct BoundedTeam : TicketTeam {
+  uint64_t* bar;
+  unsigned long long limit;
+  uint32_t met = 0;
+  __device__ __forceinline__ BoundedTeam(uint64_t* barrier, unsigned long long timeout) : bar(barrier), limit(timeout) {}
+  __device__ __forceinline__ bool meet() {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+    ok = __all_sync(0xffffffffu, wait_bounded(bar, met & 1, limit)) != 0;
+    ++met;
+    return ok;
+  }
+};
 
 }  // namespace mkxa

@@ -1,5 +1,5 @@
 """The exchange between blocks that share a tile (csrc/mkx_join.h), run on the host: threads stand for the warps of a
-block, and one of them is late on its way to every word that it reads."""
+block, and one of them is late on its way to every word that it reads, or leaves."""
 import shutil
 import subprocess
 
@@ -17,27 +17,34 @@ SOURCE = r"""
 #include "mkx_join.h"
 
 constexpr int WARPS = 8;
+#ifndef GONE
+#define GONE 99  // the warp that leaves: none
+#define LIMIT_MS 20000
+#else
+#define LIMIT_MS 10
+#endif
 struct Barrier {
   std::mutex m;
   std::condition_variable cv;
   int come = 0, phase = 0;
-  void wait() {
+  bool wait() {
     std::unique_lock<std::mutex> l(m);
     const int now = phase;
     if (++come == WARPS) {
       come = 0;
       ++phase;
       cv.notify_all();
-    } else {
-      cv.wait(l, [&] { return phase != now; });
+      return true;
     }
+    return cv.wait_for(l, std::chrono::milliseconds(LIMIT_MS), [&] { return phase != now; });
   }
 };
 struct Team {
   Barrier* barrier;
   int warp, late;
+  bool ok = true;
   bool leads() const { return warp == 0; }
-  void meet() const { barrier->wait(); }
+  bool meet() { return ok = barrier->wait(); }
   bool read(const int* w) const {
     if (warp == late) std::this_thread::sleep_for(std::chrono::milliseconds(4));
     return __atomic_load_n(w, __ATOMIC_SEQ_CST) != 0;
@@ -68,14 +75,19 @@ int main() {
       for (int w = 0; w < WARPS; ++w)
         warps.emplace_back([&, w] {
           Team team{&barrier, w, late};
+          if (w == GONE) return;  // before the first question
           for (int i = 0; i < 3; ++i) {
             const bool yes = kind[i] ? mkxa::others_done(team, &tickets[i], 2, words) : mkxa::last_of(team, &tickets[i], 2, words);
+            if (GONE < WARPS) {  // nobody hears yes, and everybody learns that somebody is missing
+              bad[w] += yes || team.ok;
+              return;
+            }
             bad[w] += yes != (there[i] == 1);
           }
         });
       for (auto& t : warps) t.join();
       for (int b : bad) wrong += b;
-      for (int i = 0; i < 3; ++i) wrong += tickets[i] != (there[i] ? 0u : kind[i] ? 0u : 1u);
+      for (int i = 0; i < 3 && GONE >= WARPS; ++i) wrong += tickets[i] != (there[i] ? 0u : kind[i] ? 0u : 1u);
     }
   printf("%d\n", wrong);
   return 0;
@@ -102,3 +114,20 @@ def test_one_word_for_both_questions_is_not_enough(tmp_path):
     """The same with both answers in one word: others_done writes before its first meeting, while a late warp still reads
     last_of's answer. (Shows that the test above sees it.)"""
     assert _wrong(tmp_path, "-DONE_WORD") > 0
+
+
+@pytest.mark.parametrize("gone", [0, 5])
+def test_a_warp_that_left_is_not_waited_for(gone, tmp_path):
+    """A warp gave up before the first question (the one that asks, or another): the others come back within their limit,
+    with a no, and know that the answer is none."""
+    assert _wrong(tmp_path, f"-DGONE={gone}") == 0
+
+
+def test_no_unbounded_barrier_among_warps_that_may_leave():
+    """In the kernel of chunks a warp may leave its role early; between the roles' start and their common end nothing but
+    mbarriers with a limit is waited for."""
+    text = (ROOT / "reki_megakernel_b200" / "csrc" / "mk_attend.cu").read_text()
+    body = text[text.index("chunk_kernel(const __grid_constant__"):text.index("// ---- host ---")]
+    roles = body[body.index("if (warp >= 8) {"):body.rindex("__syncthreads();")]
+    assert "__syncthreads" not in roles and "bar.sync" not in roles and "BarrierTeam" not in roles and "row_barrier" not in roles
+    assert "BoundedTeam" in roles
