@@ -114,6 +114,7 @@ mkx_status mkx_cache_store(const mkx_store_inputs* in, int device, cudaStream_t 
  * and zero where a row sees nothing. Sums, maxima and outputs are held in fp32 and rounded once; what a
  * K/V page holds beyond an episode's length, and pages that no row sees, do not matter, whatever they
  * hold; K and V rows below the length are finite. Table entries outside 0 .. pages - 1 read as zero rows.
+ * A row of a head that sees a score of NaN or +inf, or only scores of -inf, is NaN there.
  * Rows behind start[B] are left as they were. head_dim 64 or 128; window > 0 only with causal.
  * max_rows: no episode has more new rows in this call (more: those behind are left as they were).
  *

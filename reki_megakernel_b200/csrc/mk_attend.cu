@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
       const int t = by_group(p, r);
       char* out = (char*)p.out + 2 * ((long long)(sg.first_row + t) * p.o_row +
                                       (long long)(sg.kvh * p.group + r - t * p.group) * p.o_head + q * D);
-      const float inv = ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls);  // nothing seen: zero; NaN stays
+      const float inv = over_total(p, sg.first_row + t, ls);
 #pragma unroll
       for (int quarter = 0; quarter < 4; ++quarter)
 #pragma unroll
@@ -936,13 +936,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         }
         float tops[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) tops[k] = fmaxf(__uint_as_float(s[0][k]), __uint_as_float(s[0][k + 8]));
+        for (int k = 0; k < 8; ++k) tops[k] = max_nan(__uint_as_float(s[0][k]), __uint_as_float(s[0][k + 8]));
 #pragma unroll
         for (int j = 16; j < 128; j += 16)
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            tops[k] = fmaxf(fmaxf(tops[k], __uint_as_float(s[j >> 6][(j & 63) + k])),
-                            __uint_as_float(s[j >> 6][(j & 63) + k + 8]));
+            tops[k] = max_nan(tops[k], __uint_as_float(s[j >> 6][(j & 63) + k]), __uint_as_float(s[j >> 6][(j & 63) + k + 8]));
         // half of a block's probabilities, as words of P; their sum is added to `sums`
         auto half_of = [&](const uint32_t (&sh)[64], float base, uint32_t (&w)[32], uint64_t (&sums)[4]) {
           const uint64_t base2 = f2(-base, -base);
@@ -963,8 +962,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         uint32_t w[32];
         uint64_t sums[4] = {0, 0, 0, 0};
         const float top = p.scale_log2 *  // > 0: -inf stays
-                          fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
-                                fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
+                          max_nan(max_nan(tops[0], tops[1], tops[2]), max_nan(tops[3], tops[4], tops[5]), max_nan(tops[6], tops[7]));
         const bool grow = top > m + LAZY || (m == -INFINITY && top > m);
         const bool any_grow = __any_sync(0xffffffffu, grow);
         if ((S::EARLY || any_grow) && n > n0) {  // the last V product: read P (EARLY) and wrote O
@@ -985,6 +983,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           l *= fix;
           m = now;
         }
+        // a score that is NaN or infinite makes the row NaN (exp2_pair would take it for a weight of zero)
+        if (!(top < INFINITY)) l = __int_as_float(0x7fffffff);
         const float base = (m == -INFINITY ? 0.f : m) - CHUNK_LIFT<DT>;
         half_of(s[0], base, w, sums);
 #pragma unroll
@@ -1012,7 +1012,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       if (lane == 0) mbar_arrive(&sm.jempty[jn % JOBS]);
       char* out = (char*)p.out + 2 * ((long long)(sg.first_row + t) * p.o_row +
                                       (long long)(sg.kvh * p.group + r - t * p.group) * p.o_head);
-      auto scale_of = [](float ls) { return ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls); };  // nothing seen: zero; NaN stays
+      auto scale_of = [&](float ls) { return over_total(p, sg.first_row + t, ls); };
       auto write = [&](const float (&o)[32], int j, float inv) {
 #pragma unroll
         for (int d = 0; d < 32; d += 8)
@@ -1030,11 +1030,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         for (int d = 0; d < 32; ++d) o[d] = __uint_as_float(u[d]);
       };
       if (sg.parts == 1) {
+        const float inv = r <= r1 ? scale_of(l) : 0.f;
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j) {
           float o[32];
           sums_of(j, o);
-          if (r <= r1) write(o, j, scale_of(l));
+          if (r <= r1) write(o, j, inv);
         }
         tmem_fence_before();
         continue;

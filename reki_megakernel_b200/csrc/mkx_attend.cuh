@@ -340,6 +340,25 @@ __device__ __forceinline__ uint32_t seen_mask(const AttendParams& p, const Keys&
   if (p.window) m &= ~below(position - p.window + 1 - key0) | below(p.sinks - key0);
   return m;
 }
+// Whether new row `row` of the call sees any key.
+__device__ __noinline__ bool sees_any(const AttendParams& p, int row) {
+  int b = 0, end = p.B;  // its episode: the last one that starts at or before it
+  while (end - b > 1) {
+    const int mid = (b + end) >> 1;
+    if (p.start[mid] <= row) b = mid;
+    else end = mid;
+  }
+  const int length = max(p.length[b], 0), position = length - p.start[b + 1] + row;
+  const int held = (int)min((long long)length, (long long)p.table_width << p.shift);
+  const int hi = p.causal ? min(held, position + 1) : held;
+  return hi > 0 && (!p.window || hi > position - p.window + 1 || p.sinks > 0);
+}
+// What a row's sums are multiplied by, for the total `l` of its weights: zero where nothing is seen. No total although
+// keys are seen means that all their scores are -inf: softmax has no value there, as for NaN or an infinite score. That
+// is rare, so the row's episode and position are looked up again instead of being kept.
+__device__ __forceinline__ float over_total(const AttendParams& p, int row, float l) {
+  return l > 0.f ? 1.f / l : l == 0.f && !sees_any(p, row) ? 0.f : __int_as_float(0x7fffffff);
+}
 // The page that holds keys [page << shift, ..), or -1 (its rows read as zero) where no row sees any.
 __device__ __forceinline__ int page_of(const AttendParams& p, const Keys& k, int b, int page) {
   const int first = page << p.shift;
@@ -354,6 +373,18 @@ __device__ __forceinline__ uint32_t signed_q(const AttendParams& p, uint32_t v) 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The maximum, NaN if one of them is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 

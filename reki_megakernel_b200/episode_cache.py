@@ -277,7 +277,7 @@ def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table:
 
     A row at position p sees the rows j < length[b] of its episode with j <= p (all of them if not ``causal``) and,
     with a ``window`` > 0, with j > p - window or j < ``sinks``. out = softmax(scale q k^T) v (scale: 1 / sqrt(head_dim)),
-    zero for a row that sees nothing; rows behind start[B] are left as they were. ``out`` may be q. What pages hold beyond an
+    zero for a row that sees nothing, NaN where a score is NaN or infinite; rows behind start[B] are left as they were. ``out`` may be q. What pages hold beyond an
     episode's length does not matter; the K and V rows below it are finite. ``max_rows``: no episode has more new rows
     (default: q's rows). The kernel is chosen by ``max_rows`` and by what a table row can hold, so tight values of both
     pick the one that fits. A wait that ran out on the device surfaces in
