@@ -81,9 +81,9 @@ typedef struct {
   int interleaved;
 } mkx_rotary;
 
-/* cos, sin [rows][head_dim] fp32 of positions [axes][rows] int32 (axis stride pos_stride), the layout
- * mkx_prep_run and mkx_run read; dims that pass through get 1 and 0. head_dim a multiple of 16,
- * <= 256. */
+/* cos, sin [rows][head_dim] fp32 of positions [axes][rows] int32 (axis stride pos_stride); dims that pass
+ * through get 1 and 0. head_dim a multiple of 16, <= 256. mkx_prep_run and mkx_run read this layout, but turn
+ * dims i and i + head_dim / 2 together: tables for them have half = head_dim / 2. */
 mkx_status mkx_rope_tables(const mkx_rotary* rot, const int* positions, long long pos_stride, int rows, int head_dim,
                            float* cos, float* sin, int device, cudaStream_t stream);
 

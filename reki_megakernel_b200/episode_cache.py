@@ -154,9 +154,10 @@ def _positions(positions: torch.Tensor, axes: int, rows: int, device) -> torch.T
 
 def rope_tables(positions: torch.Tensor, head_dim: int, *, sections=None, base: float = 10000.0,
                 interleaved: bool = False):
-    """cos, sin [rows, head_dim] fp32 of ``positions`` [axes, rows] (or [rows]) int32, as ``RegisterPrepare.run`` and
-    ``ExpertMegakernel.run`` take them. Frequency i of ``sum(sections)`` (default: one axis, head_dim / 2) belongs to
-    dims i and i + sum(sections); see ``write_rows``."""
+    """cos, sin [rows, head_dim] fp32 of ``positions`` [axes, rows] (or [rows]) int32. Frequency i of ``sum(sections)``
+    (default: one axis, head_dim / 2) belongs to dims i and i + sum(sections), the others get 1 and 0; see ``write_rows``.
+    ``RegisterPrepare.run`` and ``ExpertMegakernel.run`` turn dims i and i + head_dim / 2 together: for them the
+    sections add up to head_dim / 2."""
     dev = _cuda(positions, "positions")
     if not 16 <= head_dim <= 256 or head_dim % 16:
         raise ValueError("head_dim must be a multiple of 16 up to 256")

@@ -36,6 +36,19 @@ def check_run_args(dims, device, S: int, SP: int, cos: torch.Tensor, sin: torch.
                 raise ValueError(f"out {name} must be a contiguous {list(shape)} bf16 tensor on {device}")
 
 
+def check_position_args(dims, positions, cos, sin, sections, interleaved) -> None:
+    """What ``RegisterPrepare.run`` checks of positions. K's dims d and d + HD / 2 turn together, so the sections have to
+    take up all HD / 2 frequencies: with fewer, ``rope_tables`` pairs other dims. Raises ValueError."""
+    if positions is None:
+        if sections is not None or interleaved:
+            raise ValueError("sections belong to positions")
+        return
+    if cos is not None or sin is not None:
+        raise ValueError("give positions or tables, not both")
+    if sections is not None and sum(sections) != dims.HD // 2:
+        raise ValueError(f"sections must add up to {dims.HD // 2}: dims d and d + {dims.HD // 2} turn together")
+
+
 class RegisterPrepare:
     """``RegisterPrepare(weights).run(src) -> (k, v)``, both [L, SP, NH, HD] bf16 on src's device."""
 
@@ -69,16 +82,16 @@ class RegisterPrepare:
             SP: int | None = None, out=None, *, positions: torch.Tensor | None = None, sections=None,
             interleaved: bool = False):
         """K and V of the source rows; their RoPE tables are ``cos`` / ``sin``, or those of ``positions`` [axes, S] int32
-        (time, height, width of image rows: ``episode_cache.rope_tables``), or of the row indexes."""
+        (time, height, width of image rows: ``episode_cache.rope_tables``; ``sections`` add up to HD / 2), or of the row
+        indexes."""
         d = self.dims
+        check_position_args(d, positions, cos, sin, sections, interleaved)
         if src.dim() != 2 or src.shape[1] != d.src_dim or src.dtype != torch.bfloat16 or src.device != self.device:
             raise ValueError(f"src must be [S, {d.src_dim}] bf16 on {self.device}")
         src = src.contiguous()
         S = src.shape[0]
         SP = SP or S
         if positions is not None:
-            if cos is not None or sin is not None:
-                raise ValueError("give positions or tables, not both")
             cos, sin = rope_tables(positions, d.HD, sections=sections, interleaved=interleaved)
         elif cos is None or sin is None:
             cos, sin = self.tables(S)

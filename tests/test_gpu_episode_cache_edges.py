@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from _cache_cases import attend_tolerance, pages_for
-from oracle.cache_oracle import attend_oracle
+from oracle.cache_oracle import angles_oracle, attend_oracle, turn_oracle
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -47,3 +47,37 @@ def test_attend_queries_not_finite(value, window, sinks, hd, extra_width):
     assert (got[blind] == 0).all()
     assert torch.isnan(got[spoilt & ~blind]).all()
     assert bool(((got - ref).abs() <= tol)[~spoilt].all())
+
+
+# ---- rotary geometries ---------------------------------------------------------------------------------
+
+def test_prepare_turns_k_by_its_positions():
+    """K of ``RegisterPrepare.run`` with positions is K without turned by the formula's angles; sections that leave dims out
+    are refused. K without is rounded to bf16 (half a step of each of two terms), K with once more, and the tables are
+    off by 2e-6."""
+    from reki_megakernel_b200.prepare import RegisterPrepare
+    from reki_megakernel_b200.synthetic import ExpertDims, make_prepare_weights, make_source
+    d = ExpertDims(L=1)
+    rp = RegisterPrepare(make_prepare_weights(d, seed=0).to(DEV))
+    src = make_source(70, d.src_dim, seed=1).to(DEV)
+    pos = torch.stack([torch.arange(70) // 35, torch.arange(70) % 35 // 7, torch.arange(70) % 7]).to(torch.int32)
+    plain, v0 = rp.run(src, positions=torch.zeros_like(pos).to(DEV), sections=(8, 12, 12))
+    u = torch.finfo(BF).eps / 2
+    for n, sections, interleaved in ((3, (8, 12, 12), False), (2, (20, 12), True), (1, None, False)):
+        k, v = rp.run(src, positions=pos[:n].to(DEV), sections=sections, interleaved=interleaved)
+        ang = angles_oracle(pos[:n], sections or (32,), interleaved=interleaved)
+        ref = turn_oracle(plain[0], ang)
+        x = plain[0].cpu().double().abs()
+        c, s = ang.cos().abs()[:, None], ang.sin().abs()[:, None]
+        a, b = x[..., :32], x[..., 32:]
+        size = torch.cat([a * c + b * s, b * c + a * s], -1)
+        err = (k[0].cpu().double() - ref).abs()
+        assert bool((err <= u * ref.abs() + (u * (1 + u) + 4e-6) * size).all()), float((err / (u * ref.abs() + u * size)).max())
+        assert torch.equal(v, v0)
+    with pytest.raises(ValueError):
+        rp.run(src, positions=pos[:2].to(DEV), sections=(8, 8))
+    with pytest.raises(ValueError):
+        rp.run(src, sections=(16, 16))
+    torch.cuda.synchronize()
+    rp.check_device_error()
+    rp.close()
