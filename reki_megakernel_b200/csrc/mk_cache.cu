@@ -455,8 +455,11 @@ extern "C" mkx_status mkx_cache_plan(const mkx_plan_inputs* in, int device, cuda
   if (!cuda_ok(scope.err)) return MKX_ERR_CUDA;
   const int sms = sm_count(device);
   if (sms == 0) return MKX_ERR_CUDA;
-  const int smem = 64 + p.B * (int)(sizeof(long long) + sizeof(PlanShared));
-  if (smem > 48 * 1024 && !cuda_ok(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))
+  const auto smem_of = [](int episodes) { return 64 + episodes * (int)(sizeof(long long) + sizeof(PlanShared)); };
+  const int smem = smem_of(p.B);
+  // always the largest size there is: a call's own size might fall below what another thread is about to launch with
+  if (smem > 48 * 1024 && !cuda_ok(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                        smem_of(MKX_MAX_EPISODES))))
     return MKX_ERR_CUDA;
   long long grid = ((long long)p.rows + NT * ROWS_PER_THREAD - 1) / (NT * ROWS_PER_THREAD);
   grid = grid < 1 ? 1 : grid > sms ? sms : grid;

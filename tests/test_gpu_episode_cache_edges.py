@@ -1,5 +1,8 @@
 """Calls of the paged episode cache at its edges: queries that are not finite, parts of split tiles one by one, geometries and
 arguments that are refused, several threads. Oracles as in ``test_gpu_episode_cache.py``."""
+import ctypes as C
+import threading
+
 import pytest
 import torch
 
@@ -81,3 +84,38 @@ def test_prepare_turns_k_by_its_positions():
     torch.cuda.synchronize()
     rp.check_device_error()
     rp.close()
+
+
+# ---- several threads -----------------------------------------------------------------------------------
+
+def test_plans_of_two_threads():
+    """The C ABI from two threads at once (ctypes lets go of Python's lock), both with more episodes than the default shared
+    memory holds, and not as many: no launch fails, and both plans are right."""
+    from reki_megakernel_b200 import _lib
+    lib = _lib.load()
+    failed, starts = [], {}
+
+    def plans(B, times):
+        i32 = dict(dtype=torch.int32, device=DEV)
+        length, new, ring = torch.zeros(B, **i32), torch.ones(B, **i32), torch.arange(B, **i32)
+        table, marks = torch.full((B, 2), -1, **i32), torch.tensor([0, B, 0], dtype=torch.int64, device=DEV)
+        start, slot = torch.zeros(B + 1, **i32), torch.zeros(B, dtype=torch.int64, device=DEV)
+        episode, position, after, marks_after = torch.zeros(B, **i32), torch.zeros(B, **i32), torch.zeros(B, **i32), torch.zeros_like(marks)
+        a = _lib.PlanInputs(*(t.data_ptr() for t in (length, new, table, ring, marks, start, slot, episode, position, after, marks_after)),
+                            None, B, 2, B, 16, B)
+        stream = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        for _ in range(times):
+            if lib.mkx_cache_plan(C.byref(a), 0, stream.cuda_stream):
+                failed.append(B)
+        torch.cuda.synchronize()
+        starts[B] = (start.tolist(), slot.tolist(), marks_after.tolist())
+
+    threads = [threading.Thread(target=plans, args=(B, 4000)) for B in (4096, 2100)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for B in (4096, 2100):
+        assert starts[B] == (list(range(B + 1)), [16 * b for b in range(B)], [B, B, 0])
