@@ -140,6 +140,13 @@ mkx_status mkx_cache_attend(const mkx_attend_inputs* in, size_t workspace_bytes,
 /* Bytes of workspace that a call with these sizes needs (0 for sizes that are refused). */
 size_t mkx_attend_workspace(const mkx_attend_inputs* in, int device);
 
+/* MKX_CACHE_KEY as the library was built with: a number that the build derives from this header. A caller that was built
+ * apart and hands structs over compares it with its own (0: built without). */
+#ifndef MKX_CACHE_KEY
+#define MKX_CACHE_KEY 0ull
+#endif
+unsigned long long mkx_cache_key(void);
+
 /* Last CUDA error string seen by the cache entry points (thread-local, static storage). */
 const char* mkx_cache_last_cuda_error(void);
 

@@ -146,6 +146,7 @@ SIGNATURES = {
     "mkx_cache_attend": (C.c_int, [P, C.c_size_t, C.c_int, P]),
     "mkx_attend_workspace": (C.c_size_t, [P, C.c_int]),
     "mkx_cache_last_cuda_error": (C.c_char_p, []),
+    "mkx_cache_key": (C.c_ulonglong, []),
 }
 
 _LIB = None
@@ -195,22 +196,18 @@ _TORCH = None
 
 
 def load_torch():
-    """The torch binding of the episode cache (``_mkx_torch.so``, built first if missing or stale), bound to the library
-    that ``load`` loads. There is no fallback."""
+    """The torch binding of the episode cache (built first if there is none of these sources, this torch and this
+    Python), bound to the library that ``load`` loads. There is no fallback."""
     global _TORCH
     if _TORCH is None:
-        path = _build.TORCH_LIB
-        try:
-            _build.build_torch()
-        except RuntimeError:
-            if not path.exists():
-                raise
-        spec = importlib.util.spec_from_file_location("_mkx_torch", path)
+        spec = importlib.util.spec_from_file_location("_mkx_torch", _build.build_torch())
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         lib = load()
-        module.bind(*(C.cast(getattr(lib, n), C.c_void_p).value
-                      for n in ("mkx_cache_plan", "mkx_cache_store", "mkx_cache_attend", "mkx_attend_workspace")))
+        if module.bind(lib.mkx_cache_key(), *(C.cast(getattr(lib, n), C.c_void_p).value for n in (
+                "mkx_cache_plan", "mkx_cache_store", "mkx_cache_attend", "mkx_attend_workspace"))) is not True:
+            raise ImportError(f"{lib_path()} and the torch binding were built from different versions of include/mkx_cache.h: "
+                              "run `python -m reki_megakernel_b200.build --force`")
         _TORCH = module
     return _TORCH
 

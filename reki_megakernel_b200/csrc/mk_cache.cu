@@ -440,6 +440,7 @@ int sm_count(int device) {
 using namespace mkxc;
 
 extern "C" const char* mkx_cache_last_cuda_error(void) { return last_error; }
+extern "C" unsigned long long mkx_cache_key(void) { return MKX_CACHE_KEY; }
 
 extern "C" mkx_status mkx_cache_plan(const mkx_plan_inputs* in, int device, cudaStream_t stream) {
   if (!in) return MKX_ERR_INVALID_ARG;

@@ -383,16 +383,18 @@ PyObject* error_code(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (addresses of mkx_cache_plan, mkx_cache_store, mkx_cache_attend, mkx_attend_workspace)
+// (mkx_cache_key of the library, addresses of mkx_cache_plan, mkx_cache_store, mkx_cache_attend, mkx_attend_workspace); None,
+// and nothing is bound, if the library was built from another mkx_cache.h
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  long long v[4];
-  if (n != 4) return none();
-  for (int i = 0; i < 4; ++i)
+  long long v[5];
+  if (n != 5) return none();
+  for (int i = 0; i < 5; ++i)
     if (!integer(a[i], v[i])) return none();
-  plan_fn = reinterpret_cast<decltype(plan_fn)>(v[0]);
-  store_fn = reinterpret_cast<decltype(store_fn)>(v[1]);
-  attend_fn = reinterpret_cast<decltype(attend_fn)>(v[2]);
-  workspace_fn = reinterpret_cast<decltype(workspace_fn)>(v[3]);
+  if ((unsigned long long)v[0] != MKX_CACHE_KEY) return none();
+  plan_fn = reinterpret_cast<decltype(plan_fn)>(v[1]);
+  store_fn = reinterpret_cast<decltype(store_fn)>(v[2]);
+  attend_fn = reinterpret_cast<decltype(attend_fn)>(v[3]);
+  workspace_fn = reinterpret_cast<decltype(workspace_fn)>(v[4]);
   Py_RETURN_TRUE;
 }
 

@@ -19,3 +19,36 @@ def test_prepare_refuses_sections_that_leave_dims_out():
                  (pos, None, table, (32,), False), (None, None, None, (8, 8), False), (None, table, table, None, True)):
         with pytest.raises(ValueError):
             check_position_args(d, *args)
+
+
+def test_no_binding_but_that_of_these_sources(monkeypatch):
+    """Another torch, Python or source has a binding of its own, and where that one cannot be built, none is loaded."""
+    import importlib.metadata
+    import shutil
+    from reki_megakernel_b200 import _lib, build
+    _lib.load_torch()
+    here = build.torch_lib()
+    assert here.exists() and here.suffix == ".so"
+    monkeypatch.setattr(_lib, "_TORCH", None)
+    monkeypatch.setattr(shutil, "which", lambda name: None)
+    assert _lib.load_torch() is not None            # it is there: nothing to build
+    monkeypatch.setattr(_lib, "_TORCH", None)
+    for change in ("torch", "source"):
+        with monkeypatch.context() as m:
+            if change == "torch":
+                m.setattr(importlib.metadata, "version", lambda name: "0.0.1")
+            else:
+                m.setattr(build, "TORCH_SOURCES", build.TORCH_SOURCES[1:])
+            assert build.torch_lib() != here
+            with pytest.raises(RuntimeError):
+                _lib.load_torch()
+            assert _lib._TORCH is None and here.exists()
+
+
+def test_binding_refuses_a_library_of_another_header():
+    from reki_megakernel_b200 import _lib, build
+    m, lib = _lib.load_torch(), _lib.load()
+    key = lib.mkx_cache_key()
+    assert key == build.cache_key() != 0
+    assert m.bind(key + 1, 8, 8, 8, 8) is None and m.bind(key, 8, 8, 8) is None and m.bind(0, 8, 8, 8, 8) is None
+    assert m.plan(*[torch.zeros(3)] * 8) is None    # and what was bound still is
