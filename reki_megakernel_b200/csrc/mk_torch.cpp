@@ -14,6 +14,7 @@
 #include <utility>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -43,6 +44,8 @@ bool tensor(PyObject* o, Tensor& t) {
 bool vector(const Tensor& t, int64_t n, at::ScalarType type, at::Device dev) {
   return t.scalar_type() == type && t.dim() == 1 && t.size(0) == n && t.device() == dev && t.is_contiguous();
 }
+// Whether autograd would expect this call in its graph: it records nothing.
+bool recorded(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
 bool page_size(int64_t n) { return n == 16 || n == 32 || n == 64 || n == 128 || n == 256; }
 bool half_type(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
 bool table_fits(const Tensor& t, int64_t b, int64_t page_rows, at::Device dev) {
@@ -193,6 +196,8 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
   } else if (a[8] != Py_None) {
     return none();
   }
+  for (const Tensor* t : {&k, &v, &kp, &vp, &q, &out})
+    if (recorded(*t)) return none();
   if (!strides(k, s2)) return none();
   p.k_row = s2[0];
   p.k_head = s2[1];
@@ -294,6 +299,8 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   } else if (!tensor(a[11], out) || out.sizes() != q.sizes() || out.scalar_type() != type || out.device() != dev) {
     return none();
   }
+  for (const Tensor* t : {&q, &kp, &vp, &out})
+    if (recorded(*t)) return none();
   mkx_attend_inputs p;
   std::memset(&p, 0, sizeof(p));
   long long s2[2], s3[3];

@@ -15,7 +15,8 @@ share one pool of pages. One step of serving is
 ``EpisodeCache`` keeps the pools, tables and counters of such a cache. ``rope_tables`` makes the
 cos / sin tables of the same positions for ``RegisterPrepare.run`` and ``ExpertMegakernel.run``. All
 calls are asynchronous on the current stream of the tensors' device and can be captured in a CUDA
-graph. There is no CPU fallback: the CUDA library must load. Inference only: nothing records gradients.
+graph. There is no CPU fallback: the CUDA library must load. Inference only: nothing records gradients, and a tensor that
+requires grad is refused unless ``torch.no_grad()`` says that none are wanted.
 """
 from __future__ import annotations
 
@@ -79,6 +80,14 @@ def _check_strides(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name}: the last dim must be contiguous")
     if t.data_ptr() % 16 or any(s % 8 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
         raise ValueError(f"{name}: rows, heads and pages must start on 16-byte boundaries")
+
+
+def _check_gradients(**tensors) -> None:
+    """Nothing here is differentiable: a tensor that requires grad is refused while gradients are recorded."""
+    if torch.is_grad_enabled():
+        for name, t in tensors.items():
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} requires grad, and no gradients are recorded: call under torch.no_grad(), or detach it")
 
 
 def _refused(what: str):
@@ -189,6 +198,7 @@ def check_write_args(k, v, slot, k_pages, v_pages, q, positions, out) -> None:
         if t.dtype != dtype or t.device != dev:
             raise ValueError(f"k_pages and v_pages must be {dtype} on {dev}")
     _vector(slot, "slot", rows, torch.int64, dev)
+    _check_gradients(k=k, v=v, k_pages=k_pages, v_pages=v_pages, q=q, out=out)
     if q is None:
         if out is not None:
             raise ValueError("out belongs to q")
@@ -266,6 +276,7 @@ def check_attend_args(q, k_pages, v_pages, table, length, start, max_rows, causa
         raise ValueError("scale must be finite")
     if out is not None and (out.shape != shape or out.dtype != dtype or out.device != dev):
         raise ValueError("out must be like q")
+    _check_gradients(q=q, k_pages=k_pages, v_pages=v_pages, out=out)
 
 
 def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, length: torch.Tensor,

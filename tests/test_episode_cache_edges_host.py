@@ -52,3 +52,22 @@ def test_binding_refuses_a_library_of_another_header():
     assert key == build.cache_key() != 0
     assert m.bind(key + 1, 8, 8, 8, 8) is None and m.bind(key, 8, 8, 8) is None and m.bind(0, 8, 8, 8, 8) is None
     assert m.plan(*[torch.zeros(3)] * 8) is None    # and what was bound still is
+
+
+def grad_cases(host, dev):
+    """(name, good arguments, names of the tensors that must not require grad)."""
+    return [("write", host.write_args(dev)[0], ("k", "v", "q", "k_pages", "v_pages")), ("attend", host.attend_args(dev)[0], ("q", "k_pages", "v_pages"))]
+
+
+def test_gradients_are_not_dropped_in_silence():
+    import test_episode_cache_host as host
+    from reki_megakernel_b200 import episode_cache as E
+    for name, good, floats in grad_cases(host, host.META):
+        check = getattr(E, f"check_{name}_args")
+        for arg in floats + ("out",):
+            t = torch.empty(7, 6, 64, dtype=host.BF, device=host.META) if arg == "out" else good[arg].clone()
+            kw = {**good, arg: t.requires_grad_(True)}
+            with pytest.raises(ValueError, match=f"{arg} requires grad"):
+                check(**kw)
+            with torch.no_grad():
+                check(**kw)

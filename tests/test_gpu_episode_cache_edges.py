@@ -119,3 +119,20 @@ def test_plans_of_two_threads():
     assert not failed
     for B in (4096, 2100):
         assert starts[B] == (list(range(B + 1)), [16 * b for b in range(B)], [B, B, 0])
+
+
+# ---- autograd ------------------------------------------------------------------------------------------
+
+def test_gradients_are_not_dropped_in_silence():
+    """A tensor that requires grad is refused by the calls while gradients are recorded, and taken under no_grad."""
+    import test_episode_cache_host as host
+    from test_episode_cache_edges_host import grad_cases
+    for name, good, floats in grad_cases(host, DEV):
+        f = {"write": ec().write_rows, "attend": ec().attend}[name]
+        for arg in floats:
+            kw = {**good, arg: good[arg].clone().requires_grad_(True)}
+            with pytest.raises(ValueError, match=f"{arg} requires grad"):
+                f(**kw)
+            with torch.no_grad():
+                assert not f(**kw).requires_grad
+    torch.cuda.synchronize()
