@@ -46,6 +46,11 @@ bool vector(const Tensor& t, int64_t n, at::ScalarType type, at::Device dev) {
 }
 // Whether autograd would expect this call in its graph: it records nothing.
 bool recorded(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
+// A tensor that a call has written in place: what autograd saved of it before is out of date. (Inference tensors are
+// not versioned.)
+void written(const Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 bool page_size(int64_t n) { return n == 16 || n == 32 || n == 64 || n == 128 || n == 256; }
 bool half_type(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
 bool table_fits(const Tensor& t, int64_t b, int64_t page_rows, at::Device dev) {
@@ -131,6 +136,9 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   p.rows = (int)rows;
   const mkx_status st = plan_fn(&p, dev.index(), stream_of(dev));
   if (st) return PyLong_FromLong(st);
+  written(table);
+  if (in_place)
+    for (const Tensor* t : {&length, &marks, &ticket}) written(*t);
   PyObject* out = PyTuple_New(6);
   if (!out) return nullptr;
   const Tensor* all[6] = {&start, &slot, &episode, &position, &after, &marks_after};
@@ -225,6 +233,7 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
   p.page_rows = (int)kp.size(1);
   const mkx_status st = store_fn(&p, dev.index(), stream_of(dev));
   if (st) return PyLong_FromLong(st);
+  for (const Tensor* t : {&kp, &vp, &out}) written(*t);
   if (!out.defined()) Py_RETURN_TRUE;
   if (a[8] != Py_None) return Py_NewRef(a[8]);
   return THPVariable_Wrap(out);
@@ -352,6 +361,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.workspace = space.data_ptr();
     const mkx_status st = attend_fn(&p, (size_t)space.numel(), dev.index(), stream);
     if (st) return PyLong_FromLong(st);
+    written(out);
   }
   if (a[11] != Py_None) return Py_NewRef(a[11]);
   return THPVariable_Wrap(out);

@@ -377,6 +377,9 @@ class EpisodeCache:
                                self.marks.data_ptr(), self._ticket.data_ptr(), self.episodes, self.table.shape[1],
                                self.free.shape[0], self.page_rows)
         _lib.check(_lib.load().mkx_cache_release(C.byref(a), self.device.index, _stream(self.device)), "mkx_cache_release")
+        for t in (self.length, self.table, self.free, self.marks, self._ticket):
+            if not t.is_inference():
+                torch.autograd.graph.increment_version(t)
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, plan: RowPlan, **kw):
         """``write_rows`` into the pages of ``layer``."""

@@ -136,3 +136,37 @@ def test_gradients_are_not_dropped_in_silence():
             with torch.no_grad():
                 assert not f(**kw).requires_grad
     torch.cuda.synchronize()
+
+
+def test_writes_in_place_are_seen_by_autograd():
+    """What a call writes in place has a new version, so that a backward pass that saved it refuses; inference tensors,
+    which have none, are taken as well."""
+    E = ec()
+
+    def changed(f, *tensors):
+        before = [t._version for t in tensors]
+        f()
+        return [t._version > b for t, b in zip(tensors, before)]
+
+    c = E.EpisodeCache(layers=2, pages=8, episodes=2, page_rows=16, kv_heads=2, pages_per_episode=4, device=DEV)
+    new = torch.ones(2, dtype=torch.int32, device=DEV)
+    x = torch.ones(2, 2, 64, dtype=BF, device=DEV)
+    plans = []
+    assert all(changed(lambda: plans.append(c.plan(new, 2)), c.table, c.length, c.marks))
+    pos = torch.arange(2, dtype=torch.int32, device=DEV)
+    q = x.clone()
+    assert all(changed(lambda: c.write(1, x, x, plans[0], q=q, positions=pos, out=q), c.k, c.v, q))
+    assert all(changed(lambda: c.attend(1, x, plans[0], out=q), q)) and changed(lambda: c.attend(1, x, plans[0]), c.k, c.v, x) == [False] * 3
+    w = torch.ones((), device=DEV, requires_grad=True)
+    loss = (c.k[1].float() * w * c.k[1].float()).sum() + (c.k[1] * w).sum()
+    c.write(1, x, x, plans[0])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    assert all(changed(lambda: c.release(torch.ones(2, dtype=torch.bool, device=DEV)), c.table, c.length, c.marks, c.free))
+    with torch.inference_mode():
+        i = E.EpisodeCache(layers=1, pages=8, episodes=2, page_rows=16, kv_heads=2, pages_per_episode=4, device=DEV)
+    plan = i.plan(new, 2)
+    i.write(0, x, x, plan)
+    i.attend(0, x, plan)
+    i.release(torch.ones(2, dtype=torch.bool, device=DEV))
+    torch.cuda.synchronize()
