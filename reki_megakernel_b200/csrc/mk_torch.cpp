@@ -284,6 +284,10 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !integer(a[9], sinks))
     return none();
   const int causal = PyObject_IsTrue(a[7]);
+  if (causal < 0) {  // it has no truth value
+    PyErr_Clear();
+    return none();
+  }
   double scale = 0;
   if (a[10] != Py_None) {
     scale = PyFloat_AsDouble(a[10]);
@@ -300,7 +304,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !page_size(kp.size(1)) || kp.size(2) < 1 || heads < 1 || heads % kp.size(2) || kp.scalar_type() != type ||
       kp.device() != dev || vp.scalar_type() != type || vp.device() != dev || b < 1 || b > MKX_MAX_EPISODES ||
       !vector(length, b, at::kInt, dev) || !vector(start, b + 1, at::kInt, dev) ||
-      !table_fits(table, b, kp.size(1), dev) || max_rows < -1 || window < 0 || sinks < 0 || causal < 0 ||
+      !table_fits(table, b, kp.size(1), dev) || max_rows < -1 || window < 0 || sinks < 0 ||
       (window > 0 && !causal) || (sinks > 0 && window == 0) || !std::isfinite(scale))
     return none();
   if (a[11] == Py_None) {

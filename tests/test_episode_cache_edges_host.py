@@ -71,3 +71,10 @@ def test_gradients_are_not_dropped_in_silence():
                 check(**kw)
             with torch.no_grad():
                 check(**kw)
+
+
+def test_binding_answers_none_to_a_flag_without_a_truth_value():
+    """It returned with Python's error set, which the interpreter makes a SystemError of."""
+    from reki_megakernel_b200 import _lib
+    x = torch.zeros(3)
+    assert _lib.load_torch().attend(x, x, x, x, x, x, 1, x, 0, 0, None, None) is None
