@@ -78,3 +78,12 @@ def test_binding_answers_none_to_a_flag_without_a_truth_value():
     from reki_megakernel_b200 import _lib
     x = torch.zeros(3)
     assert _lib.load_torch().attend(x, x, x, x, x, x, 1, x, 0, 0, None, None) is None
+
+
+def test_what_is_written_to_is_not_expanded():
+    from reki_megakernel_b200 import episode_cache as E
+    t = torch.zeros(7, 1, 64, dtype=torch.bfloat16).expand(7, 6, 64)
+    E._check_strides(t, "q")
+    E._check_strides(torch.zeros(7, 6, 64, dtype=torch.bfloat16)[:, :1].expand(7, 1, 64), "out", written=True)
+    with pytest.raises(ValueError, match="share a place"):
+        E._check_strides(t, "out", written=True)

@@ -170,3 +170,22 @@ def test_writes_in_place_are_seen_by_autograd():
     i.attend(0, x, plan)
     i.release(torch.ones(2, dtype=torch.bool, device=DEV))
     torch.cuda.synchronize()
+
+
+# ---- outputs that overlap ------------------------------------------------------------------------------
+
+def test_outputs_that_share_a_place_are_refused():
+    """An expanded tensor may be read (one row for all heads), not written to."""
+    import test_episode_cache_host as host
+    good = host.write_args(DEV)[0]
+    one = torch.ones(7, 1, 64, dtype=BF, device=DEV)
+    pool = torch.zeros(1, 32, 2, 64, dtype=BF, device=DEV)
+    wide = ec().write_rows(**{**good, "q": one.expand(7, 6, 64), "k": one.expand(7, 2, 64)})
+    assert wide.shape == (7, 6, 64) and (wide[:, 0] == wide[:, 5]).all()
+    for kw in (dict(out=one.clone().expand(7, 6, 64)), dict(k_pages=pool.expand(4, 32, 2, 64)), dict(v_pages=pool.expand(4, 32, 2, 64))):
+        with pytest.raises(ValueError, match="share a place"):
+            ec().write_rows(**{**good, **kw})
+    good = host.attend_args(DEV)[0]
+    with pytest.raises(ValueError, match="share a place"):
+        ec().attend(**{**good, "out": one.clone().expand(7, 6, 64)})
+    torch.cuda.synchronize()
