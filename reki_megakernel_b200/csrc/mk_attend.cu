@@ -1158,7 +1158,9 @@ bool encode_pages(CUtensorMap* m, const void* base, int dtype, int head_dim, int
   EncodeTiledFn fn = tensor_map_encoder();
   if (!fn) return false;
   const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)page_rows, (cuuint64_t)kv_heads, (cuuint64_t)pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)head * 2, (cuuint64_t)page * 2};
+  // a dim of size one has no stride of its own
+  const cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)(kv_heads > 1 ? head : head_dim) * 2,
+                                 (cuuint64_t)(pages > 1 ? page : head_dim) * 2};
   const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   return fn(m, dtype == MKX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
@@ -1250,6 +1252,10 @@ extern "C" mkx_status mkx_cache_attend(const mkx_attend_inputs* in, size_t works
                                a.vp_page, a.vp_row, a.vp_head};
   for (long long s : strides)
     if (s < 0 || s % 8 != 0 || s >= (1ll << 38)) return MKX_ERR_INVALID_ARG;
+  // a tensor map's strides are not zero
+  if ((a.pages > 1 && (a.kp_page == 0 || a.vp_page == 0)) || a.kp_row == 0 || a.vp_row == 0 ||
+      (a.kv_heads > 1 && (a.kp_head == 0 || a.vp_head == 0)))
+    return MKX_ERR_INVALID_ARG;
   const void* pointers[] = {a.q, a.out, a.k_pages, a.v_pages, a.workspace};
   for (const void* q : pointers)
     if ((reinterpret_cast<uintptr_t>(q) & 15) != 0) return MKX_ERR_INVALID_ARG;

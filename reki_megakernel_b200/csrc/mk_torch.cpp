@@ -58,15 +58,16 @@ bool table_fits(const Tensor& t, int64_t b, int64_t page_rows, at::Device dev) {
          t.is_contiguous() && t.size(1) * page_rows <= MAX_ROWS;
 }
 // Strides of the leading dims; dims contiguous, everything else on 16-byte boundaries. A dim of size one has
-// no stride of its own. What is written to has no stride of zero: several rows would share a place.
-enum Use { READ, WRITTEN };
+// no stride of its own. Where rows lie apart no stride is zero: what is written to
+// (several rows would share a place), and pages that a tensor map describes.
+enum Use { SHARED, APART };
 template <int N>
 bool strides(const Tensor& t, long long (&out)[N], Use use) {
   if (t.size(N) > 1 && t.stride(N) != 1) return false;
   if (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) return false;
   for (int i = 0; i < N; ++i) {
     out[i] = t.size(i) > 1 ? t.stride(i) : t.size(N);
-    if (out[i] & 7 || (use == WRITTEN && out[i] == 0)) return false;
+    if (out[i] & 7 || (use == APART && out[i] == 0)) return false;
   }
   return true;
 }
@@ -193,11 +194,11 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
     } else if (!tensor(a[8], out) || out.sizes() != q.sizes() || out.scalar_type() != type || out.device() != dev) {
       return none();
     }
-    if (!strides(q, s2, READ)) return none();
+    if (!strides(q, s2, SHARED)) return none();
     p.q = q.data_ptr();
     p.q_row = s2[0];
     p.q_head = s2[1];
-    if (!strides(out, s2, WRITTEN)) return none();
+    if (!strides(out, s2, APART)) return none();
     p.q_out = out.data_ptr();
     p.qo_row = s2[0];
     p.qo_head = s2[1];
@@ -207,17 +208,17 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   for (const Tensor* t : {&k, &v, &kp, &vp, &q, &out})
     if (recorded(*t)) return none();
-  if (!strides(k, s2, READ)) return none();
+  if (!strides(k, s2, SHARED)) return none();
   p.k_row = s2[0];
   p.k_head = s2[1];
-  if (!strides(v, s2, READ)) return none();
+  if (!strides(v, s2, SHARED)) return none();
   p.v_row = s2[0];
   p.v_head = s2[1];
-  if (!strides(kp, s3, WRITTEN)) return none();
+  if (!strides(kp, s3, APART)) return none();
   p.kp_page = s3[0];
   p.kp_row = s3[1];
   p.kp_head = s3[2];
-  if (!strides(vp, s3, WRITTEN)) return none();
+  if (!strides(vp, s3, APART)) return none();
   p.vp_page = s3[0];
   p.vp_row = s3[1];
   p.vp_head = s3[2];
@@ -318,17 +319,17 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   mkx_attend_inputs p;
   std::memset(&p, 0, sizeof(p));
   long long s2[2], s3[3];
-  if (!strides(q, s2, READ)) return none();
+  if (!strides(q, s2, SHARED)) return none();
   p.q_row = s2[0];
   p.q_head = s2[1];
-  if (!strides(out, s2, WRITTEN)) return none();
+  if (!strides(out, s2, APART)) return none();
   p.o_row = s2[0];
   p.o_head = s2[1];
-  if (!strides(kp, s3, READ)) return none();
+  if (!strides(kp, s3, APART)) return none();
   p.kp_page = s3[0];
   p.kp_row = s3[1];
   p.kp_head = s3[2];
-  if (!strides(vp, s3, READ)) return none();
+  if (!strides(vp, s3, APART)) return none();
   p.vp_page = s3[0];
   p.vp_row = s3[1];
   p.vp_head = s3[2];

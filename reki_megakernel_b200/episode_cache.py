@@ -74,15 +74,15 @@ def _stream(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def _check_strides(t: torch.Tensor, name: str, written: bool = False) -> None:
+def _check_strides(t: torch.Tensor, name: str, apart: bool = False) -> None:
     """Dims must be contiguous, rows, heads and pages 16 bytes apart or a multiple, and the start 16-byte aligned. What is
-    written to is no expanded tensor."""
+    written to, and the pages that attend reads by TMA, are no expanded tensors (``apart``)."""
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name}: the last dim must be contiguous")
     if t.data_ptr() % 16 or any(s % 8 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
         raise ValueError(f"{name}: rows, heads and pages must start on 16-byte boundaries")
-    if written and any(s == 0 for s, n in zip(t.stride(), t.shape) if n > 1):
-        raise ValueError(f"{name} is written to, and several of its rows or heads share a place")
+    if apart and any(s == 0 for s, n in zip(t.stride(), t.shape) if n > 1):
+        raise ValueError(f"{name} must not be expanded: several of its rows, heads or pages share a place")
 
 
 def _check_gradients(**tensors) -> None:
@@ -238,7 +238,7 @@ def write_rows(k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, k_pages: to
             _positions(positions, axes, k.shape[0], k.device)
         for name, t in (("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages), ("q", q), ("out", out)):
             if t is not None:
-                _check_strides(t, name, written=name in ("k_pages", "v_pages", "out"))
+                _check_strides(t, name, apart=name in ("k_pages", "v_pages", "out"))
         raise _refused("write_rows")
     if type(r) is int:
         _lib.check(r, "mkx_cache_store")
@@ -304,7 +304,7 @@ def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table:
         check_attend_args(q, k_pages, v_pages, table, length, start, max_rows, causal, window, sinks, scale, out)
         for name, t in (("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("out", out)):
             if t is not None:
-                _check_strides(t, name, written=name == "out")
+                _check_strides(t, name, apart=name != "q")
         raise _refused("attend")
     if r is False:
         raise RuntimeError("call attend once on this device before its first capture")

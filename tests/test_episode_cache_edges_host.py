@@ -80,10 +80,19 @@ def test_binding_answers_none_to_a_flag_without_a_truth_value():
     assert _lib.load_torch().attend(x, x, x, x, x, x, 1, x, 0, 0, None, None) is None
 
 
+def test_c_attend_refuses_pages_without_a_stride():
+    import ctypes as C
+    import test_episode_cache_host as host
+    from reki_megakernel_b200 import _lib
+    for name in ("kp_page", "vp_page", "kp_row", "vp_row", "kp_head", "vp_head"):
+        a = host._attend_inputs(**{name: 0})
+        assert _lib.load().mkx_cache_attend(C.byref(a), 1 << 30, 0, None) == _lib.MKX_ERR_INVALID_ARG
+
+
 def test_what_is_written_to_is_not_expanded():
     from reki_megakernel_b200 import episode_cache as E
     t = torch.zeros(7, 1, 64, dtype=torch.bfloat16).expand(7, 6, 64)
     E._check_strides(t, "q")
-    E._check_strides(torch.zeros(7, 6, 64, dtype=torch.bfloat16)[:, :1].expand(7, 1, 64), "out", written=True)
+    E._check_strides(torch.zeros(7, 6, 64, dtype=torch.bfloat16)[:, :1].expand(7, 1, 64), "out", apart=True)
     with pytest.raises(ValueError, match="share a place"):
-        E._check_strides(t, "out", written=True)
+        E._check_strides(t, "out", apart=True)

@@ -175,7 +175,7 @@ def test_writes_in_place_are_seen_by_autograd():
 # ---- outputs that overlap ------------------------------------------------------------------------------
 
 def test_outputs_that_share_a_place_are_refused():
-    """An expanded tensor may be read (one row for all heads), not written to."""
+    """An expanded tensor may be read (one row for all heads), but not written to, nor be the pages of attend."""
     import test_episode_cache_host as host
     good = host.write_args(DEV)[0]
     one = torch.ones(7, 1, 64, dtype=BF, device=DEV)
@@ -186,6 +186,10 @@ def test_outputs_that_share_a_place_are_refused():
         with pytest.raises(ValueError, match="share a place"):
             ec().write_rows(**{**good, **kw})
     good = host.attend_args(DEV)[0]
-    with pytest.raises(ValueError, match="share a place"):
-        ec().attend(**{**good, "out": one.clone().expand(7, 6, 64)})
+    for kw in (dict(out=one.clone().expand(7, 6, 64)), dict(k_pages=pool.expand(4, 32, 2, 64)), dict(v_pages=pool[:, :, :1].expand(1, 32, 2, 64))):
+        kw = {**good, **kw}
+        if kw["v_pages"].shape[0] == 1:
+            kw["k_pages"] = pool
+        with pytest.raises(ValueError, match="share a place"):
+            ec().attend(**kw)
     torch.cuda.synchronize()
