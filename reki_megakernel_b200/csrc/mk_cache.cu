@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(NT) release_kernel(const __grid_constant__ mkx
 // within half a turn, so cos and sin are as exact for a position of a million as for a small one
 // (fp32 angles would be off by 0.03 rad there).
 struct Rates {
-  float hi[128], lo[128];  // rate = base^(-i / half) / (2 pi)
+  float hi[128], lo[128];  // rate = base^(-i / half) / (2 pi), at most half a turn
   unsigned char axis[128];
   int half;
 };
@@ -379,7 +379,7 @@ bool same_rotary(const mkx_rotary& a, const mkx_rotary& b) {
 }
 
 bool rotary_fits(const mkx_rotary& r, int head_dim) {
-  if (!(r.base > 0.0) || !std::isfinite(r.base) || r.axes < 1 || r.axes > MKX_MAX_AXES) return false;
+  if (!(r.base > 0.0) || !std::isfinite(r.base) || !std::isfinite(1.0 / r.base) || r.axes < 1 || r.axes > MKX_MAX_AXES) return false;
   int half = 0;
   for (int i = 0; i < r.axes; ++i) {
     if (r.sections[i] < 0 || r.sections[i] > 128) return false;
@@ -406,7 +406,8 @@ const Rates& rates_of(const mkx_rotary& r) {
     rates.axis[i] = (unsigned char)axis;
     --left[axis];
     if (r.interleaved) axis = (axis + 1) % r.axes;
-    const double rate = std::pow(r.base, -(double)i / half) / (2.0 * 3.14159265358979323846);
+    double rate = std::pow(r.base, -(double)i / half) / (2.0 * 3.14159265358979323846);
+    rate -= std::nearbyint(rate);  // positions are whole, and so are these turns (a base below 1 has such rates)
     rates.hi[i] = (float)rate;
     rates.lo[i] = (float)(rate - (double)rates.hi[i]);
   }

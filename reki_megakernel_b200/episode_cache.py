@@ -146,7 +146,7 @@ def _rotary(head_dim: int, sections, base: float, interleaved: bool):
     half = sum(sections)
     if not 1 <= len(sections) <= 4 or min(sections) < 0 or half < 8 or half % 8 or 2 * half > head_dim:
         raise ValueError(f"sections must be 1 to 4 counts whose sum is a multiple of 8 up to {head_dim // 2}")
-    if not (base > 0 and math.isfinite(base)):
+    if not (base > 0 and math.isfinite(base) and math.isfinite(1 / base)):
         raise ValueError("base must be positive")
     return _lib.pack_rotary(base, len(sections), *sections, *(0,) * (4 - len(sections)), int(interleaved)), len(sections)
 

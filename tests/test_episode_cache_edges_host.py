@@ -96,3 +96,10 @@ def test_what_is_written_to_is_not_expanded():
     E._check_strides(torch.zeros(7, 6, 64, dtype=torch.bfloat16)[:, :1].expand(7, 1, 64), "out", apart=True)
     with pytest.raises(ValueError, match="share a place"):
         E._check_strides(t, "out", apart=True)
+
+
+def test_rotary_refuses_a_base_without_an_inverse():
+    from reki_megakernel_b200 import episode_cache as E
+    E._rotary(64, (32,), 1e-300, False)
+    with pytest.raises(ValueError):
+        E._rotary(64, (32,), 1e-310, False)

@@ -86,6 +86,19 @@ def test_prepare_turns_k_by_its_positions():
     rp.close()
 
 
+@pytest.mark.parametrize("base", [1.0, 0.3, 1e-4, 1e-6])
+def test_rope_tables_of_a_base_up_to_one(base):
+    """Frequencies of many turns a position. 2e-6 as for any base; the rates in 64 bits, here and in the oracle, are off by
+    two units of 2^-53 of the angle each (a power, a quotient)."""
+    g = torch.Generator().manual_seed(0)
+    pos = torch.randint(10 ** 6 - 5000, 10 ** 6, (1, 77), generator=g).to(torch.int32)
+    cos, sin = ec().rope_tables(pos.to(DEV), 64, base=base)
+    ang = angles_oracle(pos, (32,), base=base)
+    tol = 2e-6 + 4 * 2.0 ** -53 * float(ang.abs().max())
+    assert (cos.cpu().double() - torch.cat([ang.cos()] * 2, 1)).abs().max() <= tol
+    assert (sin.cpu().double() - torch.cat([ang.sin()] * 2, 1)).abs().max() <= tol
+
+
 # ---- several threads -----------------------------------------------------------------------------------
 
 def test_plans_of_two_threads():
