@@ -52,6 +52,64 @@ def test_attend_queries_not_finite(value, window, sinks, hd, extra_width):
     assert bool(((got - ref).abs() <= tol)[~spoilt].all())
 
 
+# ---- parts of split tiles ------------------------------------------------------------------------------
+
+def _stripes(c, page):
+    """V in head_dim stretches of an episode's keys, each 1 in a dim of its own: every output dim is the weight of one
+    stretch, so that a part of a tile that is lost, or counted twice, shows in it."""
+    hd = c["q"].shape[2]
+    for b, n in enumerate(c["length"].tolist()):
+        j = torch.arange(n, device=DEV)
+        v = torch.nn.functional.one_hot(j * hd // n, hd).to(c["v_pages"].dtype)
+        c["v_pages"][c["table"][b, :-(-n // page)].long()[j // page], j % page] = v[:, None].expand(n, c["v_pages"].shape[2], hd)
+    return c
+
+
+def _check_stripes(got, c, **kw):
+    """Half a step of the output and of each weight, 2^-12 for scores and exponentials as everywhere; what fp16 drops of a
+    key is below 2^-32 of the largest weight (lifted by 2^7 or more). No term grows with the keys in bf16."""
+    ref, weight = attend_oracle(**c, **kw)
+    u = torch.finfo(c["q"].dtype).eps / 2
+    lost = int(c["length"].max()) * 2.0 ** -32 if c["q"].dtype == FP else 2.0 ** -133
+    tol = u * ref.abs() + (u + 2.0 ** -12) * weight + lost
+    err = (got.double() - ref).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
+# 16-row tiles in up to 26 parts, in more; chunks in a few parts, in more than 12 (joined in two levels); those of the
+# tests of determinism and of two streams
+SPLIT = pytest.mark.parametrize("heads,kv,hd,page,new,past", [
+    (12, 12, 64, 32, [1], [20000]), (16, 2, 128, 128, [1], [60000]), (16, 8, 128, 64, [1, 1, 3], [38000, 17, 9000]),
+    (4, 1, 64, 256, [1], [70000]), (16, 8, 128, 256, [40], [38000]), (8, 1, 64, 128, [100], [50000]),
+    (32, 8, 128, 64, [300], [9000]), (12, 4, 64, 32, [500, 33, 200], [7000, 3000, 0]),
+    (8, 2, 128, 64, [1, 1], [8999, 4999]), (8, 2, 128, 64, [200], [5800]), (8, 2, 64, 64, [180], [5820])])
+
+
+@SPLIT
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_attend_counts_every_part_once(heads, kv, hd, page, new, past, dtype):
+    c = _stripes(pages_for(new, past, heads, kv, hd, page=page, dtype=dtype, seed=5, q_scale=0.7, extra_width=1), page)
+    for kw in (dict(), dict(causal=False), dict(window=max(past) // 2, sinks=300)):
+        want = ec().attend(**c, max_rows=max(new), **kw)
+        ec().check_device_error(DEV)
+        _check_stripes(want, c, **kw)
+        for _ in range(3):      # whichever block comes last
+            assert torch.equal(ec().attend(**c, max_rows=max(new), **kw), want)
+
+
+def test_stripes_show_a_lost_part():
+    """The check above with one stretch of 1024 of 38,001 keys left out, or counted twice, on the oracle's side."""
+    c = _stripes(pages_for([1], [38000], 4, 2, 128, page=256, seed=5, q_scale=0.7), 256)
+    got = ec().attend(**c)
+    _check_stripes(got, c)
+    for factor in (0.0, 2.0):
+        ids = c["table"][0, 40:44].long()
+        spoilt = dict(c, v_pages=c["v_pages"].clone())
+        spoilt["v_pages"][ids] *= factor
+        with pytest.raises(AssertionError):
+            _check_stripes(got, spoilt)
+
+
 # ---- rotary geometries ---------------------------------------------------------------------------------
 
 def test_prepare_turns_k_by_its_positions():
