@@ -111,7 +111,11 @@ mkx_status mkx_cache_store(const mkx_store_inputs* in, int device, cudaStream_t 
  * sees the rows j < length[b] with (not causal, or j <= p) and (window == 0, or j > p - window, or
  * j < sinks):
  *   out[row, h] = sum_j softmax_j(scale * q[row, h] . k[j, h / group]) v[j, h / group],  group = heads / kv_heads
- * and zero where a row sees nothing. Sums, maxima and outputs are held in fp32 and rounded once; what a
+ * and zero where a row sees nothing. Scores, maxima and sums are held in fp32, outputs rounded once; the
+ * probabilities exp(score - maximum) enter the second product as two 16-bit words (2^-16 of each in bf16, 2^-22 in
+ * fp16) or, in the kernel of long chunks, as one (2^-8, 2^-11; the sum that they are divided by is of the unrounded
+ * ones). Which of the two a call of more than 16 rows of a K/V head takes goes by max_rows and table_width, so the same
+ * row may differ in its last bits between calls that differ in those; the same call repeats itself. What a
  * K/V page holds beyond an episode's length, and pages that no row sees, do not matter, whatever they
  * hold; K and V rows below the length are finite. Table entries outside 0 .. pages - 1 read as zero rows.
  * A row of a head that sees a score of NaN or +inf, or only scores of -inf, is NaN there.

@@ -11,8 +11,8 @@
 // warps each take a quarter of a block's keys with mma.sync m16n8k16 (tcgen05 needs 128 rows to a tile,
 // of which a single row of 4 heads would fill 4) and keep their own running maximum and sum, joined once
 // at the end; long caches are split over blocks, the last part to finish joins the tile in the order of
-// the parts. The probabilities enter the second product as the sum of two 16-bit words, so that it is
-// as exact as fp32 weights; the tensor pipe is idle enough for that here.
+// the parts. The probabilities enter the second product as the sum of two 16-bit words, so that a weight
+// is off by 2^-16 (bf16; fp16 2^-22) where one word has 2^-8 (2^-11); the tensor pipe is idle enough for that here.
 // Two blocks per SM with three stages each. 96 single rows after 4,170 rows each, 32/8 heads x 128
 // (1641 MB): 268 us, 6.1 TB/s; 10 rows of 128 episodes of 470, 12 heads x 64, not causal (192 MB): 43 us, 4.5 TB/s
 // -- 3 us to the first bytes, and stretches end up to 10 % apart, since the SMs get unequal shares of HBM.
@@ -423,11 +423,13 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
 // 64 P has columns of its own, and the next scores are there before the last ones are done.
 // Bound by the exponentials at head_dim 64 (16 a clock per SM: 2048 clocks for two 128 x 128 tiles, whose
 // products take 1024), by both alike at 128; a quarter of them is taken off that unit (exp2_pair). What is
-// reached is 2950 to 3030 clocks for the two tiles at 128, where the softmax between two products of a
-// tile (load, maximum, exponentials, store) is a chain that the other tile's covers in part.
-// 2011 rows after 6007, 32/8 heads x 128 (231 GFLOP): 222 us by itself, 246 to 253 us in a long run under
-// the power cap (0.92 PFLOP/s); six chunks of 1,000 rows, window 1024 and 70 sinks, 12 heads x 64 (20
-// GFLOP): 64 us.
+// reached is 3850 clocks for the two tiles at 128 (2011 rows after 3007 to 12,007 keys: 1.96 us for each
+// further 128 keys of 256 rows at 1965 MHz, 2.24 at 1720), where the softmax between two products of a
+// tile (load, maximum, exponentials, store) is a chain that the other tile's covers in part. The start, Q, O,
+// parts and joins take some 60,000 clocks of a call beside it.
+// 2011 rows after 6007, 32/8 heads x 128 (231 GFLOP): 227 us in short runs, 246 to 253 us in a long one under
+// the power cap (0.92 PFLOP/s, 1.75 GHz); six chunks of 1,000 rows, window 1024 and 70 sinks, 12 heads x 64 (20
+// GFLOP): 64.6 us.
 constexpr int CT = 256;
 constexpr int CK = 128;
 constexpr int TILE_THREADS = 256;                   // warps 0-3 tile A, 4-7 tile B
@@ -1181,8 +1183,8 @@ struct Plan {
 // tile against 59 / 79 a million keys of a 16-row tile on the whole GPU, 25 against 8 for the launch, and 20 more where so
 // few tiles share the SMs that parts are joined twice. How long the caches are is not known here: what the tables can hold
 // stands for it. Beyond one 16-row tile, rows_kernel against chunk_kernel (us; episodes x rows per K/V head after keys, K/V
-// heads, head_dim): 1 x 32 after 4000, 12, 64: 14.9, 25.5; 1 x 64 after 4000: 16.0, 25.9; after 40000: 68.7, 55.5; 128 x 20
-// after 500: 79.7, 124.9; 64 x 32 after 4000: 360, 237; 8 x 32 after 8000, 8, 128: 91, 71; 1 x 32 after 100000, 1: 33, 62.
+// heads, head_dim): 1 x 32 after 4000, 12, 64: 13.8, 23.0; 1 x 64 after 4000: 14.3, 23.3; after 40000: 57.2, 54.1; 128 x 20
+// after 500: 71, 107; 64 x 32 after 4000: 291, 226; 8 x 32 after 8000, 8, 128: 97, 76; 1 x 32 after 100000, 1: 30, 61.
 bool chunk_is_faster(const mkx_attend_inputs& a, long long rows) {
   double keys = (double)a.table_width * a.page_rows;
   if (a.window > 0 && (double)a.window + a.sinks + a.max_rows < keys) keys = (double)a.window + a.sinks + a.max_rows;

@@ -278,7 +278,8 @@ __global__ void __launch_bounds__(256) tables_kernel(const __grid_constant__ Rat
 // A thread takes 8 dims and their 8 partners (16-byte accesses) of a row for up to HG heads of one of
 // q, k, v, and forms the 8 angles once for those heads. Bound by HBM: every row is read and written
 // once. The angles are reduced as above, and within half a turn __cosf and __sinf are off by 2^-21 at
-// most, 2^9 times finer than half a step of fp16; with sincospif, 20 more instructions an angle and 74
+// most: x cos - y sin is off by 2^-21 (|x| + |y|), 2^10 times finer than half a step of fp16 at that size (a result in
+// which the two nearly cancel is smaller, and off by as much); with sincospif, 20 more instructions an angle and 74
 // registers, the same calls take 128 instead of 118 us (30,011 rows of 32 + 8 + 8 heads x 128, 738 MB: 6.2
 // TB/s) and 10.0 instead of 8.2 (4096 rows of 3 x 12 heads x 64). With 8 heads (132 registers) they take 162 and
 // 14.1 us; 2 heads and sincospif, 174 and 11.3.

@@ -295,7 +295,8 @@ def attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table:
     zero for a row that sees nothing, NaN where a score is NaN or infinite; rows behind start[B] are left as they were. ``out`` may be q. What pages hold beyond an
     episode's length does not matter; the K and V rows below it are finite. ``max_rows``: no episode has more new rows
     (default: q's rows). The kernel is chosen by ``max_rows`` and by what a table row can hold, so tight values of both
-    pick the one that fits. A wait that ran out on the device surfaces in
+    pick the one that fits; that of long chunks (more than 16 rows of a K/V head) rounds each probability to 16 bits
+    before the second product, the other keeps twice as many. A wait that ran out on the device surfaces in
     ``check_device_error()``."""
     most = -1 if max_rows is None else max_rows if max_rows >= 0 else -2  # -1: q's rows; below: refused
     r = _lib.load_torch().attend(q, k_pages, v_pages, table, length, start, most, causal, window, sinks, scale, out)
