@@ -58,6 +58,19 @@ template <int DT>
 constexpr float ROWS_LIFT = DT == MKX_FP16 ? 15.f : 0.f;
 template <int DT>
 constexpr float CHUNK_LIFT = DT == MKX_FP16 ? 7.f : 0.f;
+// What is taken off the scores whose largest is `top`: top - LIFT, rounded up, since from 2^24 on it is a whole number of
+// units of a float, which the lift may not be; rounded down the largest weight would be 2^16, which fp16 does not have. A
+// row's maximum is kept in this form, so that sums of different blocks are lifted alike whatever the rounding.
+template <int DT>
+__device__ __forceinline__ float rows_base(float top) {
+  if constexpr (ROWS_LIFT<DT> == 0.f) return top;
+  return __fsub_ru(top, ROWS_LIFT<DT>);
+}
+template <int DT>
+__device__ __forceinline__ float chunk_base(float top) {
+  if constexpr (CHUNK_LIFT<DT> == 0.f) return top;
+  return __fsub_ru(top, CHUNK_LIFT<DT>);
+}
 
 template <int DT>
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -257,10 +270,10 @@ __global__ void __launch_bounds__(ROW_THREADS, 2)
       for (int x = 0; x < 2; ++x) {
         top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
         top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
-        const float now = fmaxf(m[x], top[x]), safe = now == -INFINITY ? 0.f : now;
-        fix[x] = ex2(m[x] - safe);
+        const float now = fmaxf(m[x], rows_base<DT>(top[x]));
+        top[x] = now == -INFINITY ? 0.f : now;
+        fix[x] = ex2(m[x] - top[x]);
         m[x] = now;
-        top[x] = safe - ROWS_LIFT<DT>;
         l[x] *= fix[x];
       }
 #pragma unroll
@@ -945,11 +958,11 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           for (int k = 0; k < 8; ++k)
             tops[k] = max_nan(tops[k], __uint_as_float(s[j >> 6][(j & 63) + k]), __uint_as_float(s[j >> 6][(j & 63) + k + 8]));
         // half of a block's probabilities, as words of P; their sum is added to `sums`
-        auto half_of = [&](const uint32_t (&sh)[64], float base, uint32_t (&w)[32], uint64_t (&sums)[4]) {
+        auto half_of = [&](const uint32_t (&sh)[64], uint64_t by, float base, uint32_t (&w)[32], uint64_t (&sums)[4]) {
           const uint64_t base2 = f2(-base, -base);
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const uint64_t y = fma2(f2(__uint_as_float(sh[2 * j]), __uint_as_float(sh[2 * j + 1])), scale2, base2);
+            const uint64_t y = fma2(f2(__uint_as_float(sh[2 * j]), __uint_as_float(sh[2 * j + 1])), by, base2);
             float2 v;
             if (j % S::POLY_EACH == S::POLY_EACH - 1) {
               v = exp2_pair<DT>(y);
@@ -965,14 +978,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         uint64_t sums[4] = {0, 0, 0, 0};
         const float top = p.scale_log2 *  // > 0: -inf stays
                           max_nan(max_nan(tops[0], tops[1], tops[2]), max_nan(tops[3], tops[4], tops[5]), max_nan(tops[6], tops[7]));
-        const bool grow = top > m + LAZY || (m == -INFINITY && top > m);
+        const float lifted = chunk_base<DT>(top);
+        const bool grow = lifted > __fadd_rd(m, LAZY);  // (rounded down: P stays below 2^8 as lifted)
         const bool any_grow = __any_sync(0xffffffffu, grow);
         if ((S::EARLY || any_grow) && n > n0) {  // the last V product: read P (EARLY) and wrote O
           wait(&sm.ofull[x], (n - 1) & 1);
           tmem_fence_after();
         }
         if (any_grow) {
-          const float now = grow ? top : m, fix = grow ? ex2(m - now) : 1.f;
+          const float now = grow ? lifted : m, fix = grow ? ex2(m - now) : 1.f;
           if (n > n0)
 #pragma unroll
             for (int j = 0; j < HD / 32; ++j) {
@@ -987,11 +1001,19 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         }
         // a score that is NaN or infinite makes the row NaN (exp2_pair would take it for a weight of zero)
         if (!(top < INFINITY)) l = __int_as_float(0x7fffffff);
-        const float base = (m == -INFINITY ? 0.f : m) - CHUNK_LIFT<DT>;
-        half_of(s[0], base, w, sums);
+        const float base = m == -INFINITY ? 0.f : m;
+        // Beyond 2^21 the fma's exact product is as much as a weight's exponent away from the rounded one that the maximum
+        // is: the scores are rounded first, as it was (finite weights for finite scores of any size)
+        uint64_t by = scale2;
+        if (__any_sync(0xffffffffu, fabsf(base) > 2097152.f)) {
+          by = f2(1.f, 1.f);
+#pragma unroll
+          for (int j = 0; j < 128; ++j) s[j >> 6][j & 63] = __float_as_uint(__uint_as_float(s[j >> 6][j & 63]) * p.scale_log2);
+        }
+        half_of(s[0], by, base, w, sums);
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-          if (part == 1) half_of(s[1], base, w, sums);
+          if (part == 1) half_of(s[1], by, base, w, sums);
           tmem_st32(pt + 32 * part, w);
           tmem_wait_st();
           tmem_fence_before();

@@ -52,6 +52,42 @@ def test_attend_queries_not_finite(value, window, sinks, hd, extra_width):
     assert bool(((got - ref).abs() <= tol)[~spoilt].all())
 
 
+# ---- scores of any size --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,bits", [(FP, b) for b in (0, 12, 20, 24, 25, 26, 27, 28, 30, 31)] + [(BF, b) for b in (0, 24, 28, 31, 36, 60, 100)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("hd", [64, 128])
+@WIDTHS
+def test_attend_scores_of_any_size(dtype, bits, sign, hd, extra_width):
+    """Finite queries and keys have a finite output, however large their scores: here sign * 2^bits * c of whole numbers c
+    up to 40, exact in fp32 (a factor of 2^6 of the sum over 64 dims, the others zero), so that equal scores stay equal and all
+    others are units apart. From 2^24 on a unit in the last place of a score is more than what the kernels shift it by. The rounding of
+    score x scale to fp32 is off by 2^-24 of it: 2^-18 at scores of 40, more where one key takes all."""
+    new, past = [40, 3, 150], [700, 0, 90]
+    c = pages_for(new, past, 4, 2, hd, page=32, dtype=dtype, seed=bits, extra_width=extra_width)
+    g = torch.Generator().manual_seed(bits)
+    n = c["k_pages"].shape[0]
+    k = torch.zeros(n, 32, 2, hd)
+    of_k = (bits - 6) // 2 if dtype == BF else min((bits - 6) // 2, 10)     # 40 * 2^10 and 2^15 are below 65504
+    k[..., :64] = sign * torch.randint(1, 41, (n, 32, 2, 1), generator=g).float() * 2.0 ** of_k
+    held = ~torch.isnan(c["k_pages"])
+    c["k_pages"] = torch.where(held, k.to(dtype).to(DEV), c["k_pages"])
+    c["q"] = torch.zeros_like(c["q"])
+    c["q"][..., :64] = 2.0 ** (bits - 6 - of_k)
+    assert torch.isfinite(c["q"]).all() and torch.isfinite(c["k_pages"][held]).all()
+    got = _attended(c, scale=1.0)
+    ref, weight = attend_oracle(**c, scale=1.0)
+    tol = attend_tolerance(ref, weight, dtype, 0)
+    assert bool(((got.double() - ref).abs() <= tol).all()), float(((got.double() - ref).abs() / tol).max())
+
+
+def _attended(c, **kw):
+    got = ec().attend(**c, **kw)
+    ec().check_device_error(DEV)
+    assert torch.isfinite(got.float()).all()
+    return got
+
+
 # ---- parts of split tiles ------------------------------------------------------------------------------
 
 def _stripes(c, page):
